@@ -55,7 +55,7 @@ extern "C" {
 /* Message of the last failing call on this thread ("" if none). */
 const char* pck_last_error(void);
 
-/* ABI version of this library (increases when a declaration here changes): 6. */
+/* ABI version of this library (increases when a declaration here changes, not when one is added): 6. */
 int pck_abi_version(void);
 
 /*
@@ -68,7 +68,8 @@ const char* pck_source_digest(void);
 
 /*
  * Device status word shared by every kernel of the library: bit 0 = a bounded wait gave up
- * (the result of that launch is not valid). Synchronizes the current device, stores the
+ * (the result of that launch is not valid); bit 1 = an index in device memory was out of range
+ * (serving operators; the access was left out). Synchronizes the current device, stores the
  * word in *status and, if `clear`, resets it.
  */
 int pck_device_status(unsigned int* status, int clear);
@@ -405,6 +406,91 @@ int pck_peer_close(void* ptr);
  * reference, which runs on one GPU).
  */
 int pck_peer_all_gather(const pck_peer_gather* gather, void* stream);
+
+/* ------------------------------------------------------------------------------------ */
+/* Serving operators of a decode step: 4-bit key/value cache, adapters, logits.            */
+
+/*
+ * The operators below have no counterpart in the reference and are not part of the trusted
+ * path. Element types are PCK_LOGITS_F32, _BF16 and _F16. Indices that they read from device
+ * memory (slots, pages, adapters, token ids) are checked by the kernels: a page, slot or
+ * adapter beyond its range is left out and sets bit 1 of pck_device_status.
+ *
+ * The 4-bit cache: `cache` is (pages, kv_heads, page_tiles, 18 * dim) bytes, contiguous and
+ * 16-byte aligned, dim 64, 128 or 256. A page holds 16 * page_tiles tokens of every head. A tile
+ * holds 16 of them: 8*dim bytes of key codes, dim bytes of key scales, then the same of the
+ * values. Each token's channels go in groups of 64 that share a (scale, zero) pair of bfloat16
+ * (scale first), stored by (token, group); an element is code * scale + zero. A byte holds the
+ * codes of channels c (low four bits) and c + 1. Code bytes go by planes of w = min(2, dim / 64)
+ * groups: key bytes by (plane, token, (c % 64) / 16, group, (c % 16) / 2), value bytes by (plane,
+ * token / 8, (c % 64) / 8, (token % 8) / 2, group, (c % 8) / 4, token % 2, (c % 4) / 2).
+ */
+
+/*
+ * Quantises `tokens` keys and values (row t, head h at x + t*token_stride + h*head_stride, dim
+ * contiguous elements of `dtype`) and writes them to their slots: slots[t] = page * 16 *
+ * page_tiles + token in the page, distinct, negative to write nothing. Per token, head and group:
+ * scale = bf16((max - min) * fl32(1/15)), zero = bf16(min), inv = fl32(1 / scale) (0 when scale
+ * < 2^-126), code = clamp(rint((x - zero) * inv), 0, 15), each step one binary32 operation. A
+ * group whose scale or zero is not finite (it held a NaN or an infinity) is stored as NaN (0x7fc0, codes 0). k_values
+ * and v_values (both or neither) get the values that the codes stand for, (tokens, kv_heads, dim)
+ * of `dtype`, whatever the slot.
+ */
+int pck_kv4_append(void* cache, int64_t pages, int64_t kv_heads, int64_t page_tiles, int64_t dim, const void* k,
+                   const void* v, int dtype, int64_t tokens, int64_t k_token_stride, int64_t k_head_stride,
+                   int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots, void* k_values, void* v_values,
+                   void* stream);
+
+/*
+ * Attention over the cache: q (batch, queries, heads, dim) bfloat16 or float16 by its strides (the
+ * last dimension contiguous), heads a multiple of kv_heads (head h reads key/value head h /
+ * (heads / kv_heads)). Request b holds lengths[b] tokens, the last `queries` of them the query
+ * tokens' own, in the pages page_table[b * table_stride ...] (table_pages columns; lengths beyond
+ * them are cut). Query token t sees the tokens j <= lengths[b] - queries + t, with window > 0 only
+ * the last `window` of them: out = softmax(scale * q k^T) v, (batch, queries, heads, dim) of q's
+ * type, contiguous. A query that sees no token gives zeros. `scratch` holds at least
+ * pck_kv4_attention_scratch(...) bytes (0: none needed), 256-byte aligned, of no meaning before
+ * and after the call.
+ */
+int64_t pck_kv4_attention_scratch(int64_t batch, int64_t queries, int64_t heads, int64_t kv_heads, int64_t dim,
+                                  int64_t max_tokens);
+int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_t queries, int64_t heads, int64_t dim,
+                      int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride, const void* cache,
+                      int64_t pages, int64_t kv_heads, int64_t page_tiles, const int32_t* page_table,
+                      int64_t table_stride, int64_t table_pages, const int32_t* lengths, double scale, int64_t window,
+                      void* out, void* scratch, int64_t scratch_bytes, void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection: out = y + s_a B_a (A_a x) for
+ * every row, a = adapters[row] (negative: none, out = y). x (tokens, n) bfloat16 or float16, A
+ * (count, rank, n) and B (count, m, rank) contiguous of x's type, y and out (tokens, m) binary32
+ * (out may be y). scales (count) may be NULL (1); ranks (count) gives each adapter's own rank in
+ * [0, rank] (the rest of A and B is not used) or is NULL. rank in [1, 256]. The intermediate A x is
+ * held in binary32.
+ */
+int pck_lora_add(const void* x, int dtype, int64_t tokens, int64_t n, int64_t x_stride, const float* y, int64_t m,
+                 int64_t y_stride, const void* A, const void* B, int64_t count, int64_t rank, const int32_t* adapters,
+                 const float* scales, const int32_t* ranks, float* out, int64_t out_stride, void* stream);
+
+/*
+ * Logits (rows, vocab) of `dtype` to binary32 `out` (which may be the logits), in this order, each
+ * step one binary32 operation:
+ *   repetition: l > 0 ? l / r : l * r for tokens in the row's history;
+ *   frequency:  l - f * (times put out) for tokens that were put out;
+ *   presence:   l - p for tokens that were put out;
+ *   bias:       l + the value of the last entry that names the token;
+ *   mask:       -inf where the token's bit (bit j % 32 of word j / 32) is 0, whatever l was.
+ * The history of row b is tokens[b * token_stride ...], lengths[b] ids (at most max_tokens), the
+ * first prompt_lengths[b] of them the prompt (NULL: none), the others put out by the model. Biases
+ * of row b are the entries [bias_starts[b], bias_starts[b + 1]) of bias_ids and bias_values
+ * (`biases` entries in all). Ids outside the vocabulary are skipped. tokens, each penalty (rows),
+ * bias_starts and mask may be NULL.
+ */
+int pck_process_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                       const int64_t* tokens, int64_t token_stride, int64_t max_tokens, const int32_t* prompt_lengths,
+                       const int32_t* lengths, const float* repetition, const float* frequency, const float* presence,
+                       const int32_t* bias_starts, const int64_t* bias_ids, const float* bias_values, int64_t biases,
+                       const int32_t* mask, int64_t mask_stride, float* out, int64_t out_stride, void* stream);
 
 #ifdef __cplusplus
 }

@@ -22,6 +22,7 @@ from pck.cuda.sampling import (
     topk_sample,
     topp_select,
 )
+from pck.cuda.serving import kv4_append, kv4_attention, kv4_cache, lora_add, process_logits
 
 __all__ = [
     "DEFAULT_BLOCK",
@@ -40,7 +41,12 @@ __all__ = [
     "gemv_fp8",
     "gemv_naive",
     "gemv_tc",
+    "kv4_append",
+    "kv4_attention",
+    "kv4_cache",
+    "lora_add",
     "ops",
+    "process_logits",
     "quantize_fp8",
     "round_up_bf16",
     "tc_height",

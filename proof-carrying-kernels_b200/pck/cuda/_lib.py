@@ -96,6 +96,13 @@ _SIGNATURES = {
     "pck_peer_import": ([_p, ctypes.POINTER(_p)], _int),
     "pck_peer_close": ([_p], _int),
     "pck_peer_all_gather": ([ctypes.POINTER(PeerGather), _p], _int),
+    "pck_kv4_append": ([_p, _i64, _i64, _i64, _i64, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p], _int),
+    "pck_kv4_attention_scratch": ([_i64, _i64, _i64, _i64, _i64, _i64], _i64),
+    "pck_kv4_attention": ([_p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p,
+                           _f64, _i64, _p, _p, _i64, _p], _int),
+    "pck_lora_add": ([_p, _int, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p, _i64, _p], _int),
+    "pck_process_logits": ([_p, _int, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64,
+                            _p, _i64, _p], _int),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -125,7 +132,8 @@ def check(rc: int, what: str = "pck") -> None:
 
 
 def device_status(clear: bool = True) -> int:
-    """The device status word (bit 0: a bounded wait in a kernel gave up). Synchronizes."""
+    """The device status word (bit 0: a bounded wait in a kernel gave up; bit 1: a page, slot or
+    adapter index was out of range). Synchronizes."""
     value = ctypes.c_uint(0)
     check(library().pck_device_status(ctypes.byref(value), int(clear)), "pck_device_status")
     return int(value.value)
