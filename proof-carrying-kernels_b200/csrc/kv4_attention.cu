@@ -1,13 +1,40 @@
 // pck_kv4_attention: softmax(scale * q k^T) v over the keys and values of a 4-bit cache.
 //
-// One CTA per (request, key/value head, query token); its threads share the head's group of query
-// rows, one row after another: a chunk of keys, a thread each, for the scores; then a thread for
-// each channel over the chunk's values. Running maximum and sum in binary32.
+// Bound by memory: a decode step reads every code once for a few query rows, so the cache has to
+// come in at the HBM's rate and the work per code has to stay small. What that led to:
+//   - The query rows that share a key/value head (its group of heads, and the query tokens of a
+//     request) are the 8, 16 or 32 rows of one matrix product: a tile of 16 tokens is read and
+//     unpacked once for all of them. mma.sync takes the unpacked codes from registers; tcgen05
+//     would want them written to shared memory first, which alone would exceed its bandwidth at
+//     the rate of two codes a byte.
+//   - Codes are unpacked with a mask, a shift and an or: the four bits become the low mantissa bits
+//     of a 16-bit float. Scales never touch the codes: with k = code * s + z,
+//       q.k = sum over groups of s (q.code) + z sum(q),
+//     and for the values the weight p s of a token and group goes into the matrix product instead
+//     of p; sum of p z is added at the end.
+//   - Scores and sums are binary32. The weights p s are rounded to binary16 (11 bits, below the
+//     rounding of a bfloat16 output): they are first divided by a power of two that follows the
+//     size of the values' scales, so neither large nor small scales leave binary16's range.
+//   - The running maximum is raised only when a score passes it by 2^8 (weights then stay within
+//     2^8, which binary16 and the sums hold), so the accumulators are rarely rescaled and the
+//     common tile needs no exchange between lanes for it.
+//   - The tiles of all (request, head, row block) items form one line that is cut into equal parts,
+//     a CTA each, whatever the lengths: a part of an item leaves its sums in scratch memory and a
+//     second kernel (a programmatic dependent) joins them. A CTA's four warps take tiles in turn,
+//     each through its own ring of bulk copies.
+#include <algorithm>
+
 #include "kv4_layout.cuh"
 #include "serving_common.cuh"
 
 namespace pck {
 namespace {
+
+constexpr int kAttnWarps = 4;
+constexpr int kAttnThreads = kAttnWarps * kWarp;
+constexpr int kMinTiles = 8;        // tiles of a part, at least: two for each warp
+constexpr float kRaise = 8.0f;      // log2 by which a score may pass the running maximum
+constexpr int kJoinThreads = 256;
 
 struct AttentionArgs {
   const void* q;
@@ -18,114 +45,739 @@ struct AttentionArgs {
   int64_t table_stride;
   const int32_t* lengths;
   void* out;
-  float scale;
-  int64_t window;
-  int64_t max_tokens;  // page table columns * page tokens
+  float* sums;        // (2 * parts, rows, dim) unnormalised outputs of split items
+  float2* top_total;  // (2 * parts, rows): maximum (log2), sum of weights
+  float scale_log2;
+  int64_t batch;
+  int32_t window;
+  int32_t max_tokens;  // page table columns * page tokens
   int32_t queries, heads, kv_heads, page_tiles;
+  int32_t group;       // heads of a key/value head
+  int32_t row_blocks;  // blocks of rows of a (request, key/value head)
+  int32_t parts;       // most parts of the line of tiles
+  int32_t q_vector;    // q rows are 16-byte aligned
 };
 
-constexpr int kChunk = 128;
+struct Range {
+  int first;  // first tile
+  int tiles;
+};
 
-__device__ __forceinline__ float decode(uint8_t byte, int c, uint32_t pair) {
-  const float code = static_cast<float>((byte >> (c % 2 * 4)) & 15);
-  return code * bf16_lo(pair) + bf16_hi(pair);
+// Tiles that any query of request b sees.
+__device__ __forceinline__ Range request_tiles(const AttentionArgs& a, int64_t b) {
+  const int length = min(a.lengths[b], a.max_tokens);
+  if (length <= 0) return {0, 0};
+  int first = 0;
+  if (a.window > 0) first = max(0, max(0, length - a.queries) + 1 - a.window) / kKv4Tile;
+  return {first, (length - 1) / kKv4Tile - first + 1};
 }
 
-template <typename T, int kDim>
-__global__ void __launch_bounds__(kChunk) attention_kernel(const AttentionArgs a) {
-  __shared__ float q[kDim];
-  __shared__ float p[kChunk];
-  __shared__ const uint8_t* tiles[kChunk / kKv4Tile];
-  __shared__ float red[kChunk / kWarp];
-  const int64_t item = blockIdx.x;
-  const int t = static_cast<int>(item % a.queries);
-  const int kvh = static_cast<int>(item / a.queries % a.kv_heads);
-  const int64_t b = item / a.queries / a.kv_heads;
-  const int group = a.heads / a.kv_heads;
-  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
-  int64_t length = a.lengths[b];
-  length = length < 0 ? 0 : length > a.max_tokens ? a.max_tokens : length;
-  const int64_t last = length - a.queries + t;  // this row's own position
-  int64_t first = a.window > 0 && last + 1 > a.window ? last + 1 - a.window : 0;
-  constexpr int kPer = (kDim + kChunk - 1) / kChunk;
-  for (int r = 0; r < group; ++r) {
-    const int head = kvh * group + r;
-    __syncthreads();
-    for (int c = tid; c < kDim; c += kChunk) {
-      q[c] = to_float(static_cast<const T*>(a.q)[b * a.q_batch_stride + t * a.q_token_stride + head * a.q_head_stride + c]);
-    }
-    float top = -INFINITY, sum = 0.0f, acc[kPer] = {};
-    for (int64_t j0 = first / kChunk * kChunk; j0 <= last; j0 += kChunk) {
-      __syncthreads();
-      if (tid < kChunk / kKv4Tile) {
-        const int64_t tile = j0 / kKv4Tile + tid;
-        const uint8_t* at = nullptr;
-        if (tile * kKv4Tile <= last) {
-          const int64_t page = a.page_table[b * a.table_stride + tile / a.page_tiles];
-          if (page >= 0 && page < a.pages) {
-            at = a.cache + ((page * a.kv_heads + kvh) * a.page_tiles + tile % a.page_tiles) * kv4_tile_bytes(kDim);
-          } else {
-            report(kDevIndex);
-          }
-        }
-        tiles[tid] = at;
-      }
-      __syncthreads();
-      const uint8_t* tile = tiles[tid / kKv4Tile];
-      const int at = tid % kKv4Tile;
-      float s = -INFINITY;
-      if (tile && j0 + tid >= first && j0 + tid <= last) {
-        s = 0.0f;
-        for (int c = 0; c < kDim; ++c) {
-          const uint32_t pair = *reinterpret_cast<const uint32_t*>(tile + kv4_key_scale(kDim, at, c / kKv4Group));
-          s = fmaf(q[c], decode(tile[kv4_key_byte(kDim, at, c & ~1)], c, pair), s);
-        }
-        s *= a.scale;
-      }
-      float m = s;
-      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
-      if (lane == 0) red[warp] = m;
-      __syncthreads();
-      m = top;
-      for (int w = 0; w < kChunk / kWarp; ++w) m = fmaxf(m, red[w]);
-      const float keep = top == m ? 1.0f : expf(top - m);
-      top = m;
-      p[tid] = s == -INFINITY ? 0.0f : expf(s - top);
-      __syncthreads();
-      sum *= keep;
-      for (int j = 0; j < kChunk; ++j) sum += p[j];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int c = tid + i * kChunk;
-        acc[i] *= keep;
-        for (int j = 0; j < kChunk; ++j) {
-          if (c < kDim && p[j] != 0.0f) {
-            const uint8_t* from = tiles[j / kKv4Tile];
-            const int k = j % kKv4Tile;
-            const uint32_t pair = *reinterpret_cast<const uint32_t*>(from + kv4_value_scale(kDim, k, c / kKv4Group));
-            acc[i] = fmaf(p[j], decode(from[kv4_value_byte(kDim, k, c & ~1)], c, pair), acc[i]);
-          }
-        }
-      }
-    }
-    T* out = static_cast<T*>(a.out) + ((b * a.queries + t) * a.heads + head) * kDim;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int c = tid + i * kChunk;
-      if (c < kDim) out[c] = from_float<T>(sum == 0.0f ? 0.0f : acc[i] / sum);
-    }
-  }
+template <int kThreads>
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* shared) {
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+  __syncthreads();
+  if (threadIdx.x % kWarp == 0) shared[threadIdx.x / kWarp] = v;
+  __syncthreads();
+  v = 0;
+  for (int w = 0; w < kThreads / kWarp; ++w) v += shared[w];
+  return v;
+}
+
+// Parts the line of `total` tiles is cut into, and where part c begins.
+__device__ __forceinline__ int64_t part_count(const AttentionArgs& a, int64_t total) {
+  return max(int64_t{1}, min(static_cast<int64_t>(a.parts), total / kMinTiles));
+}
+__device__ __forceinline__ int64_t part_begin(int64_t total, int64_t parts, int64_t c) { return total * c / parts; }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 template <typename T>
-cudaError_t launch_attention(const AttentionArgs& a, int64_t batch, int dim, cudaStream_t stream) {
-  const int64_t blocks = batch * a.kv_heads * a.queries;
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const unsigned grid = static_cast<unsigned>(blocks);
-  if (dim == 64) attention_kernel<T, 64><<<grid, kChunk, 0, stream>>>(a);
-  if (dim == 128) attention_kernel<T, 128><<<grid, kChunk, 0, stream>>>(a);
-  if (dim == 256) attention_kernel<T, 256><<<grid, kChunk, 0, stream>>>(a);
-  return cudaGetLastError();
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+
+// Four pairs of codes of a 32-bit word, nibbles (i, i + 4), as the products take them. binary16: the
+// code - 8, exactly (1024 + n and 1024 + 16 n have their codes in the mantissa). bfloat16: the code +
+// 128, whose excess goes into the zero's term (kKeyBias), with no further operation per code.
+template <typename T>
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&out)[4]) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 low = __floats2half2_rn(1032.0f, 1032.0f);
+    const __half2 part = __floats2half2_rn(0.0625f, 0.0625f), high = __floats2half2_rn(-72.0f, -72.0f);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      uint32_t x = (w & 0x000f000fu) | 0x64006400u;
+      uint32_t y = (w & 0x00f000f0u) | 0x64006400u;
+      out[i] = half2_bits(__hsub2(*reinterpret_cast<__half2*>(&x), low));
+      out[i + 1] = half2_bits(__hfma2(*reinterpret_cast<__half2*>(&y), part, high));
+      w >>= 8;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  }
+}
+template <typename T>
+constexpr float kKeyBias = std::is_same_v<T, __half> ? 8.0f : -128.0f;
+
+template <int kWords>
+__device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t* p) {
+  if constexpr (kWords == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
+  }
+}
+
+// Rows 8: one eight-row half of a 16-row product (the other half is empty and its results are not
+// kept); 16, 32: one or two full products.
+template <typename T, int kDim, int kRows>
+struct Shape {
+  static constexpr int kGroups = kDim / kKv4Group;
+  static constexpr int kPlanes = kGroups > 2 ? kGroups / 2 : 1;
+  static constexpr int kWidth = kGroups > 1 ? 2 : 1;  // groups of a plane
+  static constexpr int kHalves = kRows / 8;           // rows of a lane: lane / 4 + 8 h
+  static constexpr int kBlocks = kRows > 16 ? 2 : 1;  // products
+  static constexpr int kTileBytes = kv4_tile_bytes(kDim);
+  // 32 rows or 256 channels take twice the registers: fewer CTAs run beside each other, with more slots.
+  static constexpr bool kWide = kRows == 32 || kDim == 256;
+  static constexpr int kSlots = kDim == 64 ? 8 : kDim == 128 ? (kWide ? 8 : 5) : 4;
+  static constexpr int kRing = kAttnWarps * kSlots * kTileBytes;
+  static constexpr int kSmem = kRing + 1024;
+  static_assert(kRing >= kAttnWarps * kRows * kDim * 4, "the warps' sums overlay the rings");
+};
+
+template <typename T, int kDim, int kRows>
+__global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2 : 4)
+    attention_kernel(const __grid_constant__ AttentionArgs a) {
+  using S = Shape<T, kDim, kRows>;
+  constexpr int kG = S::kGroups, kH = S::kHalves, kMB = S::kBlocks;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[kAttnWarps][S::kSlots];
+  __shared__ int64_t scan[kAttnWarps];
+  __shared__ int64_t found[2];
+  __shared__ float2 state[kAttnWarps][kRows];
+
+  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
+  const int row8 = lane / 4, quarter = lane % 4;
+  if (lane == 0) {
+    for (int s = 0; s < S::kSlots; ++s) mbar_init(&full[warp][s], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  allow_dependents();
+  wait_for_producers();
+
+  // Requests that hold nothing give zeros.
+  T* const out = static_cast<T*>(a.out);
+  const int64_t row_size = static_cast<int64_t>(a.queries) * a.heads * kDim;
+  for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (request_tiles(a, b).tiles == 0) {
+      for (int64_t i = tid; i < row_size; i += kAttnThreads) out[b * row_size + i] = from_float<T>(0.0f);
+    }
+  }
+
+  // This CTA's part of the line of tiles: items in the order (request, head, row block).
+  const int64_t items = static_cast<int64_t>(a.kv_heads) * a.row_blocks;  // of a request
+  int64_t mine = 0;
+  for (int64_t b = tid; b < a.batch; b += kAttnThreads) mine += request_tiles(a, b).tiles;
+  const int64_t total = block_sum<kAttnThreads>(mine, scan) * items;
+  const int64_t parts = part_count(a, total);
+  if (blockIdx.x >= parts) return;
+  const int64_t begin = part_begin(total, parts, blockIdx.x), end = part_begin(total, parts, blockIdx.x + 1);
+  if (begin >= end) return;
+  // The request in which it begins: its tiles hold `begin` between them.
+  int64_t carry = 0;
+  for (int64_t b0 = 0; b0 < a.batch; b0 += kAttnThreads) {
+    const int64_t b = b0 + tid;
+    const int64_t n = b < a.batch ? request_tiles(a, b).tiles : 0;
+    int64_t before = n;
+    for (int o = 1; o < kWarp; o <<= 1) {
+      const int64_t v = __shfl_up_sync(kFullMask, before, o);
+      if (lane >= o) before += v;
+    }
+    __syncthreads();
+    if (lane == kWarp - 1) scan[warp] = before;
+    __syncthreads();
+    before += carry - n;
+    for (int w = 0; w < kAttnWarps; ++w) {
+      if (w < warp) before += scan[w];
+      carry += scan[w];
+    }
+    if (n > 0 && before * items <= begin && begin < (before + n) * items) {
+      found[0] = b;
+      found[1] = before;
+    }
+  }
+  __syncthreads();
+  int64_t b = found[0];
+  int64_t base = found[1] * items;  // of request b on the line
+
+  uint8_t* const ring = smem + warp * S::kSlots * S::kTileBytes;
+  uint32_t phase = 0;  // parity bit of each slot
+  bool dead = false;   // a wait gave up
+  for (int64_t at = begin; at < end;) {
+    const Range range = request_tiles(a, b);
+    if (at >= base + range.tiles * items) {
+      base += range.tiles * items;
+      ++b;
+      continue;
+    }
+    const int64_t item = (at - base) / range.tiles;
+    const int offset = static_cast<int>((at - base) % range.tiles);
+    const int count = static_cast<int>(min(static_cast<int64_t>(range.tiles - offset), end - at));
+    const int kvh = static_cast<int>(item / a.row_blocks), block = static_cast<int>(item % a.row_blocks);
+    const bool whole = count == range.tiles;
+    const int length = min(a.lengths[b], a.max_tokens);
+    const int rows = a.queries * a.group;
+    const int row0 = block * kRows;
+    // Positions of the block's first and last query token, and the tiles that they see.
+    const int pos0 = length - a.queries + row0 / a.group;
+    const int pos1 = length - a.queries + (min(row0 + kRows, rows) - 1) / a.group;
+    int lo = range.first + offset, hi = lo + count;
+    if (a.window > 0) lo = max(lo, max(0, pos0 + 1 - a.window) / kKv4Tile);
+    hi = pos1 < 0 ? lo : min(hi, pos1 / kKv4Tile + 1);
+    const int warp_tiles = hi - lo > warp ? (hi - lo - warp + kAttnWarps - 1) / kAttnWarps : 0;
+
+    // This lane's rows: their positions, and q as the left operand with its channels in the order
+    // of the codes: for each 8 channels the pairs (0, 4), (1, 5), (2, 6), (3, 7).
+    int pos[kH];
+    uint32_t qf[kMB][kG * 4][4];
+    float qsum[kG][kH];
+#pragma unroll
+    for (int h = 0; h < (kH == 1 ? 1 : kH); ++h) {
+      const int r = row0 + row8 + 8 * h;
+      const int t = r / a.group;
+      pos[h] = r < rows ? length - a.queries + t : -1;
+      const T* qr = static_cast<const T*>(a.q) + b * a.q_batch_stride + t * a.q_token_stride +
+                    static_cast<int64_t>(kvh * a.group + r % a.group) * a.q_head_stride;
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        uint32_t x[8];
+        float sum = 0.0f;
+        if (r < rows) {
+          const T* from = qr + g * kKv4Group + 16 * quarter;
+          if (a.q_vector) {
+            *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(from);
+            *reinterpret_cast<uint4*>(x + 4) = *reinterpret_cast<const uint4*>(from + 8);
+          } else {
+            const uint16_t* u = reinterpret_cast<const uint16_t*>(from);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = u[2 * i] | static_cast<uint32_t>(u[2 * i + 1]) << 16;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint16_t u = static_cast<uint16_t>(x[i / 2] >> (16 * (i % 2)));
+            sum += to_float(*reinterpret_cast<const T*>(&u));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = 0;
+        }
+        sum += __shfl_xor_sync(kFullMask, sum, 1);
+        sum += __shfl_xor_sync(kFullMask, sum, 2);
+        qsum[g][h] = sum;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t* y = x + 4 * w;
+          uint32_t(*f)[4] = &qf[h / 2][g * 4 + 2 * w];
+          f[0][h % 2] = __byte_perm(y[0], y[2], 0x5410);
+          f[0][2 + h % 2] = __byte_perm(y[0], y[2], 0x7632);
+          f[1][h % 2] = __byte_perm(y[1], y[3], 0x5410);
+          f[1][2 + h % 2] = __byte_perm(y[1], y[3], 0x7632);
+        }
+      }
+    }
+    if constexpr (kH == 1) {
+#pragma unroll
+      for (int k = 0; k < kG * 4; ++k) qf[0][k][1] = qf[0][k][3] = 0;
+    }
+
+    float acc[kG][8][kH][2];  // [group][channel of 8][row][lanes' two channel octets]
+    float top[kH], total_w[kH], zeros[kG][kH];
+    uint32_t unit[kG];  // exponent field of the power of two that the values' weights are divided by
+    float inv[kG];
+#pragma unroll
+    for (int h = 0; h < kH; ++h) {
+      top[h] = -INFINITY;
+      total_w[h] = 0.0f;
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        zeros[g][h] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) acc[g][n][h][0] = acc[g][n][h][1] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+      unit[g] = 127;
+      inv[g] = 1.0f;
+    }
+
+    // The warp's k-th tile is lo + warp + 4 k. Its page: 32 of them are looked up at once, a lane
+    // each, one batch ahead of their use.
+    const int32_t* table = a.page_table + b * a.table_stride;
+    auto look_up = [&](int k) -> int32_t {
+      k += lane;
+      if (k >= warp_tiles) return -1;
+      const int32_t page = table[(lo + warp + k * kAttnWarps) / a.page_tiles];
+      if (page < 0 || page >= a.pages) {
+        report(kDevIndex);
+        return -1;
+      }
+      return page;
+    };
+    int32_t pages_now = look_up(0), pages_next = look_up(kWarp);
+    uint32_t missing = 0;  // slots whose tile has no page
+    auto issue = [&](int k, int slot) {
+      if (k % kWarp == 0 && k > 0) {
+        pages_now = pages_next;
+        pages_next = look_up(k + kWarp);
+      }
+      const int32_t page = __shfl_sync(kFullMask, pages_now, k % kWarp);
+      missing = page < 0 ? missing | 1u << slot : missing & ~(1u << slot);
+      if (lane == 0) {
+        if (page < 0) {
+          mbar_arrive(&full[warp][slot]);
+        } else {
+          const int tile = lo + warp + k * kAttnWarps;
+          const uint8_t* from = a.cache + ((static_cast<int64_t>(page) * a.kv_heads + kvh) * a.page_tiles +
+                                           tile % a.page_tiles) * S::kTileBytes;
+          mbar_arrive_expect_tx(&full[warp][slot], S::kTileBytes);
+          bulk_load(ring + slot * S::kTileBytes, from, S::kTileBytes, &full[warp][slot], policy_evict_first());
+        }
+      }
+    };
+    for (int s = 0; s < S::kSlots && s < warp_tiles; ++s) issue(s, s);
+
+    // One tile in registers and shared memory. kMasked: some row does not see some of its tokens.
+    auto tile_step = [&](const uint8_t* tile, int token0, auto masked_tag) {
+      constexpr bool kMasked = decltype(masked_tag)::value;
+      float s[2][kH][2];
+      bool off[2][kH][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float part[kG][kMB][4];
+#pragma unroll
+        for (int p = 0; p < S::kPlanes; ++p) {
+          uint32_t w[2 * S::kWidth];
+          load_words(w, tile + p * 512 * S::kWidth + (j * kWarp + lane) * 8 * S::kWidth);
+#pragma unroll
+          for (int i = 0; i < S::kWidth; ++i) {
+            const int g = p * S::kWidth + i;
+#pragma unroll
+            for (int m = 0; m < kMB; ++m) part[g][m][0] = part[g][m][1] = part[g][m][2] = part[g][m][3] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t k[4];
+              unpack<T>(w[2 * i + c], k);
+#pragma unroll
+              for (int m = 0; m < kMB; ++m) {
+                mma<T>(part[g][m], qf[m][g * 4 + 2 * c], k[0], k[1]);
+                mma<T>(part[g][m], qf[m][g * 4 + 2 * c + 1], k[2], k[3]);
+              }
+            }
+          }
+        }
+        // This lane's columns: tokens 8 j + 2 quarter and the next.
+        const uint32_t* pairs = reinterpret_cast<const uint32_t*>(tile + kv4_key_scale(kDim, 8 * j + 2 * quarter, 0));
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int h = 0; h < kH; ++h) s[j][h][c] = 0.0f;
+#pragma unroll
+          for (int g = 0; g < kG; ++g) {
+            const uint32_t pair = pairs[c * kG + g];
+            const float scale = bf16_lo(pair);
+            const float zero = fmaf(kKeyBias<T>, scale, bf16_hi(pair));
+#pragma unroll
+            for (int h = 0; h < kH; ++h) {
+              s[j][h][c] = fmaf(scale, part[g][h / 2][h % 2 * 2 + c], s[j][h][c]);
+              s[j][h][c] = fmaf(zero, qsum[g][h], s[j][h][c]);
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < kH; ++h) {
+            s[j][h][c] *= a.scale_log2;
+            if constexpr (kMasked) {
+              const int token = token0 + 8 * j + 2 * quarter + c;
+              off[j][h][c] = token > pos[h] || (a.window > 0 && token <= pos[h] - a.window);
+              if (off[j][h][c]) s[j][h][c] = -INFINITY;
+            }
+          }
+        }
+      }
+      // Raise the maximum where a score passes it by more than 2^kRaise.
+      bool pass = false;
+#pragma unroll
+      for (int h = 0; h < kH; ++h) {
+        const float m = fmaxf(fmaxf(s[0][h][0], s[0][h][1]), fmaxf(s[1][h][0], s[1][h][1]));
+        pass = pass || m > top[h] + kRaise;
+      }
+      if (__any_sync(kFullMask, pass)) {
+#pragma unroll
+        for (int h = 0; h < kH; ++h) {
+          float m = fmaxf(fmaxf(s[0][h][0], s[0][h][1]), fmaxf(s[1][h][0], s[1][h][1]));
+          m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 2));
+          m = fmaxf(m, top[h]);
+          const float keep = top[h] == m ? 1.0f : exp2_fast(top[h] - m);
+          top[h] = m;
+          total_w[h] *= keep;
+#pragma unroll
+          for (int g = 0; g < kG; ++g) {
+            zeros[g][h] *= keep;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+              acc[g][n][h][0] *= keep;
+              acc[g][n][h][1] *= keep;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < kH; ++h) {
+        const float m = top[h] == -INFINITY ? 0.0f : top[h];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            s[j][h][c] = exp2_fast(s[j][h][c] - m);
+            total_w[h] += s[j][h][c];
+          }
+        }
+      }
+      // The values: a group at a time, weights of its scales.
+#pragma unroll
+      for (int p = 0; p < S::kPlanes; ++p) {
+        uint32_t w[2][2 * S::kWidth];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          load_words(w[j], tile + 9 * kDim + p * 512 * S::kWidth + (j * kWarp + lane) * 8 * S::kWidth);
+        }
+#pragma unroll
+        for (int i = 0; i < S::kWidth; ++i) {
+          const int g = p * S::kWidth + i;
+          float scale[2][2], zero[2][2];
+          uint32_t largest = 0;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int token = 8 * j + 2 * quarter + c;
+              uint32_t pair = *reinterpret_cast<const uint32_t*>(tile + kv4_value_scale(kDim, token, g));
+              if constexpr (kMasked) {
+                if (token0 + token >= length) pair = 0;  // a place that nothing was written to
+              }
+              scale[j][c] = bf16_lo(pair);
+              zero[j][c] = fmaf(8.0f, scale[j][c], bf16_hi(pair));
+              largest = max(largest, pair << 16);
+            }
+          }
+          largest = __reduce_max_sync(kFullMask, largest);
+          // Keep the largest scale within 2^4 of the unit; a NaN scale leaves the unit alone.
+          const uint32_t field = largest >> 23;
+          if (field + 4 < unit[g] || field > unit[g] + 4) {
+            if (largest != 0 && field < 255) {
+              const uint32_t next = min(max(field, 1u), 253u);
+              const float ratio = __uint_as_float((254u - next) << 23) * __uint_as_float(unit[g] << 23);
+              unit[g] = next;
+              inv[g] = __uint_as_float((254u - next) << 23);
+#pragma unroll
+              for (int n = 0; n < 8; ++n) {
+#pragma unroll
+                for (int h = 0; h < kH; ++h) {
+                  acc[g][n][h][0] *= ratio;
+                  acc[g][n][h][1] *= ratio;
+                }
+              }
+            }
+          }
+          uint32_t wf[kMB][4] = {};
+#pragma unroll
+          for (int h = 0; h < kH; ++h) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float x[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                x[c] = s[j][h][c] * (scale[j][c] * inv[g]);
+                float z = s[j][h][c] * zero[j][c];
+                if constexpr (kMasked) {  // a NaN scale must not reach rows that do not see its token
+                  if (off[j][h][c]) x[c] = z = 0.0f;
+                }
+                zeros[g][h] += z;
+              }
+              wf[h / 2][2 * j + h % 2] = half2_bits(__floats2half2_rn(x[0], x[1]));
+            }
+          }
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            uint32_t v0[4], v1[4];
+            unpack<__half>(w[0][2 * i + d], v0);
+            unpack<__half>(w[1][2 * i + d], v1);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+#pragma unroll
+              for (int m = 0; m < kMB; ++m) {
+                float(*to)[2] = &acc[g][4 * d + n][2 * m];
+                if constexpr (kH == 1) {
+                  float r[4] = {to[0][0], to[0][1], 0.0f, 0.0f};
+                  mma<__half>(r, wf[m], v0[n], v1[n]);
+                  to[0][0] = r[0];
+                  to[0][1] = r[1];
+                } else {
+                  float r[4] = {to[0][0], to[0][1], to[1][0], to[1][1]};
+                  mma<__half>(r, wf[m], v0[n], v1[n]);
+                  to[0][0] = r[0];
+                  to[0][1] = r[1];
+                  to[1][0] = r[2];
+                  to[1][1] = r[3];
+                }
+              }
+            }
+          }
+        }
+      }
+    };
+
+    int slot = 0;
+    for (int k = 0; k < warp_tiles; ++k) {
+      if (!dead) dead = !mbar_wait(&full[warp][slot], phase >> slot & 1u);
+      phase ^= 1u << slot;
+      dead = __any_sync(kFullMask, dead);
+      if (!(missing >> slot & 1u) && !dead) {
+        const uint8_t* tile = ring + slot * S::kTileBytes;
+        const int token0 = (lo + warp + k * kAttnWarps) * kKv4Tile;
+        if (token0 + kKv4Tile - 1 <= pos0 && (a.window <= 0 || token0 > pos1 - a.window)) {
+          tile_step(tile, token0, std::false_type{});
+        } else {
+          tile_step(tile, token0, std::true_type{});
+        }
+      }
+      __syncwarp();
+      if (k + S::kSlots < warp_tiles && !dead) issue(k + S::kSlots, slot);
+      slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+    }
+
+    // Join the warps: their sums in shared memory (over the rings, which are empty now), then a
+    // thread for each element.
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int h = 0; h < kH; ++h) {
+      float l = total_w[h];
+      l += __shfl_xor_sync(kFullMask, l, 1);
+      l += __shfl_xor_sync(kFullMask, l, 2);
+      if (quarter == 0) state[warp][row8 + 8 * h] = make_float2(top[h], l);
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        float z = zeros[g][h];
+        z += __shfl_xor_sync(kFullMask, z, 1);
+        z += __shfl_xor_sync(kFullMask, z, 2);
+        const float u = __uint_as_float(unit[g] << 23);
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          float4* to = reinterpret_cast<float4*>(sums + (warp * kRows + row8 + 8 * h) * kDim + g * kKv4Group +
+                                                 8 * (2 * quarter + o));
+          to[0] = make_float4(fmaf(acc[g][0][h][o], u, z), fmaf(acc[g][1][h][o], u, z), fmaf(acc[g][2][h][o], u, z),
+                              fmaf(acc[g][3][h][o], u, z));
+          to[1] = make_float4(fmaf(acc[g][4][h][o], u, z), fmaf(acc[g][5][h][o], u, z), fmaf(acc[g][6][h][o], u, z),
+                              fmaf(acc[g][7][h][o], u, z));
+        }
+      }
+    }
+    __syncthreads();
+    const int64_t slot_id = 2 * static_cast<int64_t>(blockIdx.x) + (at == begin ? 0 : 1);
+    const int kept = min(kRows, rows - row0);
+    for (int i = tid; i < kept * kDim; i += kAttnThreads) {
+      const int r = i / kDim, c = i % kDim;
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) m = fmaxf(m, state[w][r].x);
+      float o = 0.0f, l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) {
+        const float f = state[w][r].x == -INFINITY ? 0.0f : exp2_fast(state[w][r].x - m);
+        o = fmaf(f, sums[(w * kRows + r) * kDim + c], o);
+        l = fmaf(f, state[w][r].y, l);
+      }
+      if (whole) {
+        const int t = (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
+        out[((b * a.queries + t) * a.heads + head) * kDim + c] = from_float<T>(l == 0.0f ? 0.0f : o / l);
+      } else {
+        a.sums[(slot_id * kRows + r) * kDim + c] = o;
+        if (c == 0) a.top_total[slot_id * kRows + r] = make_float2(m, l);
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next bulk copies land here
+    __syncthreads();
+    at += count;
+  }
+}
+
+// Joins the parts of split items: a CTA for each (request, head, row).
+template <typename T, int kDim, int kRows>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttentionArgs a) {
+  constexpr int kWarps = kJoinThreads / kWarp;
+  constexpr int kPer = kDim / kWarp;
+  extern __shared__ float weight[];
+  __shared__ int64_t scan[kWarps];
+  __shared__ float sums[kWarps][kDim];
+  __shared__ float red[2][kWarps];
+  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
+  const int rows = a.queries * a.group;
+  const int r = static_cast<int>(blockIdx.x % rows);
+  const int kvh = static_cast<int>(blockIdx.x / rows % a.kv_heads);
+  const int64_t b = blockIdx.x / rows / a.kv_heads;
+  const int64_t items = static_cast<int64_t>(a.kv_heads) * a.row_blocks;
+  wait_for_producers();
+  int64_t all = 0, before = 0;
+  for (int64_t i = tid; i < a.batch; i += kJoinThreads) {
+    const int64_t n = request_tiles(a, i).tiles;
+    all += n;
+    before += i < b ? n : 0;
+  }
+  const int64_t total = block_sum<kJoinThreads>(all, scan) * items;
+  before = block_sum<kJoinThreads>(before, scan);
+  const int64_t tiles = request_tiles(a, b).tiles;
+  if (tiles == 0) return;
+  const int64_t parts = part_count(a, total);
+  const int64_t first = before * items + (kvh * static_cast<int64_t>(a.row_blocks) + r / kRows) * tiles;
+  const int64_t last = first + tiles - 1;
+  // Parts that hold the item's first and last tile.
+  auto part_of = [&](int64_t x) {
+    int64_t c = x * parts / total;
+    while (c + 1 < parts && part_begin(total, parts, c + 1) <= x) ++c;
+    while (part_begin(total, parts, c) > x) --c;
+    return c;
+  };
+  const int64_t c0 = part_of(first), c1 = part_of(last);
+  if (c0 == c1) return;  // the attention kernel wrote the whole item
+  const int n = static_cast<int>(c1 - c0 + 1);
+  auto slot_of = [&](int i) { return 2 * (c0 + i) + (first <= part_begin(total, parts, c0 + i) ? 0 : 1); };
+  float m = -INFINITY;
+  for (int i = tid; i < n; i += kJoinThreads) m = fmaxf(m, a.top_total[slot_of(i) * kRows + r % kRows].x);
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
+  if (lane == 0) red[0][warp] = m;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red[0][w]);
+  float l = 0.0f;
+  for (int i = tid; i < n; i += kJoinThreads) {
+    const float2 v = a.top_total[slot_of(i) * kRows + r % kRows];
+    const float f = v.x == -INFINITY ? 0.0f : exp2_fast(v.x - m);
+    weight[i] = f;
+    l = fmaf(f, v.y, l);
+  }
+  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(kFullMask, l, o);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  l = 0.0f;
+  for (int w = 0; w < kWarps; ++w) l += red[1][w];
+  float o[kPer] = {};
+#pragma unroll 4
+  for (int i = warp; i < n; i += kWarps) {
+    const float* from = a.sums + (slot_of(i) * kRows + r % kRows) * kDim + lane;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) o[k] = fmaf(weight[i], from[k * kWarp], o[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) sums[warp][lane + k * kWarp] = o[k];
+  __syncthreads();
+  T* out = static_cast<T*>(a.out) + ((b * a.queries + r / a.group) * a.heads + kvh * a.group + r % a.group) * kDim;
+  for (int c = tid; c < kDim; c += kJoinThreads) {
+    float v = 0.0f;
+    for (int w = 0; w < kWarps; ++w) v += sums[w][c];
+    out[c] = from_float<T>(l == 0.0f ? 0.0f : v / l);
+  }
+}
+
+// Rows of a block: as many as the item has, up to 32 (16 with 256 channels, whose sums take the
+// registers of twice as many rows).
+int block_rows(int64_t rows, int64_t dim) { return rows <= 8 ? 8 : rows <= 16 || dim == 256 ? 16 : 32; }
+
+int sm_count() {
+  static int cache[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!cache[dev]) {
+    int v = 0;
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) v = 148;
+    cache[dev] = v;
+  }
+  return cache[dev];
+}
+
+// Most parts of a call: the CTAs that run at once, and no more than the longest lengths can fill.
+int64_t most_parts(int64_t batch, int64_t queries, int64_t group, int64_t kv_heads, int64_t dim, int64_t max_tokens) {
+  const int rows = block_rows(queries * group, dim);
+  const int64_t ctas = static_cast<int64_t>(sm_count()) * (rows == 32 || dim == 256 ? 2 : 4);
+  const int64_t blocks = (queries * group + rows - 1) / rows;
+  const int64_t tiles = (max_tokens + kKv4Tile - 1) / kKv4Tile;
+  const int64_t items = batch * kv_heads * blocks;
+  if (tiles == 0 || items >= ctas * kMinTiles) return ctas;
+  return std::max<int64_t>(1, std::min(ctas, (items * tiles + kMinTiles - 1) / kMinTiles));
+}
+
+template <typename T, int kDim, int kRows>
+cudaError_t launch(const AttentionArgs& a, cudaStream_t stream) {
+  using S = Shape<T, kDim, kRows>;
+  static bool configured[64] = {};
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    const cudaError_t err = cudaFuncSetAttribute(attention_kernel<T, kDim, kRows>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (err != cudaSuccess) return err;
+    configured[dev] = true;
+  }
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(a.parts));
+  config.blockDim = dim3(kAttnThreads);
+  config.dynamicSmemBytes = S::kSmem;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  cudaError_t err = cudaLaunchKernelEx(&config, attention_kernel<T, kDim, kRows>, a);
+  if (err != cudaSuccess || a.parts == 1) return err;  // one part: nothing is split
+  const int64_t joins = a.batch * a.kv_heads * a.queries * a.group;
+  if (joins > 0x7fffffffLL) return cudaErrorInvalidValue;
+  config.gridDim = dim3(static_cast<unsigned>(joins));
+  config.blockDim = dim3(kJoinThreads);
+  config.dynamicSmemBytes = sizeof(float) * a.parts;
+  return cudaLaunchKernelEx(&config, join_kernel<T, kDim, kRows>, a);
+}
+
+template <typename T>
+cudaError_t launch_any(const AttentionArgs& a, int64_t dim, int rows, cudaStream_t s) {
+  if (dim == 64) return rows == 8 ? launch<T, 64, 8>(a, s) : rows == 16 ? launch<T, 64, 16>(a, s) : launch<T, 64, 32>(a, s);
+  if (dim == 128) {
+    return rows == 8 ? launch<T, 128, 8>(a, s) : rows == 16 ? launch<T, 128, 16>(a, s) : launch<T, 128, 32>(a, s);
+  }
+  return rows == 8 ? launch<T, 256, 8>(a, s) : launch<T, 256, 16>(a, s);
 }
 
 }  // namespace
@@ -137,7 +789,10 @@ PCK_STATUS_READER(attention_status)
 extern "C" int64_t pck_kv4_attention_scratch(int64_t batch, int64_t queries, int64_t heads, int64_t kv_heads, int64_t dim,
                                              int64_t max_tokens) {
   if (batch < 0 || queries < 1 || kv_heads < 1 || heads < kv_heads || dim < 1 || max_tokens < 0) return -1;
-  return 0;
+  const int64_t parts = pck::most_parts(batch, queries, heads / kv_heads, kv_heads, dim, max_tokens);
+  if (parts == 1) return 0;
+  const int64_t rows = pck::block_rows(queries * (heads / kv_heads), dim);
+  return 2 * parts * rows * (dim * 4 + 8);
 }
 
 extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_t queries, int64_t heads, int64_t dim,
@@ -146,15 +801,14 @@ extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_
                                  int64_t table_stride, int64_t table_pages, const int32_t* lengths, double scale,
                                  int64_t window, void* out, void* scratch, int64_t scratch_bytes, void* stream) {
   using namespace pck;
-  (void)scratch;
-  (void)scratch_bytes;
   if (dim != 64 && dim != 128 && dim != 256) return report_error(PCK_ERR_ARGUMENT, "attention: dim must be 64, 128 or 256");
   if (dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) return report_error(PCK_ERR_ARGUMENT, "attention: q must be bfloat16 or float16");
   if (batch < 0 || queries < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || heads > 0xffff ||
-      queries > 0xffff) {
-    return report_error(PCK_ERR_ARGUMENT, "attention: need batch >= 0, queries >= 1 and heads a multiple of kv_heads");
+      queries > 0x7fff) {
+    return report_error(PCK_ERR_ARGUMENT, "attention: need batch >= 0, queries in [1, 32767] and heads a multiple of kv_heads");
   }
-  if (pages < 0 || page_tiles < 1 || page_tiles > 0x7fffff || table_pages < 0 || table_stride < table_pages) {
+  if (pages < 0 || page_tiles < 1 || page_tiles > 0x7fffff || table_pages < 0 || table_pages > 0x7fffffff ||
+      table_stride < table_pages) {
     return report_error(PCK_ERR_ARGUMENT, "attention: need pages >= 0, page_tiles >= 1 and a page table of whole rows");
   }
   if (window < 0) return report_error(PCK_ERR_ARGUMENT, "attention: window must be 0 (none) or positive");
@@ -164,7 +818,20 @@ extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_
     return report_error(PCK_ERR_ARGUMENT, "attention: NULL q, cache, page_table, lengths or out");
   }
   if (!aligned_to(cache, 16)) return report_error(PCK_ERR_ARGUMENT, "attention: the cache must be 16-byte aligned");
+  const int64_t max_tokens = table_pages * page_tiles * kKv4Tile;
+  if (max_tokens > 1 << 30) return report_error(PCK_ERR_UNSUPPORTED, "attention: a request holds at most 2^30 tokens");
+  const int64_t group = heads / kv_heads;
+  const int rows = block_rows(queries * group, dim);
   AttentionArgs a{};
+  a.parts = static_cast<int32_t>(most_parts(batch, queries, group, kv_heads, dim, max_tokens));
+  if (a.parts > 1) {
+    const int64_t slots = 2LL * a.parts * rows;
+    if (!scratch || !aligned_to(scratch, 16) || scratch_bytes < slots * (dim * 4 + 8)) {
+      return report_error(PCK_ERR_ARGUMENT, "attention: needs pck_kv4_attention_scratch() bytes of aligned scratch");
+    }
+    a.sums = static_cast<float*>(scratch);
+    a.top_total = reinterpret_cast<float2*>(a.sums + slots * dim);
+  }
   a.q = q;
   a.q_batch_stride = q_batch_stride;
   a.q_token_stride = q_token_stride;
@@ -175,15 +842,19 @@ extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_
   a.table_stride = table_stride;
   a.lengths = lengths;
   a.out = out;
-  a.scale = static_cast<float>(scale);
-  a.window = window;
-  a.max_tokens = table_pages * page_tiles * kKv4Tile;
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  a.window = window < max_tokens ? static_cast<int32_t>(window) : 0;
+  a.max_tokens = static_cast<int32_t>(max_tokens);
+  a.batch = batch;
   a.queries = static_cast<int32_t>(queries);
   a.heads = static_cast<int32_t>(heads);
   a.kv_heads = static_cast<int32_t>(kv_heads);
   a.page_tiles = static_cast<int32_t>(page_tiles);
+  a.group = static_cast<int32_t>(group);
+  a.row_blocks = static_cast<int32_t>((queries * group + rows - 1) / rows);
+  a.q_vector = aligned_to(q, 16) && q_batch_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = dtype == PCK_LOGITS_BF16 ? launch_attention<__nv_bfloat16>(a, batch, static_cast<int>(dim), s)
-                                                   : launch_attention<__half>(a, batch, static_cast<int>(dim), s);
+  const cudaError_t err = dtype == PCK_LOGITS_BF16 ? launch_any<__nv_bfloat16>(a, dim, rows, s)
+                                                   : launch_any<__half>(a, dim, rows, s);
   return err == cudaSuccess ? PCK_OK : report_cuda("attention kernel", err);
 }
