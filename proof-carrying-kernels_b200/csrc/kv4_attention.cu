@@ -3,10 +3,11 @@
 // Bound by memory: a decode step reads every code once for a few query rows, so the cache has to
 // come in at the HBM's rate and the work per code has to stay small. What that led to:
 //   - The query rows that share a key/value head (its group of heads, and the query tokens of a
-//     request) are the 8, 16 or 32 rows of one matrix product: a tile of 16 tokens is read and
-//     unpacked once for all of them. mma.sync takes the unpacked codes from registers; tcgen05
-//     would want them written to shared memory first, which alone would exceed its bandwidth at
-//     the rate of two codes a byte.
+//     request) are the columns of one matrix product, 8 at a time: a tile of 16 tokens is read and
+//     unpacked once for up to 32 of them. Both products have the codes on the left (keys: tokens x
+//     channels, values: channels x tokens), which fills mma.sync's 16 rows even for a single query
+//     row, and a lane then meets the scales of only two tokens. tcgen05 would want the unpacked codes
+//     written to shared memory first, which alone would exceed its bandwidth at two codes a byte.
 //   - Codes are unpacked with a mask, a shift and an or: the four bits become the low mantissa bits
 //     of a 16-bit float. Scales never touch the codes: with k = code * s + z,
 //       q.k = sum over groups of s (q.code) + z sum(q),
@@ -96,16 +97,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 template <typename T>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    const uint32_t (&b)[2]) {
   if constexpr (std::is_same_v<T, __half>) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
   } else {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
   }
+}
+
+// Transposes an 8 x 8 matrix of 16-bit elements held two to a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
@@ -136,7 +145,9 @@ constexpr float kKeyBias = std::is_same_v<T, __half> ? 8.0f : -128.0f;
 
 template <int kWords>
 __device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t* p) {
-  if constexpr (kWords == 2) {
+  if constexpr (kWords == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (kWords == 2) {
     const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x;
     w[1] = v.y;
@@ -149,29 +160,34 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t*
   }
 }
 
-// Rows 8: one eight-row half of a 16-row product (the other half is empty and its results are not
-// kept); 16, 32: one or two full products.
+// CTAs on an SM, by the registers that the rows' products take.
+constexpr int attention_ctas(int rows, int dim) {
+  if (dim == 64) return rows <= 16 ? 4 : 2;
+  if (dim == 128) return rows <= 8 ? 4 : rows <= 16 ? 3 : 2;
+  return 2;
+}
+
 template <typename T, int kDim, int kRows>
 struct Shape {
   static constexpr int kGroups = kDim / kKv4Group;
   static constexpr int kPlanes = kGroups > 2 ? kGroups / 2 : 1;
   static constexpr int kWidth = kGroups > 1 ? 2 : 1;  // groups of a plane
-  static constexpr int kHalves = kRows / 8;           // rows of a lane: lane / 4 + 8 h
-  static constexpr int kBlocks = kRows > 16 ? 2 : 1;  // products
+  static constexpr int kCols = kRows / 8;             // column blocks of the products: 8 query rows each
   static constexpr int kTileBytes = kv4_tile_bytes(kDim);
-  // 32 rows or 256 channels take twice the registers: fewer CTAs run beside each other, with more slots.
-  static constexpr bool kWide = kRows == 32 || kDim == 256;
-  static constexpr int kSlots = kDim == 64 ? 8 : kDim == 128 ? (kWide ? 8 : 5) : 4;
+  static constexpr int kCtas = attention_ctas(kRows, kDim);
+  // Enough copies in flight for the HBM's latency: about 180 KB of rings on an SM.
+  static constexpr int kSlots = (180 << 10) / (kCtas * kAttnWarps * kTileBytes) < 12
+                                    ? (180 << 10) / (kCtas * kAttnWarps * kTileBytes) : 12;
   static constexpr int kRing = kAttnWarps * kSlots * kTileBytes;
   static constexpr int kSmem = kRing + 1024;
   static_assert(kRing >= kAttnWarps * kRows * kDim * 4, "the warps' sums overlay the rings");
 };
 
 template <typename T, int kDim, int kRows>
-__global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2 : 4)
+__global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     attention_kernel(const __grid_constant__ AttentionArgs a) {
   using S = Shape<T, kDim, kRows>;
-  constexpr int kG = S::kGroups, kH = S::kHalves, kMB = S::kBlocks;
+  constexpr int kG = S::kGroups, kN = S::kCols;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kAttnWarps][S::kSlots];
   __shared__ int64_t scan[kAttnWarps];
@@ -233,6 +249,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2
   int64_t b = found[0];
   int64_t base = found[1] * items;  // of request b on the line
 
+  const uint64_t policy = policy_evict_first();
   uint8_t* const ring = smem + warp * S::kSlots * S::kTileBytes;
   uint32_t phase = 0;  // parity bit of each slot
   bool dead = false;   // a wait gave up
@@ -259,18 +276,21 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2
     hi = pos1 < 0 ? lo : min(hi, pos1 / kKv4Tile + 1);
     const int warp_tiles = hi - lo > warp ? (hi - lo - warp + kAttnWarps - 1) / kAttnWarps : 0;
 
-    // This lane's rows: their positions, and q as the left operand with its channels in the order
-    // of the codes: for each 8 channels the pairs (0, 4), (1, 5), (2, 6), (3, 7).
-    int pos[kH];
-    uint32_t qf[kMB][kG * 4][4];
-    float qsum[kG][kH];
+    // q as the right operand: this lane's row lane / 4 of each block, its channels in the order of
+    // the codes: for each 8 channels the pairs (0, 4), (1, 5), (2, 6), (3, 7).
+    uint32_t qf[kN][kG * 4][2];
+    // What the products' columns belong to: rows 2 quarter and the next of each block.
+    float qsum[kN][kG][2];
+    int pos[kN][2];
 #pragma unroll
-    for (int h = 0; h < (kH == 1 ? 1 : kH); ++h) {
-      const int r = row0 + row8 + 8 * h;
+    for (int n = 0; n < kN; ++n) {
+      const int r = row0 + 8 * n + row8;
       const int t = r / a.group;
-      pos[h] = r < rows ? length - a.queries + t : -1;
       const T* qr = static_cast<const T*>(a.q) + b * a.q_batch_stride + t * a.q_token_stride +
                     static_cast<int64_t>(kvh * a.group + r % a.group) * a.q_head_stride;
+      const int my_pos = r < rows ? length - a.queries + t : -1;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) pos[n][e] = __shfl_sync(kFullMask, my_pos, (2 * quarter + e) * 4);
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
         uint32_t x[8];
@@ -296,36 +316,38 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2
         }
         sum += __shfl_xor_sync(kFullMask, sum, 1);
         sum += __shfl_xor_sync(kFullMask, sum, 2);
-        qsum[g][h] = sum;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) qsum[n][g][e] = __shfl_sync(kFullMask, sum, (2 * quarter + e) * 4);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const uint32_t* y = x + 4 * w;
-          uint32_t(*f)[4] = &qf[h / 2][g * 4 + 2 * w];
-          f[0][h % 2] = __byte_perm(y[0], y[2], 0x5410);
-          f[0][2 + h % 2] = __byte_perm(y[0], y[2], 0x7632);
-          f[1][h % 2] = __byte_perm(y[1], y[3], 0x5410);
-          f[1][2 + h % 2] = __byte_perm(y[1], y[3], 0x7632);
+          uint32_t(*f)[2] = &qf[n][g * 4 + 2 * w];
+          f[0][0] = __byte_perm(y[0], y[2], 0x5410);
+          f[0][1] = __byte_perm(y[0], y[2], 0x7632);
+          f[1][0] = __byte_perm(y[1], y[3], 0x5410);
+          f[1][1] = __byte_perm(y[1], y[3], 0x7632);
         }
       }
     }
-    if constexpr (kH == 1) {
-#pragma unroll
-      for (int k = 0; k < kG * 4; ++k) qf[0][k][1] = qf[0][k][3] = 0;
-    }
 
-    float acc[kG][8][kH][2];  // [group][channel of 8][row][lanes' two channel octets]
-    float top[kH], total_w[kH], zeros[kG][kH];
+    // Products with the values: element e of [n][g][m] is channel 8 (lane / 4) + 2 m + e / 2 of group
+    // g for row 2 quarter + e % 2 of block n.
+    float acc[kN][kG][4][4];
+    float top[kN][2], total_w[kN][2], zeros[kN][kG][2];
     uint32_t unit[kG];  // exponent field of the power of two that the values' weights are divided by
     float inv[kG];
 #pragma unroll
-    for (int h = 0; h < kH; ++h) {
-      top[h] = -INFINITY;
-      total_w[h] = 0.0f;
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[n][e] = -INFINITY;
+        total_w[n][e] = 0.0f;
+      }
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
-        zeros[g][h] = 0.0f;
+        zeros[n][g][0] = zeros[n][g][1] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 8; ++n) acc[g][n][h][0] = acc[g][n][h][1] = 0.0f;
+        for (int m = 0; m < 4; ++m) acc[n][g][m][0] = acc[n][g][m][1] = acc[n][g][m][2] = acc[n][g][m][3] = 0.0f;
       }
     }
 #pragma unroll
@@ -334,95 +356,83 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2
       inv[g] = 1.0f;
     }
 
-    // The warp's k-th tile is lo + warp + 4 k. Its page: 32 of them are looked up at once, a lane
-    // each, one batch ahead of their use.
+    // The warp's k-th tile is lo + warp + 4 k. Where it lies in the cache: 32 of them are looked up at
+    // once, a lane each, one batch ahead of their use; -1 without a page.
     const int32_t* table = a.page_table + b * a.table_stride;
     auto look_up = [&](int k) -> int32_t {
       k += lane;
       if (k >= warp_tiles) return -1;
-      const int32_t page = table[(lo + warp + k * kAttnWarps) / a.page_tiles];
+      const int tile = lo + warp + k * kAttnWarps;
+      const int32_t page = table[tile / a.page_tiles];
       if (page < 0 || page >= a.pages) {
         report(kDevIndex);
         return -1;
       }
-      return page;
+      return (page * a.kv_heads + kvh) * a.page_tiles + tile % a.page_tiles;
     };
-    int32_t pages_now = look_up(0), pages_next = look_up(kWarp);
+    int32_t places = look_up(0), places_next = look_up(kWarp);
     uint32_t missing = 0;  // slots whose tile has no page
     auto issue = [&](int k, int slot) {
       if (k % kWarp == 0 && k > 0) {
-        pages_now = pages_next;
-        pages_next = look_up(k + kWarp);
+        places = places_next;
+        places_next = look_up(k + kWarp);
       }
-      const int32_t page = __shfl_sync(kFullMask, pages_now, k % kWarp);
-      missing = page < 0 ? missing | 1u << slot : missing & ~(1u << slot);
+      const int32_t place = __shfl_sync(kFullMask, places, k % kWarp);
+      missing = place < 0 ? missing | 1u << slot : missing & ~(1u << slot);
       if (lane == 0) {
-        if (page < 0) {
+        if (place < 0) {
           mbar_arrive(&full[warp][slot]);
         } else {
-          const int tile = lo + warp + k * kAttnWarps;
-          const uint8_t* from = a.cache + ((static_cast<int64_t>(page) * a.kv_heads + kvh) * a.page_tiles +
-                                           tile % a.page_tiles) * S::kTileBytes;
           mbar_arrive_expect_tx(&full[warp][slot], S::kTileBytes);
-          bulk_load(ring + slot * S::kTileBytes, from, S::kTileBytes, &full[warp][slot], policy_evict_first());
+          bulk_load(ring + slot * S::kTileBytes, a.cache + static_cast<int64_t>(place) * S::kTileBytes, S::kTileBytes,
+                    &full[warp][slot], policy);
         }
       }
     };
     for (int s = 0; s < S::kSlots && s < warp_tiles; ++s) issue(s, s);
 
-    // One tile in registers and shared memory. kMasked: some row does not see some of its tokens.
+    // One tile. This lane's tokens are row8 and row8 + 8. kMasked: some row does not see some of them.
     auto tile_step = [&](const uint8_t* tile, int token0, auto masked_tag) {
       constexpr bool kMasked = decltype(masked_tag)::value;
-      float s[2][kH][2];
-      bool off[2][kH][2];
+      float s[kN][4];  // element e: token row8 + 8 (e / 2), row 2 quarter + e % 2
+      bool off[kN][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float part[kG][kMB][4];
+      for (int n = 0; n < kN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+      uint32_t pairs[2][kG];
 #pragma unroll
-        for (int p = 0; p < S::kPlanes; ++p) {
-          uint32_t w[2 * S::kWidth];
-          load_words(w, tile + p * 512 * S::kWidth + (j * kWarp + lane) * 8 * S::kWidth);
+      for (int j = 0; j < 2; ++j) load_words(pairs[j], tile + kv4_key_scale(kDim, 8 * j, 0) + row8 * 4 * kG);
 #pragma unroll
-          for (int i = 0; i < S::kWidth; ++i) {
-            const int g = p * S::kWidth + i;
+      for (int p = 0; p < S::kPlanes; ++p) {
+        uint32_t w[2][2 * S::kWidth];
 #pragma unroll
-            for (int m = 0; m < kMB; ++m) part[g][m][0] = part[g][m][1] = part[g][m][2] = part[g][m][3] = 0.0f;
+        for (int j = 0; j < 2; ++j) load_words(w[j], tile + p * 512 * S::kWidth + (j * kWarp + lane) * 8 * S::kWidth);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t k[4];
-              unpack<T>(w[2 * i + c], k);
+        for (int i = 0; i < S::kWidth; ++i) {
+          const int g = p * S::kWidth + i;
+          float part[kN][4];
 #pragma unroll
-              for (int m = 0; m < kMB; ++m) {
-                mma<T>(part[g][m], qf[m][g * 4 + 2 * c], k[0], k[1]);
-                mma<T>(part[g][m], qf[m][g * 4 + 2 * c + 1], k[2], k[3]);
+          for (int n = 0; n < kN; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.0f;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t k0[4], k1[4];
+            unpack<T>(w[0][2 * i + c], k0);
+            unpack<T>(w[1][2 * i + c], k1);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+              mma<T>(part[n], k0[0], k1[0], k0[1], k1[1], qf[n][g * 4 + 2 * c]);
+              mma<T>(part[n], k0[2], k1[2], k0[3], k1[3], qf[n][g * 4 + 2 * c + 1]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float scale = bf16_lo(pairs[j][g]);
+            const float zero = fmaf(kKeyBias<T>, scale, bf16_hi(pairs[j][g]));
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                s[n][2 * j + e] = fmaf(zero, qsum[n][g][e], fmaf(scale, part[n][2 * j + e], s[n][2 * j + e]));
               }
-            }
-          }
-        }
-        // This lane's columns: tokens 8 j + 2 quarter and the next.
-        const uint32_t* pairs = reinterpret_cast<const uint32_t*>(tile + kv4_key_scale(kDim, 8 * j + 2 * quarter, 0));
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-          for (int h = 0; h < kH; ++h) s[j][h][c] = 0.0f;
-#pragma unroll
-          for (int g = 0; g < kG; ++g) {
-            const uint32_t pair = pairs[c * kG + g];
-            const float scale = bf16_lo(pair);
-            const float zero = fmaf(kKeyBias<T>, scale, bf16_hi(pair));
-#pragma unroll
-            for (int h = 0; h < kH; ++h) {
-              s[j][h][c] = fmaf(scale, part[g][h / 2][h % 2 * 2 + c], s[j][h][c]);
-              s[j][h][c] = fmaf(zero, qsum[g][h], s[j][h][c]);
-            }
-          }
-#pragma unroll
-          for (int h = 0; h < kH; ++h) {
-            s[j][h][c] *= a.scale_log2;
-            if constexpr (kMasked) {
-              const int token = token0 + 8 * j + 2 * quarter + c;
-              off[j][h][c] = token > pos[h] || (a.window > 0 && token <= pos[h] - a.window);
-              if (off[j][h][c]) s[j][h][c] = -INFINITY;
             }
           }
         }
@@ -430,44 +440,63 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2
       // Raise the maximum where a score passes it by more than 2^kRaise.
       bool pass = false;
 #pragma unroll
-      for (int h = 0; h < kH; ++h) {
-        const float m = fmaxf(fmaxf(s[0][h][0], s[0][h][1]), fmaxf(s[1][h][0], s[1][h][1]));
-        pass = pass || m > top[h] + kRaise;
+      for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][e] *= a.scale_log2;
+          if constexpr (kMasked) {
+            const int token = token0 + row8 + 8 * (e / 2), at = pos[n][e % 2];
+            off[n][e] = token > at || (a.window > 0 && token <= at - a.window);
+            if (off[n][e]) s[n][e] = -INFINITY;
+          }
+        }
+        pass = pass || fmaxf(s[n][0], s[n][2]) > top[n][0] + kRaise || fmaxf(s[n][1], s[n][3]) > top[n][1] + kRaise;
       }
       if (__any_sync(kFullMask, pass)) {
 #pragma unroll
-        for (int h = 0; h < kH; ++h) {
-          float m = fmaxf(fmaxf(s[0][h][0], s[0][h][1]), fmaxf(s[1][h][0], s[1][h][1]));
-          m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 1));
-          m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 2));
-          m = fmaxf(m, top[h]);
-          const float keep = top[h] == m ? 1.0f : exp2_fast(top[h] - m);
-          top[h] = m;
-          total_w[h] *= keep;
+        for (int n = 0; n < kN; ++n) {
 #pragma unroll
-          for (int g = 0; g < kG; ++g) {
-            zeros[g][h] *= keep;
+          for (int e = 0; e < 2; ++e) {
+            float m = fmaxf(s[n][e], s[n][e + 2]);
+            m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16));
+            m = fmaxf(m, top[n][e]);
+            const float keep = top[n][e] == m ? 1.0f : exp2_fast(top[n][e] - m);
+            top[n][e] = m;
+            total_w[n][e] *= keep;
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
-              acc[g][n][h][0] *= keep;
-              acc[g][n][h][1] *= keep;
+            for (int g = 0; g < kG; ++g) {
+              zeros[n][g][e] *= keep;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                acc[n][g][i][e] *= keep;
+                acc[n][g][i][e + 2] *= keep;
+              }
             }
           }
         }
       }
 #pragma unroll
-      for (int h = 0; h < kH; ++h) {
-        const float m = top[h] == -INFINITY ? 0.0f : top[h];
+      for (int n = 0; n < kN; ++n) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int e = 0; e < 4; ++e) {
+          const float m = top[n][e % 2];
+          s[n][e] = exp2_fast(s[n][e] - (m == -INFINITY ? 0.0f : m));
+          total_w[n][e % 2] += s[n][e];
+        }
+      }
+      // The values, a group at a time: its scales go into the weights.
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            s[j][h][c] = exp2_fast(s[j][h][c] - m);
-            total_w[h] += s[j][h][c];
+      for (int j = 0; j < 2; ++j) {
+        load_words(pairs[j], tile + kv4_value_scale(kDim, 8 * j, 0) + row8 * 4 * kG);
+        if constexpr (kMasked) {
+          if (token0 + row8 + 8 * j >= length) {  // a place that nothing was written to
+#pragma unroll
+            for (int g = 0; g < kG; ++g) pairs[j][g] = 0;
           }
         }
       }
-      // The values: a group at a time, weights of its scales.
 #pragma unroll
       for (int p = 0; p < S::kPlanes; ++p) {
         uint32_t w[2][2 * S::kWidth];
@@ -478,57 +507,43 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2
 #pragma unroll
         for (int i = 0; i < S::kWidth; ++i) {
           const int g = p * S::kWidth + i;
-          float scale[2][2], zero[2][2];
-          uint32_t largest = 0;
+          // Keep the largest scale within 2^4 of the unit; a NaN scale leaves the unit alone.
+          const uint32_t field = __reduce_max_sync(kFullMask, max(pairs[0][g] << 16, pairs[1][g] << 16)) >> 23;
+          if (field + 4 - unit[g] > 8 && field != 0 && field < 255) {
+            const uint32_t next = min(field, 253u);
+            const float ratio = __uint_as_float((254u - next) << 23) * __uint_as_float(unit[g] << 23);
+            unit[g] = next;
+            inv[g] = __uint_as_float((254u - next) << 23);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[n][g][m][e] *= ratio;
+              }
+            }
+          }
+          uint32_t wf[kN][2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
+            const float scale = bf16_lo(pairs[j][g]), zero = fmaf(8.0f, scale, bf16_hi(pairs[j][g]));
+            const float unit_scale = scale * inv[g];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int token = 8 * j + 2 * quarter + c;
-              uint32_t pair = *reinterpret_cast<const uint32_t*>(tile + kv4_value_scale(kDim, token, g));
-              if constexpr (kMasked) {
-                if (token0 + token >= length) pair = 0;  // a place that nothing was written to
-              }
-              scale[j][c] = bf16_lo(pair);
-              zero[j][c] = fmaf(8.0f, scale[j][c], bf16_hi(pair));
-              largest = max(largest, pair << 16);
-            }
-          }
-          largest = __reduce_max_sync(kFullMask, largest);
-          // Keep the largest scale within 2^4 of the unit; a NaN scale leaves the unit alone.
-          const uint32_t field = largest >> 23;
-          if (field + 4 < unit[g] || field > unit[g] + 4) {
-            if (largest != 0 && field < 255) {
-              const uint32_t next = min(max(field, 1u), 253u);
-              const float ratio = __uint_as_float((254u - next) << 23) * __uint_as_float(unit[g] << 23);
-              unit[g] = next;
-              inv[g] = __uint_as_float((254u - next) << 23);
-#pragma unroll
-              for (int n = 0; n < 8; ++n) {
-#pragma unroll
-                for (int h = 0; h < kH; ++h) {
-                  acc[g][n][h][0] *= ratio;
-                  acc[g][n][h][1] *= ratio;
-                }
-              }
-            }
-          }
-          uint32_t wf[kMB][4] = {};
-#pragma unroll
-          for (int h = 0; h < kH; ++h) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int n = 0; n < kN; ++n) {
               float x[2];
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                x[c] = s[j][h][c] * (scale[j][c] * inv[g]);
-                float z = s[j][h][c] * zero[j][c];
+              for (int e = 0; e < 2; ++e) {
+                const float weight = s[n][2 * j + e];
+                x[e] = weight * unit_scale;
                 if constexpr (kMasked) {  // a NaN scale must not reach rows that do not see its token
-                  if (off[j][h][c]) x[c] = z = 0.0f;
+                  if (off[n][2 * j + e]) {
+                    x[e] = 0.0f;
+                    continue;
+                  }
                 }
-                zeros[g][h] += z;
+                zeros[n][g][e] = fmaf(weight, zero, zeros[n][g][e]);
               }
-              wf[h / 2][2 * j + h % 2] = half2_bits(__floats2half2_rn(x[0], x[1]));
+              wf[n][j] = transpose8(half2_bits(__floats2half2_rn(x[0], x[1])));
             }
           }
 #pragma unroll
@@ -537,24 +552,9 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2
             unpack<__half>(w[0][2 * i + d], v0);
             unpack<__half>(w[1][2 * i + d], v1);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-#pragma unroll
-              for (int m = 0; m < kMB; ++m) {
-                float(*to)[2] = &acc[g][4 * d + n][2 * m];
-                if constexpr (kH == 1) {
-                  float r[4] = {to[0][0], to[0][1], 0.0f, 0.0f};
-                  mma<__half>(r, wf[m], v0[n], v1[n]);
-                  to[0][0] = r[0];
-                  to[0][1] = r[1];
-                } else {
-                  float r[4] = {to[0][0], to[0][1], to[1][0], to[1][1]};
-                  mma<__half>(r, wf[m], v0[n], v1[n]);
-                  to[0][0] = r[0];
-                  to[0][1] = r[1];
-                  to[1][0] = r[2];
-                  to[1][1] = r[3];
-                }
-              }
+            for (int n = 0; n < kN; ++n) {
+              mma<__half>(acc[n][g][2 * d], v0[0], v0[1], v1[0], v1[1], wf[n]);
+              mma<__half>(acc[n][g][2 * d + 1], v0[2], v0[3], v1[2], v1[3], wf[n]);
             }
           }
         }
@@ -563,9 +563,8 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2
 
     int slot = 0;
     for (int k = 0; k < warp_tiles; ++k) {
-      if (!dead) dead = !mbar_wait(&full[warp][slot], phase >> slot & 1u);
+      if (!dead) dead = !__all_sync(kFullMask, mbar_wait(&full[warp][slot], phase >> slot & 1u));
       phase ^= 1u << slot;
-      dead = __any_sync(kFullMask, dead);
       if (!(missing >> slot & 1u) && !dead) {
         const uint8_t* tile = ring + slot * S::kTileBytes;
         const int token0 = (lo + warp + k * kAttnWarps) * kKv4Tile;
@@ -585,25 +584,24 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kWide ? 2
     __syncthreads();
     float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int h = 0; h < kH; ++h) {
-      float l = total_w[h];
-      l += __shfl_xor_sync(kFullMask, l, 1);
-      l += __shfl_xor_sync(kFullMask, l, 2);
-      if (quarter == 0) state[warp][row8 + 8 * h] = make_float2(top[h], l);
+    for (int n = 0; n < kN; ++n) {
 #pragma unroll
-      for (int g = 0; g < kG; ++g) {
-        float z = zeros[g][h];
-        z += __shfl_xor_sync(kFullMask, z, 1);
-        z += __shfl_xor_sync(kFullMask, z, 2);
-        const float u = __uint_as_float(unit[g] << 23);
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * n + 2 * quarter + e;
+        float l = total_w[n][e];
+        for (int o = 4; o < kWarp; o <<= 1) l += __shfl_xor_sync(kFullMask, l, o);
+        if (row8 == 0) state[warp][r] = make_float2(top[n][e], l);
 #pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          float4* to = reinterpret_cast<float4*>(sums + (warp * kRows + row8 + 8 * h) * kDim + g * kKv4Group +
-                                                 8 * (2 * quarter + o));
-          to[0] = make_float4(fmaf(acc[g][0][h][o], u, z), fmaf(acc[g][1][h][o], u, z), fmaf(acc[g][2][h][o], u, z),
-                              fmaf(acc[g][3][h][o], u, z));
-          to[1] = make_float4(fmaf(acc[g][4][h][o], u, z), fmaf(acc[g][5][h][o], u, z), fmaf(acc[g][6][h][o], u, z),
-                              fmaf(acc[g][7][h][o], u, z));
+        for (int g = 0; g < kG; ++g) {
+          float z = zeros[n][g][e];
+          for (int o = 4; o < kWarp; o <<= 1) z += __shfl_xor_sync(kFullMask, z, o);
+          const float u = __uint_as_float(unit[g] << 23);
+          float4* to = reinterpret_cast<float4*>(sums + (warp * kRows + r) * kDim + g * kKv4Group + 8 * row8);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float(*x)[4] = &acc[n][g][2 * i];
+            to[i] = make_float4(fmaf(x[0][e], u, z), fmaf(x[0][e + 2], u, z), fmaf(x[1][e], u, z), fmaf(x[1][e + 2], u, z));
+          }
         }
       }
     }
@@ -712,9 +710,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   }
 }
 
-// Rows of a block: as many as the item has, up to 32 (16 with 256 channels, whose sums take the
-// registers of twice as many rows).
-int block_rows(int64_t rows, int64_t dim) { return rows <= 8 ? 8 : rows <= 16 || dim == 256 ? 16 : 32; }
+// Rows of a block: as many as the item has, up to what the registers hold beside the products.
+int block_rows(int64_t rows, int64_t dim) {
+  if (rows <= 8) return 8;
+  if (rows <= 16 || dim == 256) return 16;
+  return dim == 128 ? 24 : 32;
+}
 
 int sm_count() {
   static int cache[64] = {0};
@@ -731,7 +732,7 @@ int sm_count() {
 // Most parts of a call: the CTAs that run at once, and no more than the longest lengths can fill.
 int64_t most_parts(int64_t batch, int64_t queries, int64_t group, int64_t kv_heads, int64_t dim, int64_t max_tokens) {
   const int rows = block_rows(queries * group, dim);
-  const int64_t ctas = static_cast<int64_t>(sm_count()) * (rows == 32 || dim == 256 ? 2 : 4);
+  const int64_t ctas = static_cast<int64_t>(sm_count()) * attention_ctas(rows, static_cast<int>(dim));
   const int64_t blocks = (queries * group + rows - 1) / rows;
   const int64_t tiles = (max_tokens + kKv4Tile - 1) / kKv4Tile;
   const int64_t items = batch * kv_heads * blocks;
@@ -775,7 +776,7 @@ template <typename T>
 cudaError_t launch_any(const AttentionArgs& a, int64_t dim, int rows, cudaStream_t s) {
   if (dim == 64) return rows == 8 ? launch<T, 64, 8>(a, s) : rows == 16 ? launch<T, 64, 16>(a, s) : launch<T, 64, 32>(a, s);
   if (dim == 128) {
-    return rows == 8 ? launch<T, 128, 8>(a, s) : rows == 16 ? launch<T, 128, 16>(a, s) : launch<T, 128, 32>(a, s);
+    return rows == 8 ? launch<T, 128, 8>(a, s) : rows == 16 ? launch<T, 128, 16>(a, s) : launch<T, 128, 24>(a, s);
   }
   return rows == 8 ? launch<T, 256, 8>(a, s) : launch<T, 256, 16>(a, s);
 }
@@ -807,7 +808,7 @@ extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_
       queries > 0x7fff) {
     return report_error(PCK_ERR_ARGUMENT, "attention: need batch >= 0, queries in [1, 32767] and heads a multiple of kv_heads");
   }
-  if (pages < 0 || page_tiles < 1 || page_tiles > 0x7fffff || table_pages < 0 || table_pages > 0x7fffffff ||
+  if (pages < 0 || pages > 0x7fffffff || page_tiles < 1 || page_tiles > 0x7fffff || table_pages < 0 || table_pages > 0x7fffffff ||
       table_stride < table_pages) {
     return report_error(PCK_ERR_ARGUMENT, "attention: need pages >= 0, page_tiles >= 1 and a page table of whole rows");
   }
@@ -818,6 +819,9 @@ extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_
     return report_error(PCK_ERR_ARGUMENT, "attention: NULL q, cache, page_table, lengths or out");
   }
   if (!aligned_to(cache, 16)) return report_error(PCK_ERR_ARGUMENT, "attention: the cache must be 16-byte aligned");
+  if (pages * kv_heads > (int64_t{1} << 31) / page_tiles) {
+    return report_error(PCK_ERR_UNSUPPORTED, "attention: a cache holds at most 2^31 tiles");
+  }
   const int64_t max_tokens = table_pages * page_tiles * kKv4Tile;
   if (max_tokens > 1 << 30) return report_error(PCK_ERR_UNSUPPORTED, "attention: a request holds at most 2^30 tokens");
   const int64_t group = heads / kv_heads;
