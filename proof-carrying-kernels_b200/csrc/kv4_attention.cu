@@ -8,8 +8,10 @@
 //     channels, values: channels x tokens), which fills mma.sync's 16 rows even for a single query
 //     row, and a lane then meets the scales of only two tokens. tcgen05 would want the unpacked codes
 //     written to shared memory first, which alone would exceed its bandwidth at two codes a byte.
-//   - Codes are unpacked with a mask, a shift and an or: the four bits become the low mantissa bits
-//     of a 16-bit float. Scales never touch the codes: with k = code * s + z,
+//   - Codes are unpacked to binary16 with a mask and an or (the four bits become the low mantissa
+//     bits of 1024 + n) and one exact subtraction, two codes an instruction; bfloat16 queries become
+//     binary16 exactly, scaled by a power of two (what falls below 2^-24 of a row's largest element
+//     is lost, as it would be in a binary32 sum). Scales never touch the codes: with k = code * s + z,
 //       q.k = sum over groups of s (q.code) + z sum(q),
 //     and for the values the weight p s of a token and group goes into the matrix product instead
 //     of p; sum of p z is added at the end.
@@ -21,8 +23,8 @@
 //     common tile needs no exchange between lanes for it.
 //   - The tiles of all (request, head, row block) items form one line that is cut into equal parts,
 //     a CTA each, whatever the lengths: a part of an item leaves its sums in scratch memory and a
-//     second kernel (a programmatic dependent) joins them. A CTA's four warps take tiles in turn,
-//     each through its own ring of bulk copies.
+//     second kernel (a programmatic dependent) joins them. A CTA's four warps take pairs of tiles in
+//     turn, each through its own ring of bulk copies.
 #include <algorithm>
 
 #include "kv4_layout.cuh"
@@ -96,18 +98,19 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                     const uint32_t (&b)[2]) {
-  if constexpr (std::is_same_v<T, __half>) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
-  } else {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
-  }
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
+}
+
+// The same, from zero.
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(0.0f));
 }
 
 // Transposes an 8 x 8 matrix of 16-bit elements held two to a lane.
@@ -119,29 +122,38 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 
 __device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 
-// Four pairs of codes of a 32-bit word, nibbles (i, i + 4), as the products take them. binary16: the
-// code - 8, exactly (1024 + n and 1024 + 16 n have their codes in the mantissa). bfloat16: the code +
-// 128, whose excess goes into the zero's term (kKeyBias), with no further operation per code.
-template <typename T>
-__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&out)[4]) {
-  if constexpr (std::is_same_v<T, __half>) {
-    const __half2 low = __floats2half2_rn(1032.0f, 1032.0f);
-    const __half2 part = __floats2half2_rn(0.0625f, 0.0625f), high = __floats2half2_rn(-72.0f, -72.0f);
+// (w & mask) | bits in one instruction: both constants come in registers.
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+  return r;
+}
+
+// A constant that the compiler keeps in a register instead of building it at each use.
+__device__ __forceinline__ uint32_t kept(uint32_t v) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+struct Masks {
+  uint32_t low, high, bits;
+};
+
+// Four pairs of codes of a 32-bit word, nibbles (i, i + 4), as binary16 code - 8, exactly: 1024 + n
+// and 1024 + 16 n have the codes in their mantissas.
+__device__ __forceinline__ void unpack(uint32_t w, const Masks& k, uint32_t (&out)[4]) {
+  const __half2 low = __floats2half2_rn(1032.0f, 1032.0f);
+  const __half2 part = __floats2half2_rn(0.0625f, 0.0625f), high = __floats2half2_rn(-72.0f, -72.0f);
 #pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      uint32_t x = (w & 0x000f000fu) | 0x64006400u;
-      uint32_t y = (w & 0x00f000f0u) | 0x64006400u;
-      out[i] = half2_bits(__hsub2(*reinterpret_cast<__half2*>(&x), low));
-      out[i + 1] = half2_bits(__hfma2(*reinterpret_cast<__half2*>(&y), part, high));
-      w >>= 8;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  for (int i = 0; i < 4; i += 2) {
+    uint32_t x = and_or(w, k.low, k.bits);
+    uint32_t y = and_or(w, k.high, k.bits);
+    out[i] = half2_bits(__hsub2(*reinterpret_cast<__half2*>(&x), low));
+    out[i + 1] = half2_bits(__hfma2(*reinterpret_cast<__half2*>(&y), part, high));
+    w >>= 8;
   }
 }
-template <typename T>
-constexpr float kKeyBias = std::is_same_v<T, __half> ? 8.0f : -128.0f;
 
 template <int kWords>
 __device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t* p) {
@@ -175,11 +187,13 @@ struct Shape {
   static constexpr int kCols = kRows / 8;             // column blocks of the products: 8 query rows each
   static constexpr int kTileBytes = kv4_tile_bytes(kDim);
   static constexpr int kCtas = attention_ctas(kRows, kDim);
-  // Enough copies in flight for the HBM's latency: about 180 KB of rings on an SM.
-  static constexpr int kSlots = (180 << 10) / (kCtas * kAttnWarps * kTileBytes) < 12
-                                    ? (180 << 10) / (kCtas * kAttnWarps * kTileBytes) : 12;
-  static constexpr int kRing = kAttnWarps * kSlots * kTileBytes;
-  static constexpr int kSmem = kRing + 1024;
+  // Tiles that a warp takes at once: two share the checks of a step, where the registers allow it.
+  static constexpr int kStage = kRows == 8 || kRows * kDim <= 16 * 64 ? 2 : 1;
+  static constexpr uint32_t kNone = kStage == 2 ? 0 : 2;  // of a slot's two bits: no tile is missing
+  static constexpr int kStageBytes = kStage * kTileBytes;
+  // Copies in flight for the HBM's latency: the SM's shared memory, less what the CTAs take beside it.
+  static constexpr int kSlots = (216 << 10) / (kCtas * kAttnWarps * kStageBytes);
+  static constexpr int kRing = kAttnWarps * kSlots * kStageBytes;
   static_assert(kRing >= kAttnWarps * kRows * kDim * 4, "the warps' sums overlay the rings");
 };
 
@@ -187,7 +201,7 @@ template <typename T, int kDim, int kRows>
 __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     attention_kernel(const __grid_constant__ AttentionArgs a) {
   using S = Shape<T, kDim, kRows>;
-  constexpr int kG = S::kGroups, kN = S::kCols;
+  constexpr int kG = S::kGroups, kN = S::kCols, kStage = S::kStage;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kAttnWarps][S::kSlots];
   __shared__ int64_t scan[kAttnWarps];
@@ -250,7 +264,8 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
   int64_t base = found[1] * items;  // of request b on the line
 
   const uint64_t policy = policy_evict_first();
-  uint8_t* const ring = smem + warp * S::kSlots * S::kTileBytes;
+  const Masks masks{kept(0x000f000fu), kept(0x00f000f0u), kept(0x64006400u)};
+  uint8_t* const ring = smem + warp * S::kSlots * S::kStageBytes;
   uint32_t phase = 0;  // parity bit of each slot
   bool dead = false;   // a wait gave up
   for (int64_t at = begin; at < end;) {
@@ -274,13 +289,16 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     int lo = range.first + offset, hi = lo + count;
     if (a.window > 0) lo = max(lo, max(0, pos0 + 1 - a.window) / kKv4Tile);
     hi = pos1 < 0 ? lo : min(hi, pos1 / kKv4Tile + 1);
-    const int warp_tiles = hi - lo > warp ? (hi - lo - warp + kAttnWarps - 1) / kAttnWarps : 0;
+    // The warp's stages: kStage tiles each, every kAttnWarps-th.
+    const int stages = max(0, hi - lo + kStage - 1) / kStage;
+    const int warp_stages = (max(0, stages - warp) + kAttnWarps - 1) / kAttnWarps;
 
     // q as the right operand: this lane's row lane / 4 of each block, its channels in the order of
     // the codes: for each 8 channels the pairs (0, 4), (1, 5), (2, 6), (3, 7).
     uint32_t qf[kN][kG * 4][2];
     // What the products' columns belong to: rows 2 quarter and the next of each block.
     float qsum[kN][kG][2];
+    float factor[kN][2];  // of a score: the softmax's scale (log2) over the row's power of two
     int pos[kN][2];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
@@ -288,31 +306,59 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       const int t = r / a.group;
       const T* qr = static_cast<const T*>(a.q) + b * a.q_batch_stride + t * a.q_token_stride +
                     static_cast<int64_t>(kvh * a.group + r % a.group) * a.q_head_stride;
-      const int my_pos = r < rows ? length - a.queries + t : -1;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) pos[n][e] = __shfl_sync(kFullMask, my_pos, (2 * quarter + e) * 4);
+      uint32_t x[kG][8];
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
-        uint32_t x[8];
-        float sum = 0.0f;
         if (r < rows) {
           const T* from = qr + g * kKv4Group + 16 * quarter;
           if (a.q_vector) {
-            *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(from);
-            *reinterpret_cast<uint4*>(x + 4) = *reinterpret_cast<const uint4*>(from + 8);
+            *reinterpret_cast<uint4*>(x[g]) = *reinterpret_cast<const uint4*>(from);
+            *reinterpret_cast<uint4*>(x[g] + 4) = *reinterpret_cast<const uint4*>(from + 8);
           } else {
             const uint16_t* u = reinterpret_cast<const uint16_t*>(from);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = u[2 * i] | static_cast<uint32_t>(u[2 * i + 1]) << 16;
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint16_t u = static_cast<uint16_t>(x[i / 2] >> (16 * (i % 2)));
-            sum += to_float(*reinterpret_cast<const T*>(&u));
+            for (int i = 0; i < 8; ++i) x[g][i] = u[2 * i] | static_cast<uint32_t>(u[2 * i + 1]) << 16;
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = 0;
+          for (int i = 0; i < 8; ++i) x[g][i] = 0;
+        }
+      }
+      float back = a.scale_log2;
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        // The row's largest element between 1 and 2 (rows of zeros, infinities or NaN as they are).
+        uint32_t largest = 0;
+#pragma unroll
+        for (int g = 0; g < kG; ++g) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) largest = max(largest, max(x[g][i] << 16 & 0x7fffffffu, x[g][i] & 0x7fff0000u));
+        }
+        largest = max(largest, __shfl_xor_sync(kFullMask, largest, 1));
+        largest = max(largest, __shfl_xor_sync(kFullMask, largest, 2));
+        uint32_t field = largest >> 23;
+        field = field == 0 || field == 255 ? 127 : min(max(field, 2u), 252u);
+        const float scale = __uint_as_float((254u - field) << 23);
+        back *= __uint_as_float(field << 23);
+#pragma unroll
+        for (int g = 0; g < kG; ++g) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[g][i] = half2_bits(__floats2half2_rn(bf16_lo(x[g][i]) * scale, bf16_hi(x[g][i]) * scale));
+        }
+      }
+      const int my_pos = r < rows ? length - a.queries + t : -1;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        pos[n][e] = __shfl_sync(kFullMask, my_pos, (2 * quarter + e) * 4);
+        factor[n][e] = __shfl_sync(kFullMask, back, (2 * quarter + e) * 4);
+      }
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 v = __half22float2(*reinterpret_cast<__half2*>(&x[g][i]));
+          sum += v.x;
+          sum += v.y;
         }
         sum += __shfl_xor_sync(kFullMask, sum, 1);
         sum += __shfl_xor_sync(kFullMask, sum, 2);
@@ -320,7 +366,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
         for (int e = 0; e < 2; ++e) qsum[n][g][e] = __shfl_sync(kFullMask, sum, (2 * quarter + e) * 4);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const uint32_t* y = x + 4 * w;
+          const uint32_t* y = x[g] + 4 * w;
           uint32_t(*f)[2] = &qf[n][g * 4 + 2 * w];
           f[0][0] = __byte_perm(y[0], y[2], 0x5410);
           f[0][1] = __byte_perm(y[0], y[2], 0x7632);
@@ -333,15 +379,16 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     // Products with the values: element e of [n][g][m] is channel 8 (lane / 4) + 2 m + e / 2 of group
     // g for row 2 quarter + e % 2 of block n.
     float acc[kN][kG][4][4];
-    float top[kN][2], total_w[kN][2], zeros[kN][kG][2];
+    float top[kN][2], total_w[kN][2], zeros[kN][kG][2];  // top: the running maximum, log2
+    float limit[kN][2], base_w[kN][2];  // top + kRaise, and top or 0 before there is one
     uint32_t unit[kG];  // exponent field of the power of two that the values' weights are divided by
     float inv[kG];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        top[n][e] = -INFINITY;
-        total_w[n][e] = 0.0f;
+        top[n][e] = limit[n][e] = -INFINITY;
+        total_w[n][e] = base_w[n][e] = 0.0f;
       }
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
@@ -356,13 +403,12 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       inv[g] = 1.0f;
     }
 
-    // The warp's k-th tile is lo + warp + 4 k. Where it lies in the cache: 32 of them are looked up at
-    // once, a lane each, one batch ahead of their use; -1 without a page.
+    // Where the tiles lie in the cache: those of 16 stages are looked up at once, a lane each, one
+    // batch ahead of their use; -1 without a page or past the end.
     const int32_t* table = a.page_table + b * a.table_stride;
     auto look_up = [&](int k) -> int32_t {
-      k += lane;
-      if (k >= warp_tiles) return -1;
-      const int tile = lo + warp + k * kAttnWarps;
+      const int tile = lo + kStage * (warp + (k + lane / kStage) * kAttnWarps) + lane % kStage;
+      if (tile >= hi) return -1;
       const int32_t page = table[tile / a.page_tiles];
       if (page < 0 || page >= a.pages) {
         report(kDevIndex);
@@ -370,68 +416,83 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
       return (page * a.kv_heads + kvh) * a.page_tiles + tile % a.page_tiles;
     };
-    int32_t places = look_up(0), places_next = look_up(kWarp);
-    uint32_t missing = 0;  // slots whose tile has no page
+    constexpr int kBatch = kWarp / kStage;
+    int32_t places = look_up(0), places_next = look_up(kBatch);
+    uint32_t missing = 0;  // two bits a slot: tiles that it does not hold
     auto issue = [&](int k, int slot) {
-      if (k % kWarp == 0 && k > 0) {
+      if (k % kBatch == 0 && k > 0) {
         places = places_next;
-        places_next = look_up(k + kWarp);
+        places_next = look_up(k + kBatch);
       }
-      const int32_t place = __shfl_sync(kFullMask, places, k % kWarp);
-      missing = place < 0 ? missing | 1u << slot : missing & ~(1u << slot);
+      const int32_t p0 = __shfl_sync(kFullMask, places, k % kBatch * kStage);
+      const int32_t p1 = kStage == 1 ? -1 : __shfl_sync(kFullMask, places, k % kBatch * kStage + 1);
+      const uint32_t gone = (p0 < 0 ? 1u : 0u) + (p1 < 0 ? 2u : 0u);
+      missing = (missing & ~(3u << 2 * slot)) | gone << 2 * slot;
       if (lane == 0) {
-        if (place < 0) {
-          mbar_arrive(&full[warp][slot]);
+        uint64_t* bar = &full[warp][slot];
+        uint8_t* to = ring + slot * S::kStageBytes;
+        if (gone == 3) {
+          mbar_arrive(bar);
         } else {
-          mbar_arrive_expect_tx(&full[warp][slot], S::kTileBytes);
-          bulk_load(ring + slot * S::kTileBytes, a.cache + static_cast<int64_t>(place) * S::kTileBytes, S::kTileBytes,
-                    &full[warp][slot], policy);
+          mbar_arrive_expect_tx(bar, gone == 0 ? 2 * S::kTileBytes : S::kTileBytes);
+          if (p0 >= 0) bulk_load(to, a.cache + static_cast<int64_t>(p0) * S::kTileBytes, S::kTileBytes, bar, policy);
+          if (p1 >= 0) {
+            bulk_load(to + S::kTileBytes, a.cache + static_cast<int64_t>(p1) * S::kTileBytes, S::kTileBytes, bar, policy);
+          }
         }
       }
     };
-    for (int s = 0; s < S::kSlots && s < warp_tiles; ++s) issue(s, s);
+    for (int s = 0; s < S::kSlots && s < warp_stages; ++s) issue(s, s);
 
-    // One tile. This lane's tokens are row8 and row8 + 8. kMasked: some row does not see some of them.
-    auto tile_step = [&](const uint8_t* tile, int token0, auto masked_tag) {
+    // One stage. This lane's tokens are row8 + 8 j. kMasked: some row does not see some of them, or
+    // a tile is missing.
+    constexpr int kJ = 2 * kStage;
+    auto stage_step = [&](const uint8_t* stage, int token0, uint32_t gone, auto masked_tag) {
       constexpr bool kMasked = decltype(masked_tag)::value;
-      float s[kN][4];  // element e: token row8 + 8 (e / 2), row 2 quarter + e % 2
-      bool off[kN][4];
+      float s[kN][kJ][2];  // element [j][e]: token row8 + 8 j, row 2 quarter + e
+      bool off[kN][kJ][2];
 #pragma unroll
-      for (int n = 0; n < kN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-      uint32_t pairs[2][kG];
+      for (int u = 0; u < kStage; ++u) {
+        const uint8_t* tile = stage + u * S::kTileBytes;
+        uint32_t pairs[2][kG];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) load_words(pairs[j], tile + kv4_key_scale(kDim, 8 * j, 0) + row8 * 4 * kG);
+        for (int j = 0; j < 2; ++j) load_words(pairs[j], tile + kv4_key_scale(kDim, 8 * j, 0) + row8 * 4 * kG);
 #pragma unroll
-      for (int p = 0; p < S::kPlanes; ++p) {
-        uint32_t w[2][2 * S::kWidth];
+        for (int p = 0; p < S::kPlanes; ++p) {
+          uint32_t w[2][2 * S::kWidth];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) load_words(w[j], tile + p * 512 * S::kWidth + (j * kWarp + lane) * 8 * S::kWidth);
+          for (int j = 0; j < 2; ++j) load_words(w[j], tile + p * 512 * S::kWidth + (j * kWarp + lane) * 8 * S::kWidth);
 #pragma unroll
-        for (int i = 0; i < S::kWidth; ++i) {
-          const int g = p * S::kWidth + i;
-          float part[kN][4];
+          for (int i = 0; i < S::kWidth; ++i) {
+            const int g = p * S::kWidth + i;
+            float part[kN][4];
 #pragma unroll
-          for (int n = 0; n < kN; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.0f;
+            for (int c = 0; c < 2; ++c) {
+              uint32_t k0[4], k1[4];
+              unpack(w[0][2 * i + c], masks, k0);
+              unpack(w[1][2 * i + c], masks, k1);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t k0[4], k1[4];
-            unpack<T>(w[0][2 * i + c], k0);
-            unpack<T>(w[1][2 * i + c], k1);
-#pragma unroll
-            for (int n = 0; n < kN; ++n) {
-              mma<T>(part[n], k0[0], k1[0], k0[1], k1[1], qf[n][g * 4 + 2 * c]);
-              mma<T>(part[n], k0[2], k1[2], k0[3], k1[3], qf[n][g * 4 + 2 * c + 1]);
+              for (int n = 0; n < kN; ++n) {
+                if (c == 0) {
+                  mma_first(part[n], k0[0], k1[0], k0[1], k1[1], qf[n][g * 4]);
+                } else {
+                  mma(part[n], k0[0], k1[0], k0[1], k1[1], qf[n][g * 4 + 2]);
+                }
+                mma(part[n], k0[2], k1[2], k0[3], k1[3], qf[n][g * 4 + 2 * c + 1]);
+              }
             }
-          }
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float scale = bf16_lo(pairs[j][g]);
-            const float zero = fmaf(kKeyBias<T>, scale, bf16_hi(pairs[j][g]));
+            for (int j = 0; j < 2; ++j) {
+              const float scale = bf16_lo(pairs[j][g]);
+              const float zero = fmaf(8.0f, scale, bf16_hi(pairs[j][g]));
 #pragma unroll
-            for (int n = 0; n < kN; ++n) {
+              for (int n = 0; n < kN; ++n) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                s[n][2 * j + e] = fmaf(zero, qsum[n][g][e], fmaf(scale, part[n][2 * j + e], s[n][2 * j + e]));
+                for (int e = 0; e < 2; ++e) {
+                  float& to = s[n][2 * u + j][e];
+                  to = g == 0 ? scale * part[n][2 * j + e] : fmaf(scale, part[n][2 * j + e], to);
+                  to = fmaf(zero, qsum[n][g][e], to);
+                }
               }
             }
           }
@@ -442,28 +503,36 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] *= a.scale_log2;
-          if constexpr (kMasked) {
-            const int token = token0 + row8 + 8 * (e / 2), at = pos[n][e % 2];
-            off[n][e] = token > at || (a.window > 0 && token <= at - a.window);
-            if (off[n][e]) s[n][e] = -INFINITY;
+        for (int e = 0; e < 2; ++e) {
+          float m = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < kJ; ++j) {
+            s[n][j][e] *= factor[n][e];
+            if constexpr (kMasked) {
+              const int token = token0 + row8 + 8 * j, at = pos[n][e];
+              off[n][j][e] = token > at || (a.window > 0 && token <= at - a.window) || (gone >> j / 2 & 1u);
+              if (off[n][j][e]) s[n][j][e] = -INFINITY;
+            }
+            m = fmaxf(m, s[n][j][e]);
           }
+          pass = pass || m > limit[n][e];
         }
-        pass = pass || fmaxf(s[n][0], s[n][2]) > top[n][0] + kRaise || fmaxf(s[n][1], s[n][3]) > top[n][1] + kRaise;
       }
       if (__any_sync(kFullMask, pass)) {
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float m = fmaxf(s[n][e], s[n][e + 2]);
+            float m = top[n][e];
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) m = fmaxf(m, s[n][j][e]);
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 4));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16));
-            m = fmaxf(m, top[n][e]);
             const float keep = top[n][e] == m ? 1.0f : exp2_fast(top[n][e] - m);
             top[n][e] = m;
+            limit[n][e] = m + kRaise;
+            base_w[n][e] = m == -INFINITY ? 0.0f : m;
             total_w[n][e] *= keep;
 #pragma unroll
             for (int g = 0; g < kG; ++g) {
@@ -480,81 +549,95 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float m = top[n][e % 2];
-          s[n][e] = exp2_fast(s[n][e] - (m == -INFINITY ? 0.0f : m));
-          total_w[n][e % 2] += s[n][e];
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int j = 0; j < kJ; ++j) {
+            s[n][j][e] = exp2_fast(s[n][j][e] - base_w[n][e]);
+            total_w[n][e] += s[n][j][e];
+          }
         }
       }
       // The values, a group at a time: its scales go into the weights.
+      uint32_t pairs[kJ][kG];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        load_words(pairs[j], tile + kv4_value_scale(kDim, 8 * j, 0) + row8 * 4 * kG);
+      for (int j = 0; j < kJ; ++j) {
+        load_words(pairs[j], stage + j / 2 * S::kTileBytes + kv4_value_scale(kDim, 8 * (j % 2), 0) + row8 * 4 * kG);
         if constexpr (kMasked) {
-          if (token0 + row8 + 8 * j >= length) {  // a place that nothing was written to
+          if (token0 + row8 + 8 * j >= length || (gone >> j / 2 & 1u)) {  // nothing was written there
 #pragma unroll
             for (int g = 0; g < kG; ++g) pairs[j][g] = 0;
           }
         }
       }
 #pragma unroll
-      for (int p = 0; p < S::kPlanes; ++p) {
-        uint32_t w[2][2 * S::kWidth];
+      for (int g = 0; g < kG; ++g) {
+        // Keep the largest scale within 2^4 of the unit; a NaN scale leaves the unit alone.
+        uint32_t largest = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          load_words(w[j], tile + 9 * kDim + p * 512 * S::kWidth + (j * kWarp + lane) * 8 * S::kWidth);
-        }
+        for (int j = 0; j < kJ; ++j) largest = max(largest, pairs[j][g] << 16);
+        const uint32_t field = __reduce_max_sync(kFullMask, largest) >> 23;
+        if (field + 4 - unit[g] > 8 && field != 0 && field < 255) {
+          const uint32_t next = min(field, 253u);
+          const float ratio = __uint_as_float((254u - next) << 23) * __uint_as_float(unit[g] << 23);
+          unit[g] = next;
+          inv[g] = __uint_as_float((254u - next) << 23);
 #pragma unroll
-        for (int i = 0; i < S::kWidth; ++i) {
-          const int g = p * S::kWidth + i;
-          // Keep the largest scale within 2^4 of the unit; a NaN scale leaves the unit alone.
-          const uint32_t field = __reduce_max_sync(kFullMask, max(pairs[0][g] << 16, pairs[1][g] << 16)) >> 23;
-          if (field + 4 - unit[g] > 8 && field != 0 && field < 255) {
-            const uint32_t next = min(field, 253u);
-            const float ratio = __uint_as_float((254u - next) << 23) * __uint_as_float(unit[g] << 23);
-            unit[g] = next;
-            inv[g] = __uint_as_float((254u - next) << 23);
+          for (int n = 0; n < kN; ++n) {
 #pragma unroll
-            for (int n = 0; n < kN; ++n) {
+            for (int m = 0; m < 4; ++m) {
 #pragma unroll
-              for (int m = 0; m < 4; ++m) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[n][g][m][e] *= ratio;
-              }
+              for (int e = 0; e < 4; ++e) acc[n][g][m][e] *= ratio;
             }
           }
-          uint32_t wf[kN][2];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kStage; ++u) {
+        const uint8_t* tile = stage + u * S::kTileBytes;
+#pragma unroll
+        for (int p = 0; p < S::kPlanes; ++p) {
+          uint32_t w[2][2 * S::kWidth];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float scale = bf16_lo(pairs[j][g]), zero = fmaf(8.0f, scale, bf16_hi(pairs[j][g]));
-            const float unit_scale = scale * inv[g];
-#pragma unroll
-            for (int n = 0; n < kN; ++n) {
-              float x[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float weight = s[n][2 * j + e];
-                x[e] = weight * unit_scale;
-                if constexpr (kMasked) {  // a NaN scale must not reach rows that do not see its token
-                  if (off[n][2 * j + e]) {
-                    x[e] = 0.0f;
-                    continue;
-                  }
-                }
-                zeros[n][g][e] = fmaf(weight, zero, zeros[n][g][e]);
-              }
-              wf[n][j] = transpose8(half2_bits(__floats2half2_rn(x[0], x[1])));
-            }
+            load_words(w[j], tile + 9 * kDim + p * 512 * S::kWidth + (j * kWarp + lane) * 8 * S::kWidth);
           }
 #pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            uint32_t v0[4], v1[4];
-            unpack<__half>(w[0][2 * i + d], v0);
-            unpack<__half>(w[1][2 * i + d], v1);
+          for (int i = 0; i < S::kWidth; ++i) {
+            const int g = p * S::kWidth + i;
+            uint32_t wf[kN][2];
 #pragma unroll
-            for (int n = 0; n < kN; ++n) {
-              mma<__half>(acc[n][g][2 * d], v0[0], v0[1], v1[0], v1[1], wf[n]);
-              mma<__half>(acc[n][g][2 * d + 1], v0[2], v0[3], v1[2], v1[3], wf[n]);
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t pair = pairs[2 * u + j][g];
+              const float scale = bf16_lo(pair), zero = fmaf(8.0f, scale, bf16_hi(pair));
+              const float unit_scale = scale * inv[g];
+#pragma unroll
+              for (int n = 0; n < kN; ++n) {
+                float x[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float weight = s[n][2 * u + j][e];
+                  x[e] = weight * unit_scale;
+                  if constexpr (kMasked) {  // a NaN scale must not reach rows that do not see its token
+                    if (off[n][2 * u + j][e]) {
+                      x[e] = 0.0f;
+                      continue;
+                    }
+                  }
+                  zeros[n][g][e] = fmaf(weight, zero, zeros[n][g][e]);
+                }
+                wf[n][j] = transpose8(half2_bits(__floats2half2_rn(x[0], x[1])));
+              }
+            }
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+              uint32_t v0[4], v1[4];
+              unpack(w[0][2 * i + d], masks, v0);
+              unpack(w[1][2 * i + d], masks, v1);
+#pragma unroll
+              for (int n = 0; n < kN; ++n) {
+                mma(acc[n][g][2 * d], v0[0], v0[1], v1[0], v1[1], wf[n]);
+                mma(acc[n][g][2 * d + 1], v0[2], v0[3], v1[2], v1[3], wf[n]);
+              }
             }
           }
         }
@@ -562,20 +645,21 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     };
 
     int slot = 0;
-    for (int k = 0; k < warp_tiles; ++k) {
+    for (int k = 0; k < warp_stages; ++k) {
       if (!dead) dead = !__all_sync(kFullMask, mbar_wait(&full[warp][slot], phase >> slot & 1u));
       phase ^= 1u << slot;
-      if (!(missing >> slot & 1u) && !dead) {
-        const uint8_t* tile = ring + slot * S::kTileBytes;
-        const int token0 = (lo + warp + k * kAttnWarps) * kKv4Tile;
-        if (token0 + kKv4Tile - 1 <= pos0 && (a.window <= 0 || token0 > pos1 - a.window)) {
-          tile_step(tile, token0, std::false_type{});
+      const uint32_t gone = missing >> 2 * slot & 3u;
+      if (gone != 3 && !dead) {
+        const uint8_t* stage = ring + slot * S::kStageBytes;
+        const int token0 = (lo + kStage * (warp + k * kAttnWarps)) * kKv4Tile;
+        if (gone == S::kNone && token0 + kStage * kKv4Tile - 1 <= pos0 && (a.window <= 0 || token0 > pos1 - a.window)) {
+          stage_step(stage, token0, 0, std::false_type{});
         } else {
-          tile_step(tile, token0, std::true_type{});
+          stage_step(stage, token0, gone, std::true_type{});
         }
       }
       __syncwarp();
-      if (k + S::kSlots < warp_tiles && !dead) issue(k + S::kSlots, slot);
+      if (k + S::kSlots < warp_stages && !dead) issue(k + S::kSlots, slot);
       slot = slot + 1 == S::kSlots ? 0 : slot + 1;
     }
 
@@ -748,7 +832,7 @@ cudaError_t launch(const AttentionArgs& a, cudaStream_t stream) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
     const cudaError_t err = cudaFuncSetAttribute(attention_kernel<T, kDim, kRows>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, S::kRing);
     if (err != cudaSuccess) return err;
     configured[dev] = true;
   }
@@ -758,7 +842,7 @@ cudaError_t launch(const AttentionArgs& a, cudaStream_t stream) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(a.parts));
   config.blockDim = dim3(kAttnThreads);
-  config.dynamicSmemBytes = S::kSmem;
+  config.dynamicSmemBytes = S::kRing;
   config.stream = stream;
   config.attrs = &attr;
   config.numAttrs = 1;
