@@ -8,10 +8,13 @@
 //     channels, values: channels x tokens), which fills mma.sync's 16 rows even for a single query
 //     row, and a lane then meets the scales of only two tokens. tcgen05 would want the unpacked codes
 //     written to shared memory first, which alone would exceed its bandwidth at two codes a byte.
-//   - Codes are unpacked to binary16 with a mask and an or (the four bits become the low mantissa
-//     bits of 1024 + n) and one exact subtraction, two codes an instruction; bfloat16 queries become
-//     binary16 exactly, scaled by a power of two (what falls below 2^-24 of a row's largest element
-//     is lost, as it would be in a binary32 sum). Scales never touch the codes: with k = code * s + z,
+//   - Codes are unpacked to binary16 with a mask and an or, two codes an instruction: the four bits
+//     become mantissa bits of 1024 + n or 1024 + 16 n. Against the keys that excess, the same for
+//     every token, is the start of the product's sum (it costs the binary32 sum 7 of its 24 bits
+//     against the size of a code, far below what the 4 bits lost); the values' codes are brought
+//     to n - 8, exactly, since there it would add up over tokens whose values cancel. Queries become
+//     binary16 scaled by a power of two of their row. Scales never touch the codes: with
+//     k = code * s + z,
 //       q.k = sum over groups of s (q.code) + z sum(q),
 //     and for the values the weight p s of a token and group goes into the matrix product instead
 //     of p; sum of p z is added at the end.
@@ -105,12 +108,12 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
 }
 
-// The same, from zero.
-__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                          const uint32_t (&b)[2]) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+// The same, from c.
+__device__ __forceinline__ void mma_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         const uint32_t (&b)[2], const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(0.0f));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
 // Transposes an 8 x 8 matrix of 16-bit elements held two to a lane.
@@ -140,18 +143,35 @@ struct Masks {
   uint32_t low, high, bits;
 };
 
-// Four pairs of codes of a 32-bit word, nibbles (i, i + 4), as binary16 code - 8, exactly: 1024 + n
-// and 1024 + 16 n have the codes in their mantissas.
+// Four pairs of codes of a 32-bit word, nibbles (i, i + 4), in the mantissas of binary16 numbers:
+// 1024 + n in the even pairs and 1024 + 16 n in the odd ones.
+__device__ __forceinline__ void unpack_raw(uint32_t w, const Masks& k, uint32_t (&out)[4]) {
+  out[0] = and_or(w, k.low, k.bits);
+  out[1] = and_or(w, k.high, k.bits);
+  w >>= 8;
+  out[2] = and_or(w, k.low, k.bits);
+  out[3] = and_or(w, k.high, k.bits);
+}
+
+// The same as n - 8, exactly.
 __device__ __forceinline__ void unpack(uint32_t w, const Masks& k, uint32_t (&out)[4]) {
   const __half2 low = __floats2half2_rn(1032.0f, 1032.0f);
   const __half2 part = __floats2half2_rn(0.0625f, 0.0625f), high = __floats2half2_rn(-72.0f, -72.0f);
+  unpack_raw(w, k, out);
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
-    uint32_t x = and_or(w, k.low, k.bits);
-    uint32_t y = and_or(w, k.high, k.bits);
-    out[i] = half2_bits(__hsub2(*reinterpret_cast<__half2*>(&x), low));
-    out[i + 1] = half2_bits(__hfma2(*reinterpret_cast<__half2*>(&y), part, high));
-    w >>= 8;
+    out[i] = half2_bits(__hsub2(*reinterpret_cast<__half2*>(&out[i]), low));
+    out[i + 1] = half2_bits(__hfma2(*reinterpret_cast<__half2*>(&out[i + 1]), part, high));
+  }
+}
+
+// Two elements of T as binary32.
+template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t v) {
+  if constexpr (std::is_same_v<T, __half>) {
+    return __half22float2(*reinterpret_cast<__half2*>(&v));
+  } else {
+    return make_float2(bf16_lo(v), bf16_hi(v));
   }
 }
 
@@ -298,6 +318,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     uint32_t qf[kN][kG * 4][2];
     // What the products' columns belong to: rows 2 quarter and the next of each block.
     float qsum[kN][kG][2];
+    float excess[kN][kG][2];  // what the 1024 beside each code adds to a product, negated
     float factor[kN][2];  // of a score: the softmax's scale (log2) over the row's power of two
     int pos[kN][2];
 #pragma unroll
@@ -324,27 +345,23 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
           for (int i = 0; i < 8; ++i) x[g][i] = 0;
         }
       }
-      float back = a.scale_log2;
-      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-        // The row's largest element between 1 and 2 (rows of zeros, infinities or NaN as they are).
-        uint32_t largest = 0;
+      // The row as binary16, its largest element between 16 and 32 by a power of two (rows of zeros,
+      // infinities or NaN as they are): what is lost of small elements is below 2^-25 of the largest.
+      uint32_t largest = 0;
 #pragma unroll
-        for (int g = 0; g < kG; ++g) {
+      for (int g = 0; g < kG; ++g) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) largest = max(largest, max(x[g][i] << 16 & 0x7fffffffu, x[g][i] & 0x7fff0000u));
-        }
-        largest = max(largest, __shfl_xor_sync(kFullMask, largest, 1));
-        largest = max(largest, __shfl_xor_sync(kFullMask, largest, 2));
-        uint32_t field = largest >> 23;
-        field = field == 0 || field == 255 ? 127 : min(max(field, 2u), 252u);
-        const float scale = __uint_as_float((254u - field) << 23);
-        back *= __uint_as_float(field << 23);
-#pragma unroll
-        for (int g = 0; g < kG; ++g) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[g][i] = half2_bits(__floats2half2_rn(bf16_lo(x[g][i]) * scale, bf16_hi(x[g][i]) * scale));
+        for (int i = 0; i < 8; ++i) {
+          const float2 v = unpack_pair<T>(x[g][i]);
+          largest = max(largest, max(__float_as_uint(fabsf(v.x)), __float_as_uint(fabsf(v.y))));
         }
       }
+      largest = max(largest, __shfl_xor_sync(kFullMask, largest, 1));
+      largest = max(largest, __shfl_xor_sync(kFullMask, largest, 2));
+      uint32_t field = largest >> 23;
+      field = field == 0 || field == 255 ? 131 : min(max(field, 8u), 250u);
+      const float scale = __uint_as_float((258u - field) << 23);
+      const float back = a.scale_log2 * __uint_as_float((field - 4u) << 23);
       const int my_pos = r < rows ? length - a.queries + t : -1;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -353,17 +370,28 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
-        float sum = 0.0f;
+        float sum = 0.0f, held = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float2 v = __half22float2(*reinterpret_cast<__half2*>(&x[g][i]));
+          // Channels that meet 16 n (the odd pairs: 1, 3, 5, 7 of each 8) are divided by 16.
+          float2 v = unpack_pair<T>(x[g][i]);
+          const __half2 h = __floats2half2_rn(v.x * scale, v.y * (scale * 0.0625f));
+          x[g][i] = half2_bits(h);
+          v = __half22float2(h);
           sum += v.x;
-          sum += v.y;
+          sum = fmaf(16.0f, v.y, sum);
+          held += v.x;
+          held += v.y;
         }
         sum += __shfl_xor_sync(kFullMask, sum, 1);
         sum += __shfl_xor_sync(kFullMask, sum, 2);
+        held += __shfl_xor_sync(kFullMask, held, 1);
+        held += __shfl_xor_sync(kFullMask, held, 2);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) qsum[n][g][e] = __shfl_sync(kFullMask, sum, (2 * quarter + e) * 4);
+        for (int e = 0; e < 2; ++e) {
+          qsum[n][g][e] = __shfl_sync(kFullMask, sum, (2 * quarter + e) * 4);
+          excess[n][g][e] = -1024.0f * __shfl_sync(kFullMask, held, (2 * quarter + e) * 4);
+        }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const uint32_t* y = x[g] + 4 * w;
@@ -469,12 +497,14 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               uint32_t k0[4], k1[4];
-              unpack(w[0][2 * i + c], masks, k0);
-              unpack(w[1][2 * i + c], masks, k1);
+              unpack_raw(w[0][2 * i + c], masks, k0);
+              unpack_raw(w[1][2 * i + c], masks, k1);
 #pragma unroll
               for (int n = 0; n < kN; ++n) {
                 if (c == 0) {
-                  mma_first(part[n], k0[0], k1[0], k0[1], k1[1], qf[n][g * 4]);
+                  // (several blocks of rows leave no registers for the sums' starts: they are added below)
+                  const float x0 = kN == 1 ? excess[n][g][0] : 0.0f, x1 = kN == 1 ? excess[n][g][1] : 0.0f;
+                  mma_from(part[n], k0[0], k1[0], k0[1], k1[1], qf[n][g * 4], {x0, x1, x0, x1});
                 } else {
                   mma(part[n], k0[0], k1[0], k0[1], k1[1], qf[n][g * 4 + 2]);
                 }
@@ -484,13 +514,14 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const float scale = bf16_lo(pairs[j][g]);
-              const float zero = fmaf(8.0f, scale, bf16_hi(pairs[j][g]));
+              const float zero = bf16_hi(pairs[j][g]);
 #pragma unroll
               for (int n = 0; n < kN; ++n) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   float& to = s[n][2 * u + j][e];
-                  to = g == 0 ? scale * part[n][2 * j + e] : fmaf(scale, part[n][2 * j + e], to);
+                  const float x = kN == 1 ? part[n][2 * j + e] : part[n][2 * j + e] + excess[n][g][e];
+                  to = g == 0 ? scale * x : fmaf(scale, x, to);
                   to = fmaf(zero, qsum[n][g][e], to);
                 }
               }
