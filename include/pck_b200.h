@@ -448,7 +448,7 @@ int pck_kv4_append(void* cache, int64_t pages, int64_t kv_heads, int64_t page_ti
  * tokens' own, in the pages page_table[b * table_stride ...] (table_pages columns; lengths beyond
  * them are cut). Query token t sees the tokens j <= lengths[b] - queries + t, with window > 0 only
  * the last `window` of them: out = softmax(scale * q k^T) v, (batch, queries, heads, dim) of q's
- * type, contiguous. A query that sees no token gives zeros. `scratch` holds at least
+ * type, contiguous, 8-byte aligned. A query that sees no token gives zeros. `scratch` holds at least
  * pck_kv4_attention_scratch(...) bytes (0: none needed), 256-byte aligned, of no meaning before
  * and after the call.
  */

@@ -38,9 +38,14 @@ namespace {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * kWarp;
-constexpr int kMinTiles = 8;        // tiles of a part, at least: two for each warp
+// What beginning and ending an item costs a CTA (its queries, the first copies' latency, the join of
+// its warps), in tiles: items count as that much longer when the line is cut, or the parts that hold
+// many short items would end last.
+constexpr int kItemCost = 8;
+constexpr int kMinPart = 16;  // length of a part, at least
 constexpr float kRaise = 8.0f;      // log2 by which a score may pass the running maximum
-constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 4;     // rows of a joining CTA, four warps each
+constexpr int kJoinThreads = kJoinRows * 4 * kWarp;
 
 struct AttentionArgs {
   const void* q;
@@ -53,6 +58,7 @@ struct AttentionArgs {
   void* out;
   float* sums;        // (2 * parts, rows, dim) unnormalised outputs of split items
   float2* top_total;  // (2 * parts, rows): maximum (log2), sum of weights
+  int2* split;        // (batch, kv_heads, row_blocks): the first part of an item, and how many it has
   float scale_log2;
   int64_t batch;
   int32_t window;
@@ -78,20 +84,12 @@ __device__ __forceinline__ Range request_tiles(const AttentionArgs& a, int64_t b
   return {first, (length - 1) / kKv4Tile - first + 1};
 }
 
-template <int kThreads>
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* shared) {
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-  __syncthreads();
-  if (threadIdx.x % kWarp == 0) shared[threadIdx.x / kWarp] = v;
-  __syncthreads();
-  v = 0;
-  for (int w = 0; w < kThreads / kWarp; ++w) v += shared[w];
-  return v;
-}
+// An item's length on the line.
+__device__ __forceinline__ int item_length(int tiles) { return tiles > 0 ? tiles + kItemCost : 0; }
 
-// Parts the line of `total` tiles is cut into, and where part c begins.
+// Parts the line is cut into, and where part c begins.
 __device__ __forceinline__ int64_t part_count(const AttentionArgs& a, int64_t total) {
-  return max(int64_t{1}, min(static_cast<int64_t>(a.parts), total / kMinTiles));
+  return max(int64_t{1}, min(static_cast<int64_t>(a.parts), total / kMinPart));
 }
 __device__ __forceinline__ int64_t part_begin(int64_t total, int64_t parts, int64_t c) { return total * c / parts; }
 
@@ -217,6 +215,19 @@ struct Shape {
   static_assert(kRing >= kAttnWarps * kRows * kDim * 4, "the warps' sums overlay the rings");
 };
 
+// Four channels of a row: sums over the sum of weights (zeros for a row that saw nothing).
+template <typename T>
+__device__ __forceinline__ void store_row(T* to, float4 o, float l) {
+  const float v[4] = {o.x, o.y, o.z, o.w};
+  uint16_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const T x = from_float<T>(l == 0.0f ? 0.0f : v[i] / l);
+    u[i] = *reinterpret_cast<const uint16_t*>(&x);
+  }
+  *reinterpret_cast<uint2*>(to) = make_uint2(u[0] | static_cast<uint32_t>(u[1]) << 16, u[2] | static_cast<uint32_t>(u[3]) << 16);
+}
+
 template <typename T, int kDim, int kRows>
 __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     attention_kernel(const __grid_constant__ AttentionArgs a) {
@@ -224,8 +235,6 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
   constexpr int kG = S::kGroups, kN = S::kCols, kStage = S::kStage;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kAttnWarps][S::kSlots];
-  __shared__ int64_t scan[kAttnWarps];
-  __shared__ int64_t found[2];
   __shared__ float2 state[kAttnWarps][kRows];
 
   const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
@@ -240,48 +249,42 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 
   // Requests that hold nothing give zeros.
   T* const out = static_cast<T*>(a.out);
+  const int64_t items = static_cast<int64_t>(a.kv_heads) * a.row_blocks;  // of a request
   const int64_t row_size = static_cast<int64_t>(a.queries) * a.heads * kDim;
   for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
     if (request_tiles(a, b).tiles == 0) {
       for (int64_t i = tid; i < row_size; i += kAttnThreads) out[b * row_size + i] = from_float<T>(0.0f);
+      for (int64_t i = tid; a.parts > 1 && i < items; i += kAttnThreads) a.split[b * items + i] = make_int2(0, 0);
     }
   }
 
-  // This CTA's part of the line of tiles: items in the order (request, head, row block).
-  const int64_t items = static_cast<int64_t>(a.kv_heads) * a.row_blocks;  // of a request
-  int64_t mine = 0;
-  for (int64_t b = tid; b < a.batch; b += kAttnThreads) mine += request_tiles(a, b).tiles;
-  const int64_t total = block_sum<kAttnThreads>(mine, scan) * items;
+  // This CTA's part of the line of items, in the order (request, head, row block); every warp for itself.
+  int64_t total = 0;
+  for (int64_t i = lane; i < a.batch; i += kWarp) total += item_length(request_tiles(a, i).tiles);
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(kFullMask, total, o);
+  total *= items;
   const int64_t parts = part_count(a, total);
   if (blockIdx.x >= parts) return;
   const int64_t begin = part_begin(total, parts, blockIdx.x), end = part_begin(total, parts, blockIdx.x + 1);
   if (begin >= end) return;
-  // The request in which it begins: its tiles hold `begin` between them.
-  int64_t carry = 0;
-  for (int64_t b0 = 0; b0 < a.batch; b0 += kAttnThreads) {
-    const int64_t b = b0 + tid;
-    const int64_t n = b < a.batch ? request_tiles(a, b).tiles : 0;
+  // The request in which it begins, and where that begins.
+  int64_t b = 0, base = 0;
+  for (; b < a.batch; b += kWarp) {
+    const int64_t n = b + lane < a.batch ? item_length(request_tiles(a, b + lane).tiles) * items : 0;
     int64_t before = n;
     for (int o = 1; o < kWarp; o <<= 1) {
       const int64_t v = __shfl_up_sync(kFullMask, before, o);
       if (lane >= o) before += v;
     }
-    __syncthreads();
-    if (lane == kWarp - 1) scan[warp] = before;
-    __syncthreads();
-    before += carry - n;
-    for (int w = 0; w < kAttnWarps; ++w) {
-      if (w < warp) before += scan[w];
-      carry += scan[w];
+    const unsigned here = __ballot_sync(kFullMask, begin < base + before);
+    if (here) {
+      const int l = __ffs(here) - 1;
+      b += l;
+      base += __shfl_sync(kFullMask, before - n, l);
+      break;
     }
-    if (n > 0 && before * items <= begin && begin < (before + n) * items) {
-      found[0] = b;
-      found[1] = before;
-    }
+    base += __shfl_sync(kFullMask, before, kWarp - 1);
   }
-  __syncthreads();
-  int64_t b = found[0];
-  int64_t base = found[1] * items;  // of request b on the line
 
   const uint64_t policy = policy_evict_first();
   const Masks masks{kept(0x000f000fu), kept(0x00f000f0u), kept(0x64006400u)};
@@ -290,16 +293,32 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
   bool dead = false;   // a wait gave up
   for (int64_t at = begin; at < end;) {
     const Range range = request_tiles(a, b);
-    if (at >= base + range.tiles * items) {
-      base += range.tiles * items;
+    const int size = item_length(range.tiles);
+    if (at >= base + size * items) {
+      base += size * items;
       ++b;
       continue;
     }
-    const int64_t item = (at - base) / range.tiles;
-    const int offset = static_cast<int>((at - base) % range.tiles);
-    const int count = static_cast<int>(min(static_cast<int64_t>(range.tiles - offset), end - at));
+    const int64_t item = (at - base) / size;
+    const int start = static_cast<int>((at - base) % size);
+    const int stop = static_cast<int>(min(static_cast<int64_t>(size), start + (end - at)));
+    at += stop - start;
+    // Its tiles come after its cost.
+    const int offset = max(0, start - kItemCost), count = max(0, stop - kItemCost) - offset;
+    if (count == 0) continue;
     const int kvh = static_cast<int>(item / a.row_blocks), block = static_cast<int>(item % a.row_blocks);
     const bool whole = count == range.tiles;
+    if (offset == 0 && a.parts > 1 && tid == 0) {
+      // Parts from this one to the one with the item's last place.
+      int64_t last = blockIdx.x;
+      if (!whole) {
+        const int64_t x = base + (item + 1) * size - 1;
+        last = x * parts / total;
+        while (last + 1 < parts && part_begin(total, parts, last + 1) <= x) ++last;
+        while (part_begin(total, parts, last) > x) --last;
+      }
+      a.split[b * items + item] = make_int2(blockIdx.x, static_cast<int>(last - blockIdx.x + 1));
+    }
     const int length = min(a.lengths[b], a.max_tokens);
     const int rows = a.queries * a.group;
     const int row0 = block * kRows;
@@ -312,6 +331,47 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     // The warp's stages: kStage tiles each, every kAttnWarps-th.
     const int stages = max(0, hi - lo + kStage - 1) / kStage;
     const int warp_stages = (max(0, stages - warp) + kAttnWarps - 1) / kAttnWarps;
+
+    // Where the tiles lie in the cache: those of 16 stages are looked up at once, a lane each, one
+    // batch ahead of their use; -1 without a page or past the end.
+    const int32_t* table = a.page_table + b * a.table_stride;
+    auto look_up = [&](int k) -> int32_t {
+      const int tile = lo + kStage * (warp + (k + lane / kStage) * kAttnWarps) + lane % kStage;
+      if (tile >= hi) return -1;
+      const int32_t page = table[tile / a.page_tiles];
+      if (page < 0 || page >= a.pages) {
+        report(kDevIndex);
+        return -1;
+      }
+      return (page * a.kv_heads + kvh) * a.page_tiles + tile % a.page_tiles;
+    };
+    constexpr int kBatch = kWarp / kStage;
+    int32_t places = look_up(0), places_next = look_up(kBatch);
+    uint32_t missing = 0;  // two bits a slot: tiles that it does not hold
+    auto issue = [&](int k, int slot) {
+      if (k % kBatch == 0 && k > 0) {
+        places = places_next;
+        places_next = look_up(k + kBatch);
+      }
+      const int32_t p0 = __shfl_sync(kFullMask, places, k % kBatch * kStage);
+      const int32_t p1 = kStage == 1 ? -1 : __shfl_sync(kFullMask, places, k % kBatch * kStage + 1);
+      const uint32_t gone = (p0 < 0 ? 1u : 0u) + (p1 < 0 ? 2u : 0u);
+      missing = (missing & ~(3u << 2 * slot)) | gone << 2 * slot;
+      if (lane == 0) {
+        uint64_t* bar = &full[warp][slot];
+        uint8_t* to = ring + slot * S::kStageBytes;
+        if (gone == 3) {
+          mbar_arrive(bar);
+        } else {
+          mbar_arrive_expect_tx(bar, gone == 0 ? 2 * S::kTileBytes : S::kTileBytes);
+          if (p0 >= 0) bulk_load(to, a.cache + static_cast<int64_t>(p0) * S::kTileBytes, S::kTileBytes, bar, policy);
+          if (p1 >= 0) {
+            bulk_load(to + S::kTileBytes, a.cache + static_cast<int64_t>(p1) * S::kTileBytes, S::kTileBytes, bar, policy);
+          }
+        }
+      }
+    };
+    for (int s = 0; s < S::kSlots && s < warp_stages; ++s) issue(s, s);
 
     // q as the right operand: this lane's row lane / 4 of each block, its channels in the order of
     // the codes: for each 8 channels the pairs (0, 4), (1, 5), (2, 6), (3, 7).
@@ -408,7 +468,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     // g for row 2 quarter + e % 2 of block n.
     float acc[kN][kG][4][4];
     float top[kN][2], total_w[kN][2], zeros[kN][kG][2];  // top: the running maximum, log2
-    float limit[kN][2], base_w[kN][2];  // top + kRaise, and top or 0 before there is one
+    float limit[kN][2], base_w[kN][2];  // the score at top + kRaise, and top or 0 before there is one
     uint32_t unit[kG];  // exponent field of the power of two that the values' weights are divided by
     float inv[kG];
 #pragma unroll
@@ -430,47 +490,6 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       unit[g] = 127;
       inv[g] = 1.0f;
     }
-
-    // Where the tiles lie in the cache: those of 16 stages are looked up at once, a lane each, one
-    // batch ahead of their use; -1 without a page or past the end.
-    const int32_t* table = a.page_table + b * a.table_stride;
-    auto look_up = [&](int k) -> int32_t {
-      const int tile = lo + kStage * (warp + (k + lane / kStage) * kAttnWarps) + lane % kStage;
-      if (tile >= hi) return -1;
-      const int32_t page = table[tile / a.page_tiles];
-      if (page < 0 || page >= a.pages) {
-        report(kDevIndex);
-        return -1;
-      }
-      return (page * a.kv_heads + kvh) * a.page_tiles + tile % a.page_tiles;
-    };
-    constexpr int kBatch = kWarp / kStage;
-    int32_t places = look_up(0), places_next = look_up(kBatch);
-    uint32_t missing = 0;  // two bits a slot: tiles that it does not hold
-    auto issue = [&](int k, int slot) {
-      if (k % kBatch == 0 && k > 0) {
-        places = places_next;
-        places_next = look_up(k + kBatch);
-      }
-      const int32_t p0 = __shfl_sync(kFullMask, places, k % kBatch * kStage);
-      const int32_t p1 = kStage == 1 ? -1 : __shfl_sync(kFullMask, places, k % kBatch * kStage + 1);
-      const uint32_t gone = (p0 < 0 ? 1u : 0u) + (p1 < 0 ? 2u : 0u);
-      missing = (missing & ~(3u << 2 * slot)) | gone << 2 * slot;
-      if (lane == 0) {
-        uint64_t* bar = &full[warp][slot];
-        uint8_t* to = ring + slot * S::kStageBytes;
-        if (gone == 3) {
-          mbar_arrive(bar);
-        } else {
-          mbar_arrive_expect_tx(bar, gone == 0 ? 2 * S::kTileBytes : S::kTileBytes);
-          if (p0 >= 0) bulk_load(to, a.cache + static_cast<int64_t>(p0) * S::kTileBytes, S::kTileBytes, bar, policy);
-          if (p1 >= 0) {
-            bulk_load(to + S::kTileBytes, a.cache + static_cast<int64_t>(p1) * S::kTileBytes, S::kTileBytes, bar, policy);
-          }
-        }
-      }
-    };
-    for (int s = 0; s < S::kSlots && s < warp_stages; ++s) issue(s, s);
 
     // One stage. This lane's tokens are row8 + 8 j. kMasked: some row does not see some of them, or
     // a tile is missing.
@@ -538,7 +557,6 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
           float m = -INFINITY;
 #pragma unroll
           for (int j = 0; j < kJ; ++j) {
-            s[n][j][e] *= factor[n][e];
             if constexpr (kMasked) {
               const int token = token0 + row8 + 8 * j, at = pos[n][e];
               off[n][j][e] = token > at || (a.window > 0 && token <= at - a.window) || (gone >> j / 2 & 1u);
@@ -554,15 +572,16 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
         for (int n = 0; n < kN; ++n) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float m = top[n][e];
+            float m = s[n][0][e];
 #pragma unroll
-            for (int j = 0; j < kJ; ++j) m = fmaxf(m, s[n][j][e]);
+            for (int j = 1; j < kJ; ++j) m = fmaxf(m, s[n][j][e]);
+            m = fmaxf(top[n][e], m * factor[n][e]);
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 4));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16));
             const float keep = top[n][e] == m ? 1.0f : exp2_fast(top[n][e] - m);
             top[n][e] = m;
-            limit[n][e] = m + kRaise;
+            limit[n][e] = (m + kRaise) / factor[n][e];
             base_w[n][e] = m == -INFINITY ? 0.0f : m;
             total_w[n][e] *= keep;
 #pragma unroll
@@ -583,7 +602,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int j = 0; j < kJ; ++j) {
-            s[n][j][e] = exp2_fast(s[n][j][e] - base_w[n][e]);
+            s[n][j][e] = exp2_fast(fmaf(s[n][j][e], factor[n][e], -base_w[n][e]));
             total_w[n][e] += s[n][j][e];
           }
         }
@@ -721,107 +740,105 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
     }
     __syncthreads();
-    const int64_t slot_id = 2 * static_cast<int64_t>(blockIdx.x) + (at == begin ? 0 : 1);
+    const int64_t slot_id = 2 * static_cast<int64_t>(blockIdx.x) + (offset == 0 ? 1 : 0);
     const int kept = min(kRows, rows - row0);
-    for (int i = tid; i < kept * kDim; i += kAttnThreads) {
+    for (int i = 4 * tid; i < kept * kDim; i += 4 * kAttnThreads) {
       const int r = i / kDim, c = i % kDim;
       float m = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kAttnWarps; ++w) m = fmaxf(m, state[w][r].x);
-      float o = 0.0f, l = 0.0f;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float l = 0.0f;
 #pragma unroll
       for (int w = 0; w < kAttnWarps; ++w) {
         const float f = state[w][r].x == -INFINITY ? 0.0f : exp2_fast(state[w][r].x - m);
-        o = fmaf(f, sums[(w * kRows + r) * kDim + c], o);
+        const float4 v = *reinterpret_cast<const float4*>(sums + (w * kRows + r) * kDim + c);
+        o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
         l = fmaf(f, state[w][r].y, l);
       }
       if (whole) {
         const int t = (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
-        out[((b * a.queries + t) * a.heads + head) * kDim + c] = from_float<T>(l == 0.0f ? 0.0f : o / l);
+        store_row(out + ((b * a.queries + t) * a.heads + head) * kDim + c, o, l);
       } else {
-        a.sums[(slot_id * kRows + r) * kDim + c] = o;
+        *reinterpret_cast<float4*>(a.sums + (slot_id * kRows + r) * kDim + c) = o;
         if (c == 0) a.top_total[slot_id * kRows + r] = make_float2(m, l);
       }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next bulk copies land here
     __syncthreads();
-    at += count;
   }
 }
 
-// Joins the parts of split items: a CTA for each (request, head, row).
+// Joins the parts of split items: a CTA for each four rows of an item, four warps a row.
 template <typename T, int kDim, int kRows>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttentionArgs a) {
-  constexpr int kWarps = kJoinThreads / kWarp;
-  constexpr int kPer = kDim / kWarp;
+  constexpr int kVectors = kDim / 128 > 1 ? 2 : 1;  // float4 of a lane (dim 64: half the lanes)
   extern __shared__ float weight[];
-  __shared__ int64_t scan[kWarps];
-  __shared__ float sums[kWarps][kDim];
-  __shared__ float red[2][kWarps];
-  const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
-  const int rows = a.queries * a.group;
-  const int r = static_cast<int>(blockIdx.x % rows);
-  const int kvh = static_cast<int>(blockIdx.x / rows % a.kv_heads);
-  const int64_t b = blockIdx.x / rows / a.kv_heads;
-  const int64_t items = static_cast<int64_t>(a.kv_heads) * a.row_blocks;
+  __shared__ float4 sums[kJoinRows][4][kDim / 4];
+  __shared__ float red[kJoinRows][4][2];
+  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp, w = warp % 4;
+  const int chunks = (min(kRows, a.queries * a.group) + kJoinRows - 1) / kJoinRows;
+  const int64_t item = blockIdx.x / chunks;
+  const int in_block = static_cast<int>(blockIdx.x % chunks) * kJoinRows + warp / 4;
+  const int row = static_cast<int>(item % a.row_blocks) * kRows + in_block;
+  const bool mine = in_block < kRows && row < a.queries * a.group;
   wait_for_producers();
-  int64_t all = 0, before = 0;
-  for (int64_t i = tid; i < a.batch; i += kJoinThreads) {
-    const int64_t n = request_tiles(a, i).tiles;
-    all += n;
-    before += i < b ? n : 0;
-  }
-  const int64_t total = block_sum<kJoinThreads>(all, scan) * items;
-  before = block_sum<kJoinThreads>(before, scan);
-  const int64_t tiles = request_tiles(a, b).tiles;
-  if (tiles == 0) return;
-  const int64_t parts = part_count(a, total);
-  const int64_t first = before * items + (kvh * static_cast<int64_t>(a.row_blocks) + r / kRows) * tiles;
-  const int64_t last = first + tiles - 1;
-  // Parts that hold the item's first and last tile.
-  auto part_of = [&](int64_t x) {
-    int64_t c = x * parts / total;
-    while (c + 1 < parts && part_begin(total, parts, c + 1) <= x) ++c;
-    while (part_begin(total, parts, c) > x) --c;
-    return c;
-  };
-  const int64_t c0 = part_of(first), c1 = part_of(last);
-  if (c0 == c1) return;  // the attention kernel wrote the whole item
-  const int n = static_cast<int>(c1 - c0 + 1);
-  auto slot_of = [&](int i) { return 2 * (c0 + i) + (first <= part_begin(total, parts, c0 + i) ? 0 : 1); };
+  const int2 split = a.split[item];
+  const int n = split.y;
+  if (n <= 1) return;  // nothing to join
+  // The part that holds the item's beginning has it in its second slot, the others in their first.
+  auto slot_of = [&](int i) { return (2 * (static_cast<int64_t>(split.x) + i) + (i == 0 ? 1 : 0)) * kRows + in_block; };
   float m = -INFINITY;
-  for (int i = tid; i < n; i += kJoinThreads) m = fmaxf(m, a.top_total[slot_of(i) * kRows + r % kRows].x);
+  for (int i = w * kWarp + lane; mine && i < n; i += 4 * kWarp) m = fmaxf(m, a.top_total[slot_of(i)].x);
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
-  if (lane == 0) red[0][warp] = m;
+  if (lane == 0) red[warp / 4][w][0] = m;
   __syncthreads();
-  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red[0][w]);
+  for (int i = 0; i < 4; ++i) m = fmaxf(m, red[warp / 4][i][0]);
+  float* const my_weight = weight + warp / 4 * n;
   float l = 0.0f;
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const float2 v = a.top_total[slot_of(i) * kRows + r % kRows];
+  for (int i = w * kWarp + lane; mine && i < n; i += 4 * kWarp) {
+    const float2 v = a.top_total[slot_of(i)];
     const float f = v.x == -INFINITY ? 0.0f : exp2_fast(v.x - m);
-    weight[i] = f;
+    my_weight[i] = f;
     l = fmaf(f, v.y, l);
   }
   for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(kFullMask, l, o);
-  if (lane == 0) red[1][warp] = l;
+  if (lane == 0) red[warp / 4][w][1] = l;
   __syncthreads();
   l = 0.0f;
-  for (int w = 0; w < kWarps; ++w) l += red[1][w];
-  float o[kPer] = {};
-#pragma unroll 4
-  for (int i = warp; i < n; i += kWarps) {
-    const float* from = a.sums + (slot_of(i) * kRows + r % kRows) * kDim + lane;
+  for (int i = 0; i < 4; ++i) l += red[warp / 4][i][1];
+  float4 o[kVectors] = {};
+  const bool holds = mine && lane * 4 < kDim;
+#pragma unroll 8
+  for (int i = w; i < n; i += 4) {
+    const float f = my_weight[i];
+    if (holds) {
+      const float4* from = reinterpret_cast<const float4*>(a.sums + slot_of(i) * kDim) + lane;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) o[k] = fmaf(weight[i], from[k * kWarp], o[k]);
+      for (int k = 0; k < kVectors; ++k) {
+        const float4 v = from[k * kWarp];
+        o[k] = make_float4(fmaf(f, v.x, o[k].x), fmaf(f, v.y, o[k].y), fmaf(f, v.z, o[k].z), fmaf(f, v.w, o[k].w));
+      }
+    }
   }
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) sums[warp][lane + k * kWarp] = o[k];
+  for (int k = 0; k < kVectors; ++k) {
+    if (holds) sums[warp / 4][w][lane + k * kWarp] = o[k];
+  }
   __syncthreads();
-  T* out = static_cast<T*>(a.out) + ((b * a.queries + r / a.group) * a.heads + kvh * a.group + r % a.group) * kDim;
-  for (int c = tid; c < kDim; c += kJoinThreads) {
-    float v = 0.0f;
-    for (int w = 0; w < kWarps; ++w) v += sums[w][c];
-    out[c] = from_float<T>(l == 0.0f ? 0.0f : v / l);
+  if (w != 0 || !holds) return;
+  const int64_t b = item / a.row_blocks / a.kv_heads;
+  const int kvh = static_cast<int>(item / a.row_blocks % a.kv_heads);
+  T* out = static_cast<T*>(a.out) + ((b * a.queries + row / a.group) * a.heads + kvh * a.group + row % a.group) * kDim;
+#pragma unroll
+  for (int k = 0; k < kVectors; ++k) {
+    float4 v = sums[warp / 4][0][lane + k * kWarp];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      const float4 x = sums[warp / 4][i][lane + k * kWarp];
+      v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+    }
+    store_row(out + 4 * (lane + k * kWarp), v, l);
   }
 }
 
@@ -851,8 +868,14 @@ int64_t most_parts(int64_t batch, int64_t queries, int64_t group, int64_t kv_hea
   const int64_t blocks = (queries * group + rows - 1) / rows;
   const int64_t tiles = (max_tokens + kKv4Tile - 1) / kKv4Tile;
   const int64_t items = batch * kv_heads * blocks;
-  if (tiles == 0 || items >= ctas * kMinTiles) return ctas;
-  return std::max<int64_t>(1, std::min(ctas, (items * tiles + kMinTiles - 1) / kMinTiles));
+  if (tiles == 0) return 1;
+  if (items >= ctas * kMinPart) return ctas;
+  return std::max<int64_t>(1, std::min(ctas, items * (tiles + kItemCost) / kMinPart));
+}
+
+// Bytes of scratch of a call: sums, maxima and totals of two partial items a part, and the split items.
+int64_t scratch_size(int64_t parts, int rows, int64_t dim, int64_t items) {
+  return parts == 1 ? 0 : 2 * parts * rows * (dim * 4 + 8) + items * 8;
 }
 
 template <typename T, int kDim, int kRows>
@@ -879,11 +902,11 @@ cudaError_t launch(const AttentionArgs& a, cudaStream_t stream) {
   config.numAttrs = 1;
   cudaError_t err = cudaLaunchKernelEx(&config, attention_kernel<T, kDim, kRows>, a);
   if (err != cudaSuccess || a.parts == 1) return err;  // one part: nothing is split
-  const int64_t joins = a.batch * a.kv_heads * a.queries * a.group;
+  const int64_t joins = a.batch * a.kv_heads * a.row_blocks * ((std::min(kRows, a.queries * a.group) + kJoinRows - 1) / kJoinRows);
   if (joins > 0x7fffffffLL) return cudaErrorInvalidValue;
   config.gridDim = dim3(static_cast<unsigned>(joins));
   config.blockDim = dim3(kJoinThreads);
-  config.dynamicSmemBytes = sizeof(float) * a.parts;
+  config.dynamicSmemBytes = kJoinRows * sizeof(float) * a.parts;
   return cudaLaunchKernelEx(&config, join_kernel<T, kDim, kRows>, a);
 }
 
@@ -906,9 +929,9 @@ extern "C" int64_t pck_kv4_attention_scratch(int64_t batch, int64_t queries, int
                                              int64_t max_tokens) {
   if (batch < 0 || queries < 1 || kv_heads < 1 || heads < kv_heads || dim < 1 || max_tokens < 0) return -1;
   const int64_t parts = pck::most_parts(batch, queries, heads / kv_heads, kv_heads, dim, max_tokens);
-  if (parts == 1) return 0;
-  const int64_t rows = pck::block_rows(queries * (heads / kv_heads), dim);
-  return 2 * parts * rows * (dim * 4 + 8);
+  const int rows = pck::block_rows(queries * (heads / kv_heads), dim);
+  const int64_t blocks = (queries * (heads / kv_heads) + rows - 1) / rows;
+  return pck::scratch_size(parts, rows, dim, batch * kv_heads * blocks);
 }
 
 extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_t queries, int64_t heads, int64_t dim,
@@ -933,7 +956,9 @@ extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_
   if (!q || !lengths || !out || (table_pages > 0 && !page_table) || (pages > 0 && !cache)) {
     return report_error(PCK_ERR_ARGUMENT, "attention: NULL q, cache, page_table, lengths or out");
   }
-  if (!aligned_to(cache, 16)) return report_error(PCK_ERR_ARGUMENT, "attention: the cache must be 16-byte aligned");
+  if (!aligned_to(cache, 16) || !aligned_to(out, 8)) {
+    return report_error(PCK_ERR_ARGUMENT, "attention: the cache must be 16-byte aligned, out 8-byte aligned");
+  }
   if (pages * kv_heads > (int64_t{1} << 31) / page_tiles) {
     return report_error(PCK_ERR_UNSUPPORTED, "attention: a cache holds at most 2^31 tiles");
   }
@@ -943,13 +968,15 @@ extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_
   const int rows = block_rows(queries * group, dim);
   AttentionArgs a{};
   a.parts = static_cast<int32_t>(most_parts(batch, queries, group, kv_heads, dim, max_tokens));
+  a.row_blocks = static_cast<int32_t>((queries * group + rows - 1) / rows);
   if (a.parts > 1) {
-    const int64_t slots = 2LL * a.parts * rows;
-    if (!scratch || !aligned_to(scratch, 16) || scratch_bytes < slots * (dim * 4 + 8)) {
+    if (!scratch || !aligned_to(scratch, 16) || scratch_bytes < scratch_size(a.parts, rows, dim, batch * kv_heads * a.row_blocks)) {
       return report_error(PCK_ERR_ARGUMENT, "attention: needs pck_kv4_attention_scratch() bytes of aligned scratch");
     }
+    const int64_t slots = 2LL * a.parts * rows;
     a.sums = static_cast<float*>(scratch);
     a.top_total = reinterpret_cast<float2*>(a.sums + slots * dim);
+    a.split = reinterpret_cast<int2*>(a.top_total + slots);
   }
   a.q = q;
   a.q_batch_stride = q_batch_stride;
@@ -970,7 +997,6 @@ extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_
   a.kv_heads = static_cast<int32_t>(kv_heads);
   a.page_tiles = static_cast<int32_t>(page_tiles);
   a.group = static_cast<int32_t>(group);
-  a.row_blocks = static_cast<int32_t>((queries * group + rows - 1) / rows);
   a.q_vector = aligned_to(q, 16) && q_batch_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t err = dtype == PCK_LOGITS_BF16 ? launch_any<__nv_bfloat16>(a, dim, rows, s)
