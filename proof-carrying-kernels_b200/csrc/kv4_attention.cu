@@ -24,10 +24,12 @@
 //   - The running maximum is raised only when a score passes it by 2^8 (weights then stay within
 //     2^8, which binary16 and the sums hold), so the accumulators are rarely rescaled and the
 //     common tile needs no exchange between lanes for it.
-//   - The tiles of all (request, head, row block) items form one line that is cut into equal parts,
-//     a CTA each, whatever the lengths: a part of an item leaves its sums in scratch memory and a
-//     second kernel (a programmatic dependent) joins them. A CTA's four warps take pairs of tiles in
-//     turn, each through its own ring of bulk copies.
+//   - Work is cut by the lengths, on the device. With few (request, head, row block) items a CTA takes
+//     an equal piece of one of them; with many, the tiles of all items form one line that is cut into
+//     equal parts, a CTA each, so one long request among short ones takes no longer than the rest. A
+//     part of an item leaves its sums in scratch memory and a second kernel (a programmatic dependent)
+//     joins them. A CTA's four warps take pairs of tiles in turn, each through its own ring of bulk
+//     copies.
 #include <algorithm>
 
 #include "kv4_layout.cuh"
@@ -42,6 +44,7 @@ constexpr int kAttnThreads = kAttnWarps * kWarp;
 // its warps), in tiles: items count as that much longer when the line is cut, or the parts that hold
 // many short items would end last.
 constexpr int kItemCost = 8;
+constexpr int kMinPiece = 8;  // tiles of a piece of an item, at least: two for each warp
 constexpr int kMinPart = 16;  // length of a part, at least
 constexpr float kRaise = 8.0f;      // log2 by which a score may pass the running maximum
 constexpr int kJoinRows = 4;     // rows of a joining CTA, four warps each
@@ -87,11 +90,27 @@ __device__ __forceinline__ Range request_tiles(const AttentionArgs& a, int64_t b
 // An item's length on the line.
 __device__ __forceinline__ int item_length(int tiles) { return tiles > 0 ? tiles + kItemCost : 0; }
 
-// Parts the line is cut into, and where part c begins.
-__device__ __forceinline__ int64_t part_count(const AttentionArgs& a, int64_t total) {
-  return max(int64_t{1}, min(static_cast<int64_t>(a.parts), total / kMinPart));
+// A 64-bit division takes several times a 32-bit one, and a CTA waits for these before its first copy.
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t by) {
+  if (x < int64_t{1} << 32 && by < int64_t{1} << 32) return static_cast<uint32_t>(x) / static_cast<uint32_t>(by);
+  return x / by;
 }
-__device__ __forceinline__ int64_t part_begin(int64_t total, int64_t parts, int64_t c) { return total * c / parts; }
+
+// The line is cut into `parts` parts of `length` or length + 1 places, the longer ones first.
+struct Cut {
+  int64_t parts, length, longer;
+  __device__ __forceinline__ int64_t begin(int64_t c) const { return c * length + min(c, longer); }
+  __device__ __forceinline__ int64_t holds(int64_t x) const {
+    const int64_t end = longer * (length + 1);
+    return x < end ? divide(x, length + 1) : longer + divide(x - end, length);
+  }
+};
+
+__device__ __forceinline__ Cut cut_line(const AttentionArgs& a, int64_t total) {
+  const int64_t parts = max(int64_t{1}, min(static_cast<int64_t>(a.parts), divide(total, kMinPart)));
+  const int64_t length = divide(total, parts);
+  return {parts, length, total - length * parts};
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -215,6 +234,84 @@ struct Shape {
   static_assert(kRing >= kAttnWarps * kRows * kDim * 4, "the warps' sums overlay the rings");
 };
 
+// A CTA's place on the line of items.
+struct Line {
+  int64_t at, end;  // what is left of its part
+  int64_t base;     // where request b begins
+  int64_t b;
+  Cut cut;
+};
+
+// The tiles of one item in a CTA's part.
+struct Segment {
+  int64_t b;
+  int64_t item;         // of all requests
+  int64_t last;         // the item's last place on the line
+  int32_t pieces;       // equal pieces of the item, a CTA each; 0: parts of the line
+  int32_t kvh, row0;    // key/value head, first row of the row block
+  int32_t length;       // the request's
+  int32_t count;        // tiles; 0: no segment is left
+  int32_t lo, hi;       // those of them that some row of the block sees
+  int32_t pos0, pos1;   // positions of the block's first and last query token
+  bool whole, first;    // all tiles of the item; the item's first tile
+};
+
+// Tiles [offset, offset + count) of an item of request b.
+template <int kRows>
+__device__ __forceinline__ void set_segment(const AttentionArgs& a, Segment& s, int64_t b, Range range, int64_t item,
+                                            int offset, int count) {
+  s.b = b;
+  s.item = b * a.kv_heads * a.row_blocks + item;
+  s.count = count;
+  s.whole = count == range.tiles;
+  s.first = offset == 0;
+  s.length = min(a.lengths[b], a.max_tokens);
+  s.kvh = static_cast<int>(item);
+  s.row0 = 0;
+  if (a.row_blocks > 1) {
+    s.kvh = static_cast<int>(divide(item, a.row_blocks));
+    s.row0 = (static_cast<int>(item) - s.kvh * a.row_blocks) * kRows;
+  }
+  s.pos0 = s.pos1 = s.length - 1;
+  if (a.queries > 1) {
+    s.pos0 = s.length - a.queries + s.row0 / a.group;
+    s.pos1 = s.length - a.queries + (min(s.row0 + kRows, a.queries * a.group) - 1) / a.group;
+  }
+  s.lo = range.first + offset;
+  s.hi = s.lo + count;
+  if (a.window > 0) s.lo = max(s.lo, max(0, s.pos0 + 1 - a.window) / kKv4Tile);
+  s.hi = s.pos1 < 0 ? s.lo : min(s.hi, s.pos1 / kKv4Tile + 1);
+}
+
+// The next segment of a part of the line (count 0: none is left).
+template <int kRows>
+__device__ __forceinline__ void next_segment(const AttentionArgs& a, Line& line, Segment& s) {
+  const int64_t items = static_cast<int64_t>(a.kv_heads) * a.row_blocks;
+  int64_t at = line.at, b = line.b, base = line.base;
+  s.count = 0;
+  while (at < line.end && s.count == 0) {
+    const Range range = request_tiles(a, b);
+    const int size = item_length(range.tiles);
+    if (at >= base + size * items) {
+      base += size * items;
+      ++b;
+      continue;
+    }
+    const int64_t item = divide(at - base, size);
+    const int start = static_cast<int>(at - base - item * size);
+    const int stop = static_cast<int>(min(static_cast<int64_t>(size), start + (line.end - at)));
+    at += stop - start;
+    // Its tiles come after its cost.
+    const int offset = max(0, start - kItemCost), count = max(0, stop - kItemCost) - offset;
+    if (count == 0) continue;
+    set_segment<kRows>(a, s, b, range, item, offset, count);
+    s.last = base + (item + 1) * size - 1;
+  }
+  line.at = at;
+  line.b = b;
+  line.base = base;
+}
+
 // Four channels of a row: sums over the sum of weights (zeros for a row that saw nothing).
 template <typename T>
 __device__ __forceinline__ void store_row(T* to, float4 o, float l) {
@@ -236,6 +333,8 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kAttnWarps][S::kSlots];
   __shared__ float2 state[kAttnWarps][kRows];
+  __shared__ Line line;
+  __shared__ Segment segment;
 
   const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
   const int row8 = lane / 4, quarter = lane % 4;
@@ -247,43 +346,87 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
   allow_dependents();
   wait_for_producers();
 
-  // Requests that hold nothing give zeros.
   T* const out = static_cast<T*>(a.out);
   const int64_t items = static_cast<int64_t>(a.kv_heads) * a.row_blocks;  // of a request
-  const int64_t row_size = static_cast<int64_t>(a.queries) * a.heads * kDim;
-  for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
-    if (request_tiles(a, b).tiles == 0) {
-      for (int64_t i = tid; i < row_size; i += kAttnThreads) out[b * row_size + i] = from_float<T>(0.0f);
-      for (int64_t i = tid; a.parts > 1 && i < items; i += kAttnThreads) a.split[b * items + i] = make_int2(0, 0);
+  if (warp == 0) {
+    // What this CTA takes, of the items in the order (request, head, row block). Few items: one of the
+    // equal pieces of one item. Many: its part of the line.
+    const int mine = lane < a.batch ? request_tiles(a, lane).tiles : 0;
+    int64_t total = item_length(mine), tiles = mine, filled = mine > 0;
+    for (int64_t i = lane + kWarp; i < a.batch; i += kWarp) {
+      const int n = request_tiles(a, i).tiles;
+      total += item_length(n);
+      tiles += n;
+      filled += n > 0;
     }
-  }
-
-  // This CTA's part of the line of items, in the order (request, head, row block); every warp for itself.
-  int64_t total = 0;
-  for (int64_t i = lane; i < a.batch; i += kWarp) total += item_length(request_tiles(a, i).tiles);
-  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(kFullMask, total, o);
-  total *= items;
-  const int64_t parts = part_count(a, total);
-  if (blockIdx.x >= parts) return;
-  const int64_t begin = part_begin(total, parts, blockIdx.x), end = part_begin(total, parts, blockIdx.x + 1);
-  if (begin >= end) return;
-  // The request in which it begins, and where that begins.
-  int64_t b = 0, base = 0;
-  for (; b < a.batch; b += kWarp) {
-    const int64_t n = b + lane < a.batch ? item_length(request_tiles(a, b + lane).tiles) * items : 0;
-    int64_t before = n;
-    for (int o = 1; o < kWarp; o <<= 1) {
-      const int64_t v = __shfl_up_sync(kFullMask, before, o);
-      if (lane >= o) before += v;
+    for (int o = 16; o && a.batch > 1; o >>= 1) {
+      total += __shfl_xor_sync(kFullMask, total, o);
+      tiles += __shfl_xor_sync(kFullMask, tiles, o);
+      filled += __shfl_xor_sync(kFullMask, filled, o);
     }
-    const unsigned here = __ballot_sync(kFullMask, begin < base + before);
-    if (here) {
-      const int l = __ffs(here) - 1;
-      b += l;
-      base += __shfl_sync(kFullMask, before - n, l);
-      break;
+    tiles = __shfl_sync(kFullMask, tiles, 0);
+    filled = __shfl_sync(kFullMask, filled, 0) * items;
+    const bool pieces = 2 * filled <= a.parts;
+    // Tiles of a piece, at most: with this many the pieces are no more than the CTAs.
+    const int piece = pieces ? static_cast<int>(max(int64_t{kMinPiece}, divide(tiles * items, a.parts - filled) + 1)) : 1;
+    auto places = [&](int n) -> int64_t { return pieces ? (n + piece - 1) / piece : item_length(n); };
+    int64_t begin = blockIdx.x, end = begin + 1;
+    if (!pieces) {
+      const Cut cut = cut_line(a, __shfl_sync(kFullMask, total, 0) * items);
+      begin = blockIdx.x < cut.parts ? cut.begin(blockIdx.x) : 0;
+      end = blockIdx.x < cut.parts ? cut.begin(blockIdx.x + 1) : 0;
+      if (lane == 0) line.cut = cut;
     }
-    base += __shfl_sync(kFullMask, before, kWarp - 1);
+    // The request in which it begins, and where that begins.
+    int64_t b = 0, base = 0;
+    bool any = false;
+    for (; begin < end && b < a.batch; b += kWarp) {
+      int64_t n = places(b == 0 ? mine : b + lane < a.batch ? request_tiles(a, b + lane).tiles : 0) * items;
+      int64_t before = n;
+      for (int o = 1; o < kWarp && o < a.batch; o <<= 1) {
+        const int64_t v = __shfl_up_sync(kFullMask, before, o);
+        if (lane >= o) before += v;
+      }
+      const unsigned here = __ballot_sync(kFullMask, begin < base + before);
+      any = here != 0;
+      if (any) {
+        const int l = __ffs(here) - 1;
+        b += l;
+        base += __shfl_sync(kFullMask, before - n, l);
+        break;
+      }
+      base += __shfl_sync(kFullMask, before, kWarp - 1);
+    }
+    if (lane == 0) {
+      line.at = begin;
+      line.end = any ? end : begin;
+      line.base = base;
+      line.b = b;
+      if (pieces) {
+        line.at = line.end;
+        segment.count = 0;
+        if (any) {
+          const Range range = request_tiles(a, b);
+          const int n = static_cast<int>(places(range.tiles));
+          const int item = static_cast<int>(begin - base) / n, i = static_cast<int>(begin - base) - item * n;
+          const int size = range.tiles / n, longer = range.tiles - size * n;
+          set_segment<kRows>(a, segment, b, range, item, i * size + min(i, longer), size + (i < longer));
+          segment.pieces = n;
+        }
+      } else {
+        segment.pieces = 0;
+        next_segment<kRows>(a, line, segment);
+      }
+    }
+  } else {
+    // Requests that hold nothing give zeros.
+    const int64_t row_size = static_cast<int64_t>(a.queries) * a.heads * kDim;
+    for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
+      if (request_tiles(a, b).tiles == 0) {
+        for (int64_t i = tid - kWarp; i < row_size; i += kAttnThreads - kWarp) out[b * row_size + i] = from_float<T>(0.0f);
+        for (int64_t i = tid - kWarp; a.parts > 1 && i < items; i += kAttnThreads - kWarp) a.split[b * items + i] = make_int2(0, 0);
+      }
+    }
   }
 
   const uint64_t policy = policy_evict_first();
@@ -291,43 +434,13 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
   uint8_t* const ring = smem + warp * S::kSlots * S::kStageBytes;
   uint32_t phase = 0;  // parity bit of each slot
   bool dead = false;   // a wait gave up
-  for (int64_t at = begin; at < end;) {
-    const Range range = request_tiles(a, b);
-    const int size = item_length(range.tiles);
-    if (at >= base + size * items) {
-      base += size * items;
-      ++b;
-      continue;
-    }
-    const int64_t item = (at - base) / size;
-    const int start = static_cast<int>((at - base) % size);
-    const int stop = static_cast<int>(min(static_cast<int64_t>(size), start + (end - at)));
-    at += stop - start;
-    // Its tiles come after its cost.
-    const int offset = max(0, start - kItemCost), count = max(0, stop - kItemCost) - offset;
-    if (count == 0) continue;
-    const int kvh = static_cast<int>(item / a.row_blocks), block = static_cast<int>(item % a.row_blocks);
-    const bool whole = count == range.tiles;
-    if (offset == 0 && a.parts > 1 && tid == 0) {
-      // Parts from this one to the one with the item's last place.
-      int64_t last = blockIdx.x;
-      if (!whole) {
-        const int64_t x = base + (item + 1) * size - 1;
-        last = x * parts / total;
-        while (last + 1 < parts && part_begin(total, parts, last + 1) <= x) ++last;
-        while (part_begin(total, parts, last) > x) --last;
-      }
-      a.split[b * items + item] = make_int2(blockIdx.x, static_cast<int>(last - blockIdx.x + 1));
-    }
-    const int length = min(a.lengths[b], a.max_tokens);
+  while (true) {
+    __syncthreads();
+    if (segment.count == 0) return;
+    const int64_t b = segment.b;
+    const int kvh = segment.kvh, row0 = segment.row0, length = segment.length;
+    const int lo = segment.lo, hi = segment.hi;
     const int rows = a.queries * a.group;
-    const int row0 = block * kRows;
-    // Positions of the block's first and last query token, and the tiles that they see.
-    const int pos0 = length - a.queries + row0 / a.group;
-    const int pos1 = length - a.queries + (min(row0 + kRows, rows) - 1) / a.group;
-    int lo = range.first + offset, hi = lo + count;
-    if (a.window > 0) lo = max(lo, max(0, pos0 + 1 - a.window) / kKv4Tile);
-    hi = pos1 < 0 ? lo : min(hi, pos1 / kKv4Tile + 1);
     // The warp's stages: kStage tiles each, every kAttnWarps-th.
     const int stages = max(0, hi - lo + kStage - 1) / kStage;
     const int warp_stages = (max(0, stages - warp) + kAttnWarps - 1) / kAttnWarps;
@@ -380,7 +493,6 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     float qsum[kN][kG][2];
     float excess[kN][kG][2];  // what the 1024 beside each code adds to a product, negated
     float factor[kN][2];  // of a score: the softmax's scale (log2) over the row's power of two
-    int pos[kN][2];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       const int r = row0 + 8 * n + row8;
@@ -407,30 +519,26 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
       // The row as binary16, its largest element between 16 and 32 by a power of two (rows of zeros,
       // infinities or NaN as they are): what is lost of small elements is below 2^-25 of the largest.
-      uint32_t largest = 0;
+      uint32_t packed = 0;
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 v = unpack_pair<T>(x[g][i]);
-          largest = max(largest, max(__float_as_uint(fabsf(v.x)), __float_as_uint(fabsf(v.y))));
-        }
+        for (int i = 0; i < 8; ++i) packed = __vmaxu2(packed, x[g][i] & 0x7fff7fffu);
       }
-      largest = max(largest, __shfl_xor_sync(kFullMask, largest, 1));
-      largest = max(largest, __shfl_xor_sync(kFullMask, largest, 2));
+      packed = __vmaxu2(packed, __shfl_xor_sync(kFullMask, packed, 1));
+      packed = __vmaxu2(packed, __shfl_xor_sync(kFullMask, packed, 2));
+      const uint32_t largest = __float_as_uint(unpack_pair<T>(max(packed & 0xffffu, packed >> 16)).x);
       uint32_t field = largest >> 23;
       field = field == 0 || field == 255 ? 131 : min(max(field, 8u), 250u);
       const float scale = __uint_as_float((258u - field) << 23);
       const float back = a.scale_log2 * __uint_as_float((field - 4u) << 23);
-      const int my_pos = r < rows ? length - a.queries + t : -1;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        pos[n][e] = __shfl_sync(kFullMask, my_pos, (2 * quarter + e) * 4);
         factor[n][e] = __shfl_sync(kFullMask, back, (2 * quarter + e) * 4);
       }
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
-        float sum = 0.0f, held = 0.0f;
+        float even = 0.0f, odd = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           // Channels that meet 16 n (the odd pairs: 1, 3, 5, 7 of each 8) are divided by 16.
@@ -438,19 +546,18 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
           const __half2 h = __floats2half2_rn(v.x * scale, v.y * (scale * 0.0625f));
           x[g][i] = half2_bits(h);
           v = __half22float2(h);
-          sum += v.x;
-          sum = fmaf(16.0f, v.y, sum);
-          held += v.x;
-          held += v.y;
+          even += v.x;
+          odd += v.y;
         }
-        sum += __shfl_xor_sync(kFullMask, sum, 1);
-        sum += __shfl_xor_sync(kFullMask, sum, 2);
-        held += __shfl_xor_sync(kFullMask, held, 1);
-        held += __shfl_xor_sync(kFullMask, held, 2);
+        even += __shfl_xor_sync(kFullMask, even, 1);
+        even += __shfl_xor_sync(kFullMask, even, 2);
+        odd += __shfl_xor_sync(kFullMask, odd, 1);
+        odd += __shfl_xor_sync(kFullMask, odd, 2);
+        const float sum = fmaf(16.0f, odd, even), held = -1024.0f * (even + odd);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           qsum[n][g][e] = __shfl_sync(kFullMask, sum, (2 * quarter + e) * 4);
-          excess[n][g][e] = -1024.0f * __shfl_sync(kFullMask, held, (2 * quarter + e) * 4);
+          excess[n][g][e] = __shfl_sync(kFullMask, held, (2 * quarter + e) * 4);
         }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
@@ -464,19 +571,27 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
     }
 
+    if (segment.first && a.parts > 1 && tid == kAttnThreads - 1) {
+      // Parts from this one to the one with the item's last place.
+      const int n = segment.pieces ? segment.pieces
+                    : segment.whole ? 1 : static_cast<int>(line.cut.holds(segment.last) - blockIdx.x + 1);
+      a.split[segment.item] = make_int2(blockIdx.x, n);
+    }
+
     // Products with the values: element e of [n][g][m] is channel 8 (lane / 4) + 2 m + e / 2 of group
     // g for row 2 quarter + e % 2 of block n.
     float acc[kN][kG][4][4];
-    float top[kN][2], total_w[kN][2], zeros[kN][kG][2];  // top: the running maximum, log2
-    float limit[kN][2], base_w[kN][2];  // the score at top + kRaise, and top or 0 before there is one
+    float total_w[kN][2], zeros[kN][kG][2];
+    // The running maximum (log2; 0 while there is none) and the score that raises it (-inf while there
+    // is none).
+    float top[kN][2], limit[kN][2];
     uint32_t unit[kG];  // exponent field of the power of two that the values' weights are divided by
-    float inv[kG];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        top[n][e] = limit[n][e] = -INFINITY;
-        total_w[n][e] = base_w[n][e] = 0.0f;
+        limit[n][e] = -INFINITY;
+        total_w[n][e] = top[n][e] = 0.0f;
       }
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
@@ -486,10 +601,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
     }
 #pragma unroll
-    for (int g = 0; g < kG; ++g) {
-      unit[g] = 127;
-      inv[g] = 1.0f;
-    }
+    for (int g = 0; g < kG; ++g) unit[g] = 127;
 
     // One stage. This lane's tokens are row8 + 8 j. kMasked: some row does not see some of them, or
     // a tile is missing.
@@ -558,7 +670,8 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
           for (int j = 0; j < kJ; ++j) {
             if constexpr (kMasked) {
-              const int token = token0 + row8 + 8 * j, at = pos[n][e];
+              const int token = token0 + row8 + 8 * j, r = row0 + 8 * n + 2 * quarter + e;
+              const int at = r < rows ? length - a.queries + r / a.group : -1;
               off[n][j][e] = token > at || (a.window > 0 && token <= at - a.window) || (gone >> j / 2 & 1u);
               if (off[n][j][e]) s[n][j][e] = -INFINITY;
             }
@@ -575,14 +688,14 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
             float m = s[n][0][e];
 #pragma unroll
             for (int j = 1; j < kJ; ++j) m = fmaxf(m, s[n][j][e]);
-            m = fmaxf(top[n][e], m * factor[n][e]);
+            const float old = limit[n][e] == -INFINITY ? -INFINITY : top[n][e];
+            m = fmaxf(old, m * factor[n][e]);
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 4));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16));
-            const float keep = top[n][e] == m ? 1.0f : exp2_fast(top[n][e] - m);
-            top[n][e] = m;
+            const float keep = old == m ? 1.0f : exp2_fast(old - m);
+            top[n][e] = m == -INFINITY ? 0.0f : m;
             limit[n][e] = (m + kRaise) / factor[n][e];
-            base_w[n][e] = m == -INFINITY ? 0.0f : m;
             total_w[n][e] *= keep;
 #pragma unroll
             for (int g = 0; g < kG; ++g) {
@@ -602,7 +715,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int j = 0; j < kJ; ++j) {
-            s[n][j][e] = exp2_fast(fmaf(s[n][j][e], factor[n][e], -base_w[n][e]));
+            s[n][j][e] = exp2_fast(fmaf(s[n][j][e], factor[n][e], -top[n][e]));
             total_w[n][e] += s[n][j][e];
           }
         }
@@ -630,7 +743,6 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
           const uint32_t next = min(field, 253u);
           const float ratio = __uint_as_float((254u - next) << 23) * __uint_as_float(unit[g] << 23);
           unit[g] = next;
-          inv[g] = __uint_as_float((254u - next) << 23);
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
 #pragma unroll
@@ -659,7 +771,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
             for (int j = 0; j < 2; ++j) {
               const uint32_t pair = pairs[2 * u + j][g];
               const float scale = bf16_lo(pair), zero = fmaf(8.0f, scale, bf16_hi(pair));
-              const float unit_scale = scale * inv[g];
+              const float unit_scale = scale * __uint_as_float((254u - unit[g]) << 23);
 #pragma unroll
               for (int n = 0; n < kN; ++n) {
                 float x[2];
@@ -702,7 +814,8 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       if (gone != 3 && !dead) {
         const uint8_t* stage = ring + slot * S::kStageBytes;
         const int token0 = (lo + kStage * (warp + k * kAttnWarps)) * kKv4Tile;
-        if (gone == S::kNone && token0 + kStage * kKv4Tile - 1 <= pos0 && (a.window <= 0 || token0 > pos1 - a.window)) {
+        if (gone == S::kNone && token0 + kStage * kKv4Tile - 1 <= segment.pos0 &&
+            (a.window <= 0 || token0 > segment.pos1 - a.window)) {
           stage_step(stage, token0, 0, std::false_type{});
         } else {
           stage_step(stage, token0, gone, std::true_type{});
@@ -724,7 +837,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
         const int r = 8 * n + 2 * quarter + e;
         float l = total_w[n][e];
         for (int o = 4; o < kWarp; o <<= 1) l += __shfl_xor_sync(kFullMask, l, o);
-        if (row8 == 0) state[warp][r] = make_float2(top[n][e], l);
+        if (row8 == 0) state[warp][r] = make_float2(limit[n][e] == -INFINITY ? -INFINITY : top[n][e], l);
 #pragma unroll
         for (int g = 0; g < kG; ++g) {
           float z = zeros[n][g][e];
@@ -740,7 +853,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
     }
     __syncthreads();
-    const int64_t slot_id = 2 * static_cast<int64_t>(blockIdx.x) + (offset == 0 ? 1 : 0);
+    const int64_t slot_id = 2 * static_cast<int64_t>(blockIdx.x) + (segment.first ? 1 : 0);
     const int kept = min(kRows, rows - row0);
     for (int i = 4 * tid; i < kept * kDim; i += 4 * kAttnThreads) {
       const int r = i / kDim, c = i % kDim;
@@ -756,7 +869,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
         o = make_float4(fmaf(f, v.x, o.x), fmaf(f, v.y, o.y), fmaf(f, v.z, o.z), fmaf(f, v.w, o.w));
         l = fmaf(f, state[w][r].y, l);
       }
-      if (whole) {
+      if (segment.whole) {
         const int t = (row0 + r) / a.group, head = kvh * a.group + (row0 + r) % a.group;
         store_row(out + ((b * a.queries + t) * a.heads + head) * kDim + c, o, l);
       } else {
@@ -765,7 +878,9 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next bulk copies land here
+    if (segment.pieces) return;
     __syncthreads();
+    if (tid == 0) next_segment<kRows>(a, line, segment);
   }
 }
 
@@ -773,9 +888,8 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 template <typename T, int kDim, int kRows>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttentionArgs a) {
   constexpr int kVectors = kDim / 128 > 1 ? 2 : 1;  // float4 of a lane (dim 64: half the lanes)
-  extern __shared__ float weight[];
   __shared__ float4 sums[kJoinRows][4][kDim / 4];
-  __shared__ float red[kJoinRows][4][2];
+  __shared__ float2 red[kJoinRows][4];
   const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp, w = warp % 4;
   const int chunks = (min(kRows, a.queries * a.group) + kJoinRows - 1) / kJoinRows;
   const int64_t item = blockIdx.x / chunks;
@@ -788,55 +902,70 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   if (n <= 1) return;  // nothing to join
   // The part that holds the item's beginning has it in its second slot, the others in their first.
   auto slot_of = [&](int i) { return (2 * (static_cast<int64_t>(split.x) + i) + (i == 0 ? 1 : 0)) * kRows + in_block; };
-  float m = -INFINITY;
-  for (int i = w * kWarp + lane; mine && i < n; i += 4 * kWarp) m = fmaxf(m, a.top_total[slot_of(i)].x);
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
-  if (lane == 0) red[warp / 4][w][0] = m;
-  __syncthreads();
-  for (int i = 0; i < 4; ++i) m = fmaxf(m, red[warp / 4][i][0]);
-  float* const my_weight = weight + warp / 4 * n;
-  float l = 0.0f;
-  for (int i = w * kWarp + lane; mine && i < n; i += 4 * kWarp) {
-    const float2 v = a.top_total[slot_of(i)];
-    const float f = v.x == -INFINITY ? 0.0f : exp2_fast(v.x - m);
-    my_weight[i] = f;
-    l = fmaf(f, v.y, l);
-  }
-  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(kFullMask, l, o);
-  if (lane == 0) red[warp / 4][w][1] = l;
-  __syncthreads();
-  l = 0.0f;
-  for (int i = 0; i < 4; ++i) l += red[warp / 4][i][1];
-  float4 o[kVectors] = {};
   const bool holds = mine && lane * 4 < kDim;
-#pragma unroll 8
-  for (int i = w; i < n; i += 4) {
-    const float f = my_weight[i];
-    if (holds) {
-      const float4* from = reinterpret_cast<const float4*>(a.sums + slot_of(i) * kDim) + lane;
+  // A warp's share of the parts, four loads at a time, by its own running maximum.
+  float m = -INFINITY, l = 0.0f;
+  float4 o[kVectors] = {};
+  for (int i0 = w; mine && i0 < n; i0 += 16) {
+    float2 tops[4];
+    float4 v[4][kVectors];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + 4 * u;
+      tops[u] = i < n ? a.top_total[slot_of(i)] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
       for (int k = 0; k < kVectors; ++k) {
-        const float4 v = from[k * kWarp];
-        o[k] = make_float4(fmaf(f, v.x, o[k].x), fmaf(f, v.y, o[k].y), fmaf(f, v.z, o[k].z), fmaf(f, v.w, o[k].w));
+        v[u][k] = i < n && holds ? reinterpret_cast<const float4*>(a.sums + slot_of(i) * kDim)[lane + k * kWarp]
+                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+    }
+    float next = m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) next = fmaxf(next, tops[u].x);
+    const float keep = m == -INFINITY ? 0.0f : exp2_fast(m - next);
+    m = next;
+    l *= keep;
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) o[k] = make_float4(o[k].x * keep, o[k].y * keep, o[k].z * keep, o[k].w * keep);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float f = tops[u].x == -INFINITY ? 0.0f : exp2_fast(tops[u].x - m);
+      l = fmaf(f, tops[u].y, l);
+#pragma unroll
+      for (int k = 0; k < kVectors; ++k) {
+        o[k] = make_float4(fmaf(f, v[u][k].x, o[k].x), fmaf(f, v[u][k].y, o[k].y), fmaf(f, v[u][k].z, o[k].z),
+                           fmaf(f, v[u][k].w, o[k].w));
       }
     }
   }
+  if (lane == 0) red[warp / 4][w] = make_float2(m, l);
 #pragma unroll
   for (int k = 0; k < kVectors; ++k) {
     if (holds) sums[warp / 4][w][lane + k * kWarp] = o[k];
   }
   __syncthreads();
   if (w != 0 || !holds) return;
+  m = -INFINITY;
+  l = 0.0f;
+  float f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = fmaxf(m, red[warp / 4][i].x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = red[warp / 4][i];
+    f[i] = v.x == -INFINITY ? 0.0f : exp2_fast(v.x - m);
+    l = fmaf(f[i], v.y, l);
+  }
   const int64_t b = item / a.row_blocks / a.kv_heads;
   const int kvh = static_cast<int>(item / a.row_blocks % a.kv_heads);
   T* out = static_cast<T*>(a.out) + ((b * a.queries + row / a.group) * a.heads + kvh * a.group + row % a.group) * kDim;
 #pragma unroll
   for (int k = 0; k < kVectors; ++k) {
-    float4 v = sums[warp / 4][0][lane + k * kWarp];
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const float4 x = sums[warp / 4][i][lane + k * kWarp];
-      v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+      v = make_float4(fmaf(f[i], x.x, v.x), fmaf(f[i], x.y, v.y), fmaf(f[i], x.z, v.z), fmaf(f[i], x.w, v.w));
     }
     store_row(out + 4 * (lane + k * kWarp), v, l);
   }
@@ -869,8 +998,7 @@ int64_t most_parts(int64_t batch, int64_t queries, int64_t group, int64_t kv_hea
   const int64_t tiles = (max_tokens + kKv4Tile - 1) / kKv4Tile;
   const int64_t items = batch * kv_heads * blocks;
   if (tiles == 0) return 1;
-  if (items >= ctas * kMinPart) return ctas;
-  return std::max<int64_t>(1, std::min(ctas, items * (tiles + kItemCost) / kMinPart));
+  return std::min(ctas, items >= ctas ? ctas : std::max<int64_t>(items * ((tiles + kMinPiece - 1) / kMinPiece), 1));
 }
 
 // Bytes of scratch of a call: sums, maxima and totals of two partial items a part, and the split items.
@@ -906,7 +1034,7 @@ cudaError_t launch(const AttentionArgs& a, cudaStream_t stream) {
   if (joins > 0x7fffffffLL) return cudaErrorInvalidValue;
   config.gridDim = dim3(static_cast<unsigned>(joins));
   config.blockDim = dim3(kJoinThreads);
-  config.dynamicSmemBytes = kJoinRows * sizeof(float) * a.parts;
+  config.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&config, join_kernel<T, kDim, kRows>, a);
 }
 
