@@ -212,7 +212,7 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t*
 // CTAs on an SM, by the registers that the rows' products take.
 constexpr int attention_ctas(int rows, int dim) {
   if (dim == 64) return rows <= 16 ? 4 : 2;
-  if (dim == 128) return rows <= 8 ? 4 : rows <= 16 ? 3 : 2;
+  if (dim == 128) return rows <= 16 ? 3 : 2;
   return 2;
 }
 
@@ -226,10 +226,10 @@ struct Shape {
   static constexpr int kCtas = attention_ctas(kRows, kDim);
   // Tiles that a warp takes at once: two share the checks of a step, where the registers allow it.
   static constexpr int kStage = kRows == 8 || kRows * kDim <= 16 * 64 ? 2 : 1;
-  static constexpr uint32_t kNone = kStage == 2 ? 0 : 2;  // of a slot's two bits: no tile is missing
   static constexpr int kStageBytes = kStage * kTileBytes;
   // Copies in flight for the HBM's latency: the SM's shared memory, less what the CTAs take beside it.
-  static constexpr int kSlots = (216 << 10) / (kCtas * kAttnWarps * kStageBytes);
+  static constexpr int kMost = (216 << 10) / (kCtas * kAttnWarps * kStageBytes);
+  static constexpr int kSlots = kMost < 16 ? kMost : 16;
   static constexpr int kRing = kAttnWarps * kSlots * kStageBytes;
   static_assert(kRing >= kAttnWarps * kRows * kDim * 4, "the warps' sums overlay the rings");
 };
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
   const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
   const int row8 = lane / 4, quarter = lane % 4;
   if (lane == 0) {
-    for (int s = 0; s < S::kSlots; ++s) mbar_init(&full[warp][s], 1);
+    for (int s = 0; s < S::kSlots; ++s) mbar_init(&full[warp][s], kStage);
     fence_barrier_init();
   }
   __syncwarp();
@@ -460,31 +460,33 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     };
     constexpr int kBatch = kWarp / kStage;
     int32_t places = look_up(0), places_next = look_up(kBatch);
-    uint32_t missing = 0;  // two bits a slot: tiles that it does not hold
-    auto issue = [&](int k, int slot) {
-      if (k % kBatch == 0 && k > 0) {
-        places = places_next;
-        places_next = look_up(k + kBatch);
-      }
-      const int32_t p0 = __shfl_sync(kFullMask, places, k % kBatch * kStage);
-      const int32_t p1 = kStage == 1 ? -1 : __shfl_sync(kFullMask, places, k % kBatch * kStage + 1);
-      const uint32_t gone = (p0 < 0 ? 1u : 0u) + (p1 < 0 ? 2u : 0u);
-      missing = (missing & ~(3u << 2 * slot)) | gone << 2 * slot;
-      if (lane == 0) {
-        uint64_t* bar = &full[warp][slot];
-        uint8_t* to = ring + slot * S::kStageBytes;
-        if (gone == 3) {
-          mbar_arrive(bar);
-        } else {
-          mbar_arrive_expect_tx(bar, gone == 0 ? 2 * S::kTileBytes : S::kTileBytes);
-          if (p0 >= 0) bulk_load(to, a.cache + static_cast<int64_t>(p0) * S::kTileBytes, S::kTileBytes, bar, policy);
-          if (p1 >= 0) {
-            bulk_load(to + S::kTileBytes, a.cache + static_cast<int64_t>(p1) * S::kTileBytes, S::kTileBytes, bar, policy);
-          }
-        }
+    uint32_t absent = __ballot_sync(kFullMask, places < 0);
+    uint32_t missing = 0;  // kStage bits a slot: tiles that it does not hold
+    constexpr uint32_t kNone = (1u << kStage) - 1;
+    // A tile's copy is issued by the lane that looked it up.
+    auto copy = [&](int slot) {
+      uint64_t* bar = &full[warp][slot];
+      if (places < 0) {
+        mbar_arrive(bar);
+      } else {
+        mbar_arrive_expect_tx(bar, S::kTileBytes);
+        bulk_load(ring + slot * S::kStageBytes + lane % kStage * S::kTileBytes,
+                  a.cache + static_cast<int64_t>(places) * S::kTileBytes, S::kTileBytes, bar, policy);
       }
     };
-    for (int s = 0; s < S::kSlots && s < warp_stages; ++s) issue(s, s);
+    auto issue = [&](int k, int slot) {
+      const int at = k % kBatch;
+      if (at == 0) {
+        places = places_next;
+        absent = __ballot_sync(kFullMask, places < 0);
+        places_next = look_up(k + kBatch);
+      }
+      missing = (missing & ~(kNone << slot * kStage)) | (absent >> at * kStage & kNone) << slot * kStage;
+      if (lane / kStage == at) copy(slot);
+    };
+    static_assert(S::kSlots <= kBatch, "the first copies come from one batch of places");
+    missing = absent;  // slot s holds the tiles of lanes kStage s and on
+    if (lane / kStage < min(S::kSlots, warp_stages)) copy(lane / kStage);
 
     // q as the right operand: this lane's row lane / 4 of each block, its channels in the order of
     // the codes: for each 8 channels the pairs (0, 4), (1, 5), (2, 6), (3, 7).
@@ -810,11 +812,11 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     for (int k = 0; k < warp_stages; ++k) {
       if (!dead) dead = !__all_sync(kFullMask, mbar_wait(&full[warp][slot], phase >> slot & 1u));
       phase ^= 1u << slot;
-      const uint32_t gone = missing >> 2 * slot & 3u;
-      if (gone != 3 && !dead) {
+      const uint32_t gone = missing >> slot * kStage & kNone;
+      if (gone != kNone && !dead) {
         const uint8_t* stage = ring + slot * S::kStageBytes;
         const int token0 = (lo + kStage * (warp + k * kAttnWarps)) * kKv4Tile;
-        if (gone == S::kNone && token0 + kStage * kKv4Tile - 1 <= segment.pos0 &&
+        if (gone == 0 && token0 + kStage * kKv4Tile - 1 <= segment.pos0 &&
             (a.window <= 0 || token0 > segment.pos1 - a.window)) {
           stage_step(stage, token0, 0, std::false_type{});
         } else {

@@ -1,14 +1,33 @@
 // pck_lora_add: out = y + s_a B_a (A_a x) for rows that each name their adapter a.
 //
-// One CTA per row: a warp per rank takes the product of A's row with x, then a thread per output
-// takes B's row with the rank-long intermediate, which stays in binary32.
+// A tile of 16 or 64 rows is walked through the distinct adapters that its rows name, an item each,
+// so rows may come in any order: a decode batch where every row has its own adapter, or prompts whose
+// rows share one. A cluster of CTAs takes an item:
+//   1. h = A x for the item's rows: the CTAs and their warps split the columns n, and each product
+//      (mma.sync, binary32 sums) takes x and A straight from memory in 16-byte loads, since nothing in
+//      a warp reads them twice;
+//   2. the warps' and then the CTAs' partial sums are added in a fixed order, through shared and
+//      distributed shared memory: h stays in binary32;
+//   3. out = y + s B h: the CTAs and warps split the outputs m. h enters the products as three (bfloat16)
+//      or two (binary16, scaled by a power of two of its row) terms whose sum is h to binary32's
+//      precision, so nothing is lost against a binary32 product.
+// Bound by the adapters' bytes for decode batches (each read once per tile that names it) and by x, y and
+// out for prompts; with few rows by the latency of the two dependent passes, which is why a single row
+// is spread over a cluster of eight CTAs.
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
 #include "serving_common.cuh"
 
 namespace pck {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kLoraMaxRank = 256;
-constexpr int kLoraThreads = 256;
+constexpr int kLoraWarps = 8;
+constexpr int kLoraThreads = kLoraWarps * kWarp;
 
 struct LoraArgs {
   const void* x;
@@ -22,40 +41,359 @@ struct LoraArgs {
   const int32_t* ranks;
   float* out;
   int64_t out_stride;
-  int64_t n, m;
+  int64_t n, m, tokens;
   int32_t count, rank;
+  int32_t n_vector;   // rows of x and A are 16-byte aligned
+  int32_t rank_vector;  // rows of B are 8-byte aligned
+  int32_t y_vector;   // rows of y and out are 16-byte aligned
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kLoraThreads) lora_kernel(const LoraArgs a) {
-  __shared__ float h[kLoraMaxRank];
-  const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
-  int adapter = a.adapters[row];
-  if (adapter >= a.count) {
-    if (threadIdx.x == 0) report(kDevIndex);
-    adapter = -1;
+__device__ __forceinline__ void lora_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
-  int rank = 0;
-  if (adapter >= 0) {
-    rank = a.ranks ? min(max(a.ranks[adapter], 0), a.rank) : a.rank;
-    const float scale = a.scales ? a.scales[adapter] : 1.0f;
-    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    for (int r = warp; r < rank; r += kLoraThreads / kWarp) {
-      const T* w = static_cast<const T*>(a.A) + (static_cast<int64_t>(adapter) * a.rank + r) * a.n;
-      float sum = 0.0f;
-      for (int64_t j = lane; j < a.n; j += kWarp) sum = fmaf(to_float(w[j]), to_float(x[j]), sum);
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-      if (lane == 0) h[r] = sum * scale;
+}
+
+// Elements [at, at + kN) of a row of 16-bit elements, zeros from `end` on (and for no row).
+template <int kN>
+__device__ __forceinline__ void load_row(uint32_t (&v)[kN / 2], const uint16_t* row, int64_t at, int64_t end, bool vector) {
+  if (row != nullptr && vector && at + kN <= end) {
+    if constexpr (kN == 8) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + at));
+      v[0] = x.x;
+      v[1] = x.y;
+      v[2] = x.z;
+      v[3] = x.w;
+    } else {
+      const uint2 x = __ldg(reinterpret_cast<const uint2*>(row + at));
+      v[0] = x.x;
+      v[1] = x.y;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) {
+    const int64_t e = at + 2 * i;
+    const uint32_t lo = row != nullptr && e < end ? __ldg(row + e) : 0;
+    const uint32_t hi = row != nullptr && e + 1 < end ? __ldg(row + e + 1) : 0;
+    v[i] = lo | hi << 16;
+  }
+}
+
+// kSub: 16-row blocks of a tile; kNT: blocks of 8 ranks.
+template <int kSub, int kNT>
+struct LoraShape {
+  static constexpr int kM = 16 * kSub;
+  static constexpr int kR = 8 * kNT;                   // ranks, padded
+  static constexpr int kStride = kR + (kR > 16 ? 16 : 0);  // of the terms' rows: 8-byte reads meet no bank twice
+  static constexpr int kSplit = kLoraWarps / kSub;     // warps that share a block's columns
+  static constexpr int kBlock = kNT < 16 ? kNT : 16;   // rank blocks whose loads are in flight together
+  static constexpr int kSteps = kNT <= 2 ? 3 : kNT <= 4 ? 2 : 1;  // 32-column steps in flight together
+  static constexpr int kPart = kSplit * kM * kR * 4;
+  static constexpr int kTerms = 3 * kM * kStride * 2;
+  static constexpr int kWork = kPart > kTerms ? kPart : kTerms;  // the terms overlay the warps' sums
+  static constexpr int kSmem = kWork + kM * kR * 4;
+};
+
+template <typename T, int kSub, int kNT>
+__global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(const __grid_constant__ LoraArgs a) {
+  using S = LoraShape<kSub, kNT>;
+  constexpr int kTerms = std::is_same_v<T, __half> ? 2 : 3;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* const part = reinterpret_cast<float*>(smem);              // [split][row][rank]
+  uint16_t* const terms = reinterpret_cast<uint16_t*>(smem);       // [term][row][stride]
+  float* const sums = reinterpret_cast<float*>(smem + S::kWork);   // [row][rank] of this CTA
+  __shared__ float unit[S::kM];  // what a row of terms is multiplied by
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cta = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
+  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+  const int row8 = lane / 4, quarter = lane % 4;
+  const int sub = warp % kSub, share = warp / kSub;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x / ctas) * S::kM;
+  wait_for_producers();
+  allow_dependents();
+
+  // The rows' adapters: lane i has row i (and 32 + i); -1 for none, -2 past the last row.
+  int owner[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 32 * i + lane;
+    owner[i] = r < S::kM && row0 + r < a.tokens ? max(a.adapters[row0 + r], -1) : -2;
+    if (owner[i] >= a.count) {
+      if (warp == 0 && cta == 0 && blockIdx.y == 0) report(kDevIndex);
+      owner[i] = -1;
     }
   }
-  __syncthreads();
-  for (int64_t i = threadIdx.x; i < a.m; i += kLoraThreads) {
-    const T* w = static_cast<const T*>(a.B) + (static_cast<int64_t>(max(adapter, 0)) * a.m + i) * a.rank;
-    float sum = 0.0f;
-    for (int r = 0; r < rank; ++r) sum = fmaf(to_float(w[r]), h[r], sum);
-    a.out[row * a.out_stride + i] = a.y[row * a.y_stride + i] + sum;
+  for (int item = blockIdx.y;; item += gridDim.y) {
+    // The item-th distinct adapter, in the order of the rows, and its rows.
+    uint32_t left[2] = {__ballot_sync(kFullMask, owner[0] >= 0), __ballot_sync(kFullMask, owner[1] >= 0)};
+    uint32_t rows[2] = {0, 0};
+    int adapter = -1;
+    for (int i = 0; left[0] | left[1]; ++i) {
+      const int first = left[0] ? __shfl_sync(kFullMask, owner[0], __ffs(left[0]) - 1)
+                                : __shfl_sync(kFullMask, owner[1], __ffs(left[1]) - 1);
+      const uint32_t in0 = __ballot_sync(kFullMask, owner[0] == first), in1 = __ballot_sync(kFullMask, owner[1] == first);
+      if (i == item) {
+        adapter = first;
+        rows[0] = in0;
+        rows[1] = in1;
+        break;
+      }
+      left[0] &= ~in0;
+      left[1] &= ~in1;
+    }
+    if (adapter < 0 && item > 0) return;
+    // Rows without an adapter go with the first item.
+    uint32_t plain[2] = {__ballot_sync(kFullMask, owner[0] == -1), __ballot_sync(kFullMask, owner[1] == -1)};
+    if (item > 0) plain[0] = plain[1] = 0;
+    const int rank = adapter < 0 ? 0 : a.ranks ? min(max(a.ranks[adapter], 0), a.rank) : a.rank;
+    const float scale = adapter >= 0 && a.scales ? a.scales[adapter] : 1.0f;
+    // This warp's 16 rows of the item.
+    const uint32_t active = (sub < 2 ? rows[0] >> 16 * sub : rows[1] >> 16 * (sub - 2)) & 0xffffu;
+    const uint32_t copied = (sub < 2 ? plain[0] >> 16 * sub : plain[1] >> 16 * (sub - 2)) & 0xffffu;
+    const int64_t m_blocks = (a.m + 31) / 32;
+    const int64_t m0 = m_blocks * cta / ctas, m1 = m_blocks * (cta + 1) / ctas;
+    const uint16_t* const Ba = static_cast<const uint16_t*>(a.B) + static_cast<int64_t>(max(adapter, 0)) * a.m * a.rank;
+    if (kSub == 1 && rank > 0) {  // B is not needed before h: have it on its way
+      const char* from = reinterpret_cast<const char*>(Ba + 32 * m0 * a.rank);
+      const int64_t bytes = (min(32 * m1, a.m) - 32 * m0) * a.rank * 2;
+      for (int64_t i = threadIdx.x * 128; i < bytes; i += kLoraThreads * 128) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(from + i));
+      }
+    }
+
+    if (rank > 0) {
+      // 1. This warp's share of A x.
+      float acc[kNT][4];
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+      const int64_t steps = (a.n + 31) / 32;
+      const int64_t k1 = steps * (cta + 1) / ctas;
+      if (active) {
+        const uint16_t* x[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          x[h] = active >> (row8 + 8 * h) & 1u
+                     ? static_cast<const uint16_t*>(a.x) + (row0 + 16 * sub + row8 + 8 * h) * a.x_stride : nullptr;
+        }
+        const uint16_t* const Aa = static_cast<const uint16_t*>(a.A) + static_cast<int64_t>(adapter) * a.rank * a.n;
+        for (int64_t k = steps * cta / ctas + share * S::kSteps; k < k1; k += S::kSplit * S::kSteps) {
+          uint32_t xv[S::kSteps][2][4];
+#pragma unroll
+          for (int u = 0; u < S::kSteps; ++u) {
+            const int64_t end = k + u < k1 ? a.n : 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) load_row<8>(xv[u][h], x[h], 32 * (k + u) + 8 * quarter, end, a.n_vector);
+          }
+#pragma unroll
+          for (int j0 = 0; j0 < kNT; j0 += S::kBlock) {
+            if (8 * j0 < rank) {
+              uint32_t wv[S::kSteps][S::kBlock][4];
+#pragma unroll
+              for (int u = 0; u < S::kSteps; ++u) {
+                const int64_t end = k + u < k1 ? a.n : 0;
+#pragma unroll
+                for (int j = 0; j < S::kBlock; ++j) {
+                  const int r = 8 * (j0 + j) + row8;
+                  load_row<8>(wv[u][j], r < rank ? Aa + r * a.n : nullptr, 32 * (k + u) + 8 * quarter, end, a.n_vector);
+                }
+              }
+#pragma unroll
+              for (int u = 0; u < S::kSteps; ++u) {
+#pragma unroll
+                for (int j = 0; j < S::kBlock; ++j) {
+                  float(&d)[4] = acc[j0 + j];
+                  lora_mma<T>(d, xv[u][0][0], xv[u][1][0], xv[u][0][1], xv[u][1][1], wv[u][j][0], wv[u][j][1]);
+                  lora_mma<T>(d, xv[u][0][2], xv[u][1][2], xv[u][0][3], xv[u][1][3], wv[u][j][2], wv[u][j][3]);
+                }
+              }
+            }
+          }
+        }
+      }
+      // 2. The warps' sums, then the cluster's, in the order of their ranks.
+      float* const mine = part + (share * S::kM + 16 * sub) * S::kR + 2 * quarter;
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) {
+        *reinterpret_cast<float2*>(mine + row8 * S::kR + 8 * j) = make_float2(acc[j][0], acc[j][1]);
+        *reinterpret_cast<float2*>(mine + (row8 + 8) * S::kR + 8 * j) = make_float2(acc[j][2], acc[j][3]);
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < S::kM * S::kR / 4; i += kLoraThreads) {
+        float4 v = reinterpret_cast<const float4*>(part)[i];
+#pragma unroll
+        for (int s = 1; s < S::kSplit; ++s) {
+          const float4 x = reinterpret_cast<const float4*>(part)[s * S::kM * S::kR / 4 + i];
+          v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+        }
+        reinterpret_cast<float4*>(sums)[i] = v;
+      }
+      cluster.sync();
+      for (int r = warp; r < S::kM; r += kLoraWarps) {  // a warp a row
+        constexpr int kPer = (S::kR + kWarp - 1) / kWarp;
+        float h[kPer];
+        float largest = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int c = i * kWarp + lane;
+          h[i] = 0.0f;
+          for (int q = 0; c < S::kR && q < ctas; ++q) h[i] += *cluster.map_shared_rank(sums + r * S::kR + c, q);
+          h[i] *= scale;
+          largest = fmaxf(largest, fabsf(h[i]));
+        }
+        float down = 1.0f;
+        if constexpr (std::is_same_v<T, __half>) {  // the row's largest between 1 and 2
+          for (int o = 16; o; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(kFullMask, largest, o));
+          uint32_t field = __float_as_uint(largest) >> 23;
+          field = field == 0 || field == 255 ? 127 : min(field, 253u);
+          down = __uint_as_float((254u - field) << 23);
+          if (lane == 0) unit[r] = __uint_as_float(field << 23);
+        } else {
+          if (lane == 0) unit[r] = 1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int c = i * kWarp + lane;
+          if (c >= S::kR) continue;
+          float v = h[i] * down;
+#pragma unroll
+          for (int t = 0; t < kTerms; ++t) {
+            const T x = from_float<T>(v);
+            terms[(t * S::kM + r) * S::kStride + c] = *reinterpret_cast<const uint16_t*>(&x);
+            v = isfinite(v) ? v - to_float(x) : 0.0f;
+          }
+        }
+      }
+      if (ctas > 1) cluster.barrier_arrive();  // this CTA has read its peers' sums
+      __syncthreads();
+    }
+
+    // 3. The outputs, 32 columns at a time: block j of a product has the columns 8 t + 2 j + e, so a lane
+    // ends with 8 neighbouring ones of its rows.
+    for (int64_t b = m0 + share; b < m1 && (active | copied); b += S::kSplit) {
+      float acc[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+      for (int k0 = 0; k0 < rank; k0 += 64) {
+        uint32_t w[4][4][2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (k0 + 16 * k < rank) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int64_t c = 32 * b + 8 * (row8 / 2) + 2 * j + row8 % 2;
+              load_row<4>(w[k][j], c < a.m ? Ba + c * a.rank : nullptr, k0 + 16 * k + 4 * quarter, rank, a.rank_vector);
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (k0 + 16 * k < rank) {
+#pragma unroll
+            for (int t = 0; t < kTerms; ++t) {
+              const uint16_t* from = terms + (t * S::kM + 16 * sub + row8) * S::kStride + k0 + 16 * k + 4 * quarter;
+              const uint2 x0 = *reinterpret_cast<const uint2*>(from);
+              const uint2 x1 = *reinterpret_cast<const uint2*>(from + 8 * S::kStride);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) lora_mma<T>(acc[j], x0.x, x1.x, x0.y, x1.y, w[k][j][0], w[k][j][1]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = row8 + 8 * h;
+        const bool on = active >> r & 1u;
+        if (!on && !(copied >> r & 1u)) continue;
+        const float by = on && rank > 0 ? unit[16 * sub + r] : 0.0f;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = on && rank > 0 ? acc[i / 2][2 * h + i % 2] * by : 0.0f;
+        const int64_t c = 32 * b + 8 * quarter;
+        const float* y = a.y + (row0 + 16 * sub + r) * a.y_stride + c;
+        float* out = a.out + (row0 + 16 * sub + r) * a.out_stride + c;
+        if (a.y_vector && c + 8 <= a.m) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float4 from = reinterpret_cast<const float4*>(y)[i];
+            reinterpret_cast<float4*>(out)[i] =
+                make_float4(from.x + v[4 * i], from.y + v[4 * i + 1], from.z + v[4 * i + 2], from.w + v[4 * i + 3]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (c + i < a.m) out[i] = y[i] + v[i];
+          }
+        }
+      }
+    }
+    if (rank > 0) {
+      if (ctas > 1) cluster.barrier_wait();  // the peers have read this CTA's sums
+      __syncthreads();
+    }
   }
+}
+
+template <typename T, int kSub, int kNT>
+cudaError_t launch_lora(const LoraArgs& a, int tiles, int items, int ctas, cudaStream_t stream) {
+  using S = LoraShape<kSub, kNT>;
+  static bool configured[64] = {};
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    const cudaError_t err =
+        cudaFuncSetAttribute(lora_kernel<T, kSub, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (err != cudaSuccess) return err;
+    configured[dev] = true;
+  }
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(tiles) * ctas, static_cast<unsigned>(items));
+  config.blockDim = dim3(kLoraThreads);
+  config.dynamicSmemBytes = S::kSmem;
+  config.stream = stream;
+  config.attrs = attr;
+  config.numAttrs = 2;
+  return cudaLaunchKernelEx(&config, lora_kernel<T, kSub, kNT>, a);
+}
+
+template <typename T, int kSub>
+cudaError_t launch_rank(const LoraArgs& a, int tiles, int items, int ctas, cudaStream_t s) {
+  if (a.rank <= 16) return launch_lora<T, kSub, 2>(a, tiles, items, ctas, s);
+  if (a.rank <= 32) return launch_lora<T, kSub, 4>(a, tiles, items, ctas, s);
+  if (a.rank <= 64) return launch_lora<T, kSub, 8>(a, tiles, items, ctas, s);
+  if (a.rank <= 128) return launch_lora<T, kSub, 16>(a, tiles, items, ctas, s);
+  return launch_lora<T, kSub, 32>(a, tiles, items, ctas, s);
+}
+
+// Up to 256 rows are taken as a decode batch: tiles of 16, an item for each of its rows' adapters, many
+// CTAs an item. More are taken as prompts: tiles of 64, four items at a time (a tile meets one or two),
+// and as many CTAs an item as give the SMs two each.
+template <typename T>
+cudaError_t launch_tokens(const LoraArgs& a, cudaStream_t s) {
+  if (a.tokens <= 256) {
+    const int tiles = static_cast<int>((a.tokens + 15) / 16);
+    const int items = static_cast<int>(a.tokens < 16 ? a.tokens : 16);
+    return launch_rank<T, 1>(a, tiles, items, a.tokens <= 64 ? 8 : 4, s);
+  }
+  const int tiles = static_cast<int>((a.tokens + 63) / 64);
+  int ctas = 8;
+  while (ctas > 1 && tiles * ctas > 2 * 148) ctas /= 2;
+  return launch_rank<T, 4>(a, tiles, 4, ctas, s);
 }
 
 }  // namespace
@@ -70,7 +408,7 @@ extern "C" int pck_lora_add(const void* x, int dtype, int64_t tokens, int64_t n,
                             int64_t out_stride, void* stream) {
   using namespace pck;
   if (dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) return report_error(PCK_ERR_ARGUMENT, "adapters: x must be bfloat16 or float16");
-  if (tokens < 0 || tokens > 0x7fffffffLL || n < 1 || m < 0 || x_stride < n || y_stride < m || out_stride < m) {
+  if (tokens < 0 || tokens > 1 << 30 || n < 1 || m < 0 || x_stride < n || y_stride < m || out_stride < m) {
     return report_error(PCK_ERR_ARGUMENT, "adapters: need tokens >= 0, n >= 1, m >= 0 and strides of whole rows");
   }
   if (count < 0 || count > 0x7fffffffLL) return report_error(PCK_ERR_ARGUMENT, "adapters: bad number of adapters");
@@ -79,15 +417,27 @@ extern "C" int pck_lora_add(const void* x, int dtype, int64_t tokens, int64_t n,
   if (!x || !y || !adapters || !out || (count > 0 && (!A || !B))) {
     return report_error(PCK_ERR_ARGUMENT, "adapters: NULL x, y, A, B, adapters or out");
   }
-  LoraArgs a{x, x_stride, y, y_stride, A, B, adapters, scales, ranks, out, out_stride, n, m,
-             static_cast<int32_t>(count), static_cast<int32_t>(rank)};
-  const unsigned grid = static_cast<unsigned>(tokens);
+  LoraArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.y = y;
+  a.y_stride = y_stride;
+  a.A = A;
+  a.B = B;
+  a.adapters = adapters;
+  a.scales = scales;
+  a.ranks = ranks;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.n = n;
+  a.m = m;
+  a.tokens = tokens;
+  a.count = static_cast<int32_t>(count);
+  a.rank = static_cast<int32_t>(rank);
+  a.n_vector = aligned_to(x, 16) && aligned_to(A, 16) && x_stride % 8 == 0 && n % 8 == 0;
+  a.rank_vector = aligned_to(B, 8) && rank % 4 == 0;
+  a.y_vector = aligned_to(y, 16) && aligned_to(out, 16) && y_stride % 4 == 0 && out_stride % 4 == 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == PCK_LOGITS_BF16) {
-    lora_kernel<__nv_bfloat16><<<grid, kLoraThreads, 0, s>>>(a);
-  } else {
-    lora_kernel<__half><<<grid, kLoraThreads, 0, s>>>(a);
-  }
-  const cudaError_t err = cudaGetLastError();
+  const cudaError_t err = dtype == PCK_LOGITS_BF16 ? launch_tokens<__nv_bfloat16>(a, s) : launch_tokens<__half>(a, s);
   return err == cudaSuccess ? PCK_OK : report_cuda("adapter kernel", err);
 }
