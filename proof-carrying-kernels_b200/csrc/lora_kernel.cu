@@ -26,6 +26,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kLoraMaxRank = 256;
+constexpr int kLoraMaxCtas = 8;  // of a cluster
 constexpr int kLoraWarps = 8;
 constexpr int kLoraThreads = kLoraWarps * kWarp;
 
@@ -62,10 +63,10 @@ __device__ __forceinline__ void lora_mma(float (&d)[4], uint32_t a0, uint32_t a1
   }
 }
 
-// Elements [at, at + kN) of a row of 16-bit elements, zeros from `end` on (and for no row).
+// Elements [at, at + kN) of a row of 16-bit elements, zeros from `end` on.
 template <int kN>
 __device__ __forceinline__ void load_row(uint32_t (&v)[kN / 2], const uint16_t* row, int64_t at, int64_t end, bool vector) {
-  if (row != nullptr && vector && at + kN <= end) {
+  if (vector && at + kN <= end) {
     if constexpr (kN == 8) {
       const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + at));
       v[0] = x.x;
@@ -82,8 +83,8 @@ __device__ __forceinline__ void load_row(uint32_t (&v)[kN / 2], const uint16_t* 
 #pragma unroll
   for (int i = 0; i < kN / 2; ++i) {
     const int64_t e = at + 2 * i;
-    const uint32_t lo = row != nullptr && e < end ? __ldg(row + e) : 0;
-    const uint32_t hi = row != nullptr && e + 1 < end ? __ldg(row + e + 1) : 0;
+    const uint32_t lo = e < end ? __ldg(row + e) : 0;
+    const uint32_t hi = e + 1 < end ? __ldg(row + e + 1) : 0;
     v[i] = lo | hi << 16;
   }
 }
@@ -100,7 +101,7 @@ struct LoraShape {
   static constexpr int kPart = kSplit * kM * kR * 4;
   static constexpr int kTerms = 3 * kM * kStride * 2;
   static constexpr int kWork = kPart > kTerms ? kPart : kTerms;  // the terms overlay the warps' sums
-  static constexpr int kSmem = kWork + kM * kR * 4;
+  static constexpr int kSmem = kWork + 2 * kM * kR * 4;
 };
 
 template <typename T, int kSub, int kNT>
@@ -111,6 +112,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
   float* const part = reinterpret_cast<float*>(smem);              // [split][row][rank]
   uint16_t* const terms = reinterpret_cast<uint16_t*>(smem);       // [term][row][stride]
   float* const sums = reinterpret_cast<float*>(smem + S::kWork);   // [row][rank] of this CTA
+  float* const whole = sums + S::kM * S::kR;                       // and of the cluster
   __shared__ float unit[S::kM];  // what a row of terms is multiplied by
   cg::cluster_group cluster = cg::this_cluster();
   const int cta = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
@@ -176,44 +178,69 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
 #pragma unroll
       for (int j = 0; j < kNT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
       const int64_t steps = (a.n + 31) / 32;
-      const int64_t k1 = steps * (cta + 1) / ctas;
+      const int64_t k0 = steps * cta / ctas, k1 = steps * (cta + 1) / ctas;
       if (active) {
+        // Rows of the tile that are not the item's, and ranks past the adapter's, take another's elements:
+        // what comes of them is not used.
+        const int other = __ffs(active) - 1;
         const uint16_t* x[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          x[h] = active >> (row8 + 8 * h) & 1u
-                     ? static_cast<const uint16_t*>(a.x) + (row0 + 16 * sub + row8 + 8 * h) * a.x_stride : nullptr;
+          const int r = active >> (row8 + 8 * h) & 1u ? row8 + 8 * h : other;
+          x[h] = static_cast<const uint16_t*>(a.x) + (row0 + 16 * sub + r) * a.x_stride;
         }
         const uint16_t* const Aa = static_cast<const uint16_t*>(a.A) + static_cast<int64_t>(adapter) * a.rank * a.n;
-        for (int64_t k = steps * cta / ctas + share * S::kSteps; k < k1; k += S::kSplit * S::kSteps) {
-          uint32_t xv[S::kSteps][2][4];
+        auto product = [&](int j, const uint32_t (&x0)[4], const uint32_t (&x1)[4], const uint32_t (&w)[4]) {
+          lora_mma<T>(acc[j], x0[0], x1[0], x0[1], x1[1], w[0], w[1]);
+          lora_mma<T>(acc[j], x0[2], x1[2], x0[3], x1[3], w[2], w[3]);
+        };
+        // Whole steps by 16-byte loads, kSteps of them in flight together.
+        const int64_t full = a.n_vector ? min(k1, a.n / 32) : k0;
+        int64_t k = k0 + share * S::kSteps;
+        for (; k + S::kSteps <= full; k += S::kSplit * S::kSteps) {
+          uint4 xv[S::kSteps][2];
 #pragma unroll
           for (int u = 0; u < S::kSteps; ++u) {
-            const int64_t end = k + u < k1 ? a.n : 0;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) load_row<8>(xv[u][h], x[h], 32 * (k + u) + 8 * quarter, end, a.n_vector);
+            for (int h = 0; h < 2; ++h) {
+              xv[u][h] = __ldg(reinterpret_cast<const uint4*>(x[h] + 32 * (k + u) + 8 * quarter));
+            }
           }
 #pragma unroll
           for (int j0 = 0; j0 < kNT; j0 += S::kBlock) {
             if (8 * j0 < rank) {
-              uint32_t wv[S::kSteps][S::kBlock][4];
+              uint4 wv[S::kSteps][S::kBlock];
 #pragma unroll
-              for (int u = 0; u < S::kSteps; ++u) {
-                const int64_t end = k + u < k1 ? a.n : 0;
+              for (int j = 0; j < S::kBlock; ++j) {
+                const uint16_t* from = Aa + min(8 * (j0 + j) + row8, rank - 1) * a.n + 32 * k + 8 * quarter;
 #pragma unroll
-                for (int j = 0; j < S::kBlock; ++j) {
-                  const int r = 8 * (j0 + j) + row8;
-                  load_row<8>(wv[u][j], r < rank ? Aa + r * a.n : nullptr, 32 * (k + u) + 8 * quarter, end, a.n_vector);
-                }
+                for (int u = 0; u < S::kSteps; ++u) wv[u][j] = __ldg(reinterpret_cast<const uint4*>(from + 32 * u));
               }
 #pragma unroll
               for (int u = 0; u < S::kSteps; ++u) {
+                const uint32_t x0[4] = {xv[u][0].x, xv[u][0].y, xv[u][0].z, xv[u][0].w};
+                const uint32_t x1[4] = {xv[u][1].x, xv[u][1].y, xv[u][1].z, xv[u][1].w};
 #pragma unroll
                 for (int j = 0; j < S::kBlock; ++j) {
-                  float(&d)[4] = acc[j0 + j];
-                  lora_mma<T>(d, xv[u][0][0], xv[u][1][0], xv[u][0][1], xv[u][1][1], wv[u][j][0], wv[u][j][1]);
-                  lora_mma<T>(d, xv[u][0][2], xv[u][1][2], xv[u][0][3], xv[u][1][3], wv[u][j][2], wv[u][j][3]);
+                  product(j0 + j, x0, x1, {wv[u][j].x, wv[u][j].y, wv[u][j].z, wv[u][j].w});
                 }
+              }
+            }
+          }
+        }
+        // What is left, a step at a time with every element's place looked at: the last columns, or rows
+        // without alignment.
+        for (; k < k1; k += S::kSplit * S::kSteps) {
+          for (int u = 0; u < S::kSteps && k + u < k1; ++u) {
+            uint32_t xv[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) load_row<8>(xv[h], x[h], 32 * (k + u) + 8 * quarter, a.n, a.n_vector);
+#pragma unroll
+            for (int j = 0; j < kNT; ++j) {
+              if (8 * j < rank) {
+                uint32_t wv[4];
+                load_row<8>(wv, Aa + min(8 * j + row8, rank - 1) * a.n, 32 * (k + u) + 8 * quarter, a.n, a.n_vector);
+                product(j, xv[0], xv[1], wv);
               }
             }
           }
@@ -237,6 +264,21 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
         reinterpret_cast<float4*>(sums)[i] = v;
       }
       cluster.sync();
+      for (int i = threadIdx.x; i < S::kM * S::kR / 4; i += kLoraThreads) {
+        float4 v[kLoraMaxCtas];
+#pragma unroll
+        for (int q = 0; q < kLoraMaxCtas; ++q) {
+          v[q] = q < ctas ? *cluster.map_shared_rank(reinterpret_cast<const float4*>(sums) + i, q)
+                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int q = 1; q < kLoraMaxCtas; ++q) {
+          v[0] = make_float4(v[0].x + v[q].x, v[0].y + v[q].y, v[0].z + v[q].z, v[0].w + v[q].w);
+        }
+        reinterpret_cast<float4*>(whole)[i] = v[0];
+      }
+      if (ctas > 1) cluster.barrier_arrive();  // this CTA has read its peers' sums
+      __syncthreads();
       for (int r = warp; r < S::kM; r += kLoraWarps) {  // a warp a row
         constexpr int kPer = (S::kR + kWarp - 1) / kWarp;
         float h[kPer];
@@ -244,9 +286,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           const int c = i * kWarp + lane;
-          h[i] = 0.0f;
-          for (int q = 0; c < S::kR && q < ctas; ++q) h[i] += *cluster.map_shared_rank(sums + r * S::kR + c, q);
-          h[i] *= scale;
+          h[i] = c < rank ? whole[r * S::kR + c] * scale : 0.0f;
           largest = fmaxf(largest, fabsf(h[i]));
         }
         float down = 1.0f;
@@ -272,7 +312,6 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
           }
         }
       }
-      if (ctas > 1) cluster.barrier_arrive();  // this CTA has read its peers' sums
       __syncthreads();
     }
 
@@ -282,16 +321,26 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
       float acc[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+      // (Columns past the last take the last one's elements: they are not stored.)
+      const uint16_t* rows_of_b[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        rows_of_b[j] = Ba + min(32 * b + 8 * (row8 / 2) + 2 * j + row8 % 2, a.m - 1) * a.rank + 4 * quarter;
+      }
       for (int k0 = 0; k0 < rank; k0 += 64) {
         uint32_t w[4][4][2];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if (k0 + 16 * k < rank) {
+          if (k0 + 16 * k + 16 <= rank && a.rank_vector) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const int64_t c = 32 * b + 8 * (row8 / 2) + 2 * j + row8 % 2;
-              load_row<4>(w[k][j], c < a.m ? Ba + c * a.rank : nullptr, k0 + 16 * k + 4 * quarter, rank, a.rank_vector);
+              const uint2 v = __ldg(reinterpret_cast<const uint2*>(rows_of_b[j] + k0 + 16 * k));
+              w[k][j][0] = v.x;
+              w[k][j][1] = v.y;
             }
+          } else if (k0 + 16 * k < rank) {  // the last ranks: what lies past them may be anything
+#pragma unroll
+            for (int j = 0; j < 4; ++j) load_row<4>(w[k][j], rows_of_b[j] - 4 * quarter, k0 + 16 * k + 4 * quarter, rank, a.rank_vector);
           }
         }
 #pragma unroll
@@ -376,19 +425,21 @@ cudaError_t launch_rank(const LoraArgs& a, int tiles, int items, int ctas, cudaS
   if (a.rank <= 16) return launch_lora<T, kSub, 2>(a, tiles, items, ctas, s);
   if (a.rank <= 32) return launch_lora<T, kSub, 4>(a, tiles, items, ctas, s);
   if (a.rank <= 64) return launch_lora<T, kSub, 8>(a, tiles, items, ctas, s);
-  if (a.rank <= 128) return launch_lora<T, kSub, 16>(a, tiles, items, ctas, s);
-  return launch_lora<T, kSub, 32>(a, tiles, items, ctas, s);
+  if constexpr (kSub == 1) {
+    if (a.rank > 128) return launch_lora<T, kSub, 32>(a, tiles, items, ctas, s);
+  }
+  return launch_lora<T, kSub, 16>(a, tiles, items, ctas, s);
 }
 
 // Up to 256 rows are taken as a decode batch: tiles of 16, an item for each of its rows' adapters, many
 // CTAs an item. More are taken as prompts: tiles of 64, four items at a time (a tile meets one or two),
-// and as many CTAs an item as give the SMs two each.
+// and as many CTAs an item as give the SMs two each. (Ranks over 128 leave no room for the sums of 64 rows.)
 template <typename T>
 cudaError_t launch_tokens(const LoraArgs& a, cudaStream_t s) {
-  if (a.tokens <= 256) {
+  if (a.tokens <= 256 || a.rank > 128) {
     const int tiles = static_cast<int>((a.tokens + 15) / 16);
     const int items = static_cast<int>(a.tokens < 16 ? a.tokens : 16);
-    return launch_rank<T, 1>(a, tiles, items, a.tokens <= 64 ? 8 : 4, s);
+    return launch_rank<T, 1>(a, tiles, items, a.tokens <= 32 ? 8 : 4, s);
   }
   const int tiles = static_cast<int>((a.tokens + 63) / 64);
   int ctas = 8;
