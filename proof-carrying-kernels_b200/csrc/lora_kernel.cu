@@ -45,7 +45,7 @@ struct LoraArgs {
   int64_t n, m, tokens;
   int32_t count, rank;
   int32_t n_vector;   // rows of x and A are 16-byte aligned
-  int32_t rank_vector;  // rows of B are 8-byte aligned
+  int32_t rank_vector;  // rows of B are aligned to a load's ranks
   int32_t y_vector;   // rows of y and out are 16-byte aligned
 };
 
@@ -63,30 +63,39 @@ __device__ __forceinline__ void lora_mma(float (&d)[4], uint32_t a0, uint32_t a1
   }
 }
 
-// Elements [at, at + kN) of a row of 16-bit elements, zeros from `end` on.
+// Elements [at, at + kN) of a row of 16-bit elements, zeros from `end` on. A row holds `held` >= end
+// elements, a multiple of kN where `vector` is set; all loads are issued before any is waited for.
 template <int kN>
-__device__ __forceinline__ void load_row(uint32_t (&v)[kN / 2], const uint16_t* row, int64_t at, int64_t end, bool vector) {
-  if (vector && at + kN <= end) {
-    if constexpr (kN == 8) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + at));
-      v[0] = x.x;
-      v[1] = x.y;
-      v[2] = x.z;
-      v[3] = x.w;
-    } else {
-      const uint2 x = __ldg(reinterpret_cast<const uint2*>(row + at));
-      v[0] = x.x;
-      v[1] = x.y;
+__device__ __forceinline__ void load_row(uint32_t (&v)[kN / 2], const uint16_t* row, int64_t at, int64_t end, int64_t held,
+                                         bool vector) {
+  if (vector) {
+#pragma unroll
+    for (int i = 0; i < kN / 2; ++i) v[i] = 0;
+    if (at < held) {
+      if constexpr (kN == 8) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + at));
+        v[0] = x.x;
+        v[1] = x.y;
+        v[2] = x.z;
+        v[3] = x.w;
+      } else {
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(row + at));
+        v[0] = x.x;
+        v[1] = x.y;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kN / 2; ++i) {
+      const int64_t e = at + 2 * i;
+      v[i] = e + 1 < end ? v[i] : e < end ? v[i] & 0xffffu : 0u;
     }
     return;
   }
+  uint32_t x[kN];
 #pragma unroll
-  for (int i = 0; i < kN / 2; ++i) {
-    const int64_t e = at + 2 * i;
-    const uint32_t lo = e < end ? __ldg(row + e) : 0;
-    const uint32_t hi = e + 1 < end ? __ldg(row + e + 1) : 0;
-    v[i] = lo | hi << 16;
-  }
+  for (int i = 0; i < kN; ++i) x[i] = at + i < end ? __ldg(row + at + i) : 0;
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) v[i] = x[2 * i] | x[2 * i + 1] << 16;
 }
 
 // kSub: 16-row blocks of a tile; kNT: blocks of 8 ranks.
@@ -94,15 +103,92 @@ template <int kSub, int kNT>
 struct LoraShape {
   static constexpr int kM = 16 * kSub;
   static constexpr int kR = 8 * kNT;                   // ranks, padded
-  static constexpr int kStride = kR + (kR > 16 ? 16 : 0);  // of the terms' rows: 8-byte reads meet no bank twice
+  static constexpr int kStride = kR + (kR > 16 ? 4 : 0);  // of the terms' rows, for 8-byte reads at all banks
   static constexpr int kSplit = kLoraWarps / kSub;     // warps that share a block's columns
   static constexpr int kBlock = kNT < 16 ? kNT : 16;   // rank blocks whose loads are in flight together
   static constexpr int kSteps = kNT <= 2 ? 3 : kNT <= 4 ? 2 : 1;  // 32-column steps in flight together
   static constexpr int kPart = kSplit * kM * kR * 4;
   static constexpr int kTerms = 3 * kM * kStride * 2;
   static constexpr int kWork = kPart > kTerms ? kPart : kTerms;  // the terms overlay the warps' sums
-  static constexpr int kSmem = kWork + 2 * kM * kR * 4;
+  static constexpr int kSums = kWork + 2 * kM * kR * 4;
+  // Tiles of several blocks: stages of 64 columns of the rows and of A, before the sums take their place.
+  static constexpr int kStageBytes = (kM + kR) * 128;
+  static constexpr int kStages = kNT <= 4 ? 7 : kNT <= 8 ? 6 : 4;
+  static constexpr int kSmem = kSub > 1 && kStages * kStageBytes > kSums ? kStages * kStageBytes : kSums;
 };
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
+// A x of a tile of several 16-row blocks, over the whole pairs of steps of [k0, k1): 64 columns of the rows
+// and of A in a ring of asynchronous copies, which all the warps that share them read (a row's 16-byte
+// pieces are exchanged by the row's parity, so a read meets no bank twice). Returns the step it got to.
+template <typename T, int kSub, int kNT>
+__device__ __forceinline__ int64_t staged_steps(const LoraArgs& a, uint8_t* smem, const uint32_t (&rows)[2], int64_t row0,
+                                                int adapter, int rank, int64_t k0, int64_t k1, bool active,
+                                                float (&acc)[kNT][4]) {
+  using S = LoraShape<kSub, kNT>;
+  if (!a.n_vector) return k0;
+  const int64_t stages = (min(k1, a.n / 32) - k0) / 2;
+  if (stages <= 0) return k0;
+  const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
+  const int row8 = lane / 4, quarter = lane % 4, sub = warp % kSub, share = warp / kSub;
+  const int other = rows[0] ? __ffs(rows[0]) - 1 : 31 + __ffs(rows[1]);
+  const uint16_t* const Aa = static_cast<const uint16_t*>(a.A) + static_cast<int64_t>(adapter) * a.rank * a.n;
+  // The pieces that this thread copies: row i / 8, piece i % 8 of 128 bytes.
+  constexpr int kPieces = (S::kM + S::kR) * 8;
+  constexpr int kMine = (kPieces + kLoraThreads - 1) / kLoraThreads;
+  const int used = (S::kM + rank) * 8;  // (what lies in the ranks past the adapter's is not used)
+  const uint16_t* from[kMine];
+  uint32_t to[kMine];
+#pragma unroll
+  for (int p = 0; p < kMine; ++p) {
+    const int i = p * kLoraThreads + threadIdx.x, r = i / 8, c = i % 8;
+    to[p] = smem_addr(smem) + r * 128 + (c ^ (r % 2 * 4)) * 16;
+    if (r < S::kM) {
+      const int x = (r < 32 ? rows[0] >> r : rows[1] >> (r - 32)) & 1u ? r : other;
+      from[p] = static_cast<const uint16_t*>(a.x) + (row0 + x) * a.x_stride + 32 * k0 + 8 * c;
+    } else {
+      from[p] = Aa + min(r - S::kM, rank - 1) * a.n + 32 * k0 + 8 * c;
+    }
+  }
+  auto copy = [&](int64_t stage) {
+    if (stage < stages) {
+#pragma unroll
+      for (int p = 0; p < kMine; ++p) {
+        if (p * kLoraThreads + static_cast<int>(threadIdx.x) < used) {
+          copy16(to[p] + static_cast<uint32_t>(stage % S::kStages) * S::kStageBytes, from[p] + 64 * stage);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int s = 0; s < S::kStages - 1; ++s) copy(s);
+  for (int64_t stage = 0; stage < stages; ++stage) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+    __syncthreads();  // this stage is there for every warp, and the one before it is read
+    copy(stage + S::kStages - 1);
+    if (active) {
+      const uint8_t* at = smem + stage % S::kStages * S::kStageBytes;
+      auto piece = [&](int r) {
+        return *reinterpret_cast<const uint4*>(at + r * 128 + ((4 * share + quarter) ^ (r % 2 * 4)) * 16);
+      };
+      const uint4 x0 = piece(16 * sub + row8), x1 = piece(16 * sub + row8 + 8);
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) {
+        if (8 * j < rank) {
+          const uint4 w = piece(S::kM + 8 * j + row8);
+          lora_mma<T>(acc[j], x0.x, x1.x, x0.y, x1.y, w.x, w.y);
+          lora_mma<T>(acc[j], x0.z, x1.z, x0.w, x1.w, w.z, w.w);
+        }
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  return k0 + 2 * stages;
+}
 
 template <typename T, int kSub, int kNT>
 __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(const __grid_constant__ LoraArgs a) {
@@ -136,21 +222,31 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
   }
   for (int item = blockIdx.y;; item += gridDim.y) {
     // The item-th distinct adapter, in the order of the rows, and its rows.
-    uint32_t left[2] = {__ballot_sync(kFullMask, owner[0] >= 0), __ballot_sync(kFullMask, owner[1] >= 0)};
     uint32_t rows[2] = {0, 0};
     int adapter = -1;
-    for (int i = 0; left[0] | left[1]; ++i) {
-      const int first = left[0] ? __shfl_sync(kFullMask, owner[0], __ffs(left[0]) - 1)
-                                : __shfl_sync(kFullMask, owner[1], __ffs(left[1]) - 1);
-      const uint32_t in0 = __ballot_sync(kFullMask, owner[0] == first), in1 = __ballot_sync(kFullMask, owner[1] == first);
-      if (i == item) {
-        adapter = first;
-        rows[0] = in0;
-        rows[1] = in1;
-        break;
+    if constexpr (kSub == 1) {
+      const uint32_t like = __match_any_sync(kFullMask, owner[0]);
+      uint32_t firsts = __ballot_sync(kFullMask, owner[0] >= 0 && __ffs(like) - 1 == lane);
+      for (int i = 0; i < item; ++i) firsts &= firsts - 1;
+      if (firsts) {
+        adapter = __shfl_sync(kFullMask, owner[0], __ffs(firsts) - 1);
+        rows[0] = __shfl_sync(kFullMask, like, __ffs(firsts) - 1);
       }
-      left[0] &= ~in0;
-      left[1] &= ~in1;
+    } else {
+      uint32_t left[2] = {__ballot_sync(kFullMask, owner[0] >= 0), __ballot_sync(kFullMask, owner[1] >= 0)};
+      for (int i = 0; left[0] | left[1]; ++i) {
+        const int first = left[0] ? __shfl_sync(kFullMask, owner[0], __ffs(left[0]) - 1)
+                                  : __shfl_sync(kFullMask, owner[1], __ffs(left[1]) - 1);
+        const uint32_t in0 = __ballot_sync(kFullMask, owner[0] == first), in1 = __ballot_sync(kFullMask, owner[1] == first);
+        if (i == item) {
+          adapter = first;
+          rows[0] = in0;
+          rows[1] = in1;
+          break;
+        }
+        left[0] &= ~in0;
+        left[1] &= ~in1;
+      }
     }
     if (adapter < 0 && item > 0) return;
     // Rows without an adapter go with the first item.
@@ -179,6 +275,10 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
       for (int j = 0; j < kNT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
       const int64_t steps = (a.n + 31) / 32;
       const int64_t k0 = steps * cta / ctas, k1 = steps * (cta + 1) / ctas;
+      int64_t k = k0 + share * S::kSteps;
+      if constexpr (kSub > 1) {
+        k = staged_steps<T, kSub, kNT>(a, smem, rows, row0, adapter, rank, k0, k1, active != 0, acc) + share * S::kSteps;
+      }
       if (active) {
         // Rows of the tile that are not the item's, and ranks past the adapter's, take another's elements:
         // what comes of them is not used.
@@ -195,8 +295,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
           lora_mma<T>(acc[j], x0[2], x1[2], x0[3], x1[3], w[2], w[3]);
         };
         // Whole steps by 16-byte loads, kSteps of them in flight together.
-        const int64_t full = a.n_vector ? min(k1, a.n / 32) : k0;
-        int64_t k = k0 + share * S::kSteps;
+        const int64_t full = a.n_vector && kSub == 1 ? min(k1, a.n / 32) : k0;
         for (; k + S::kSteps <= full; k += S::kSplit * S::kSteps) {
           uint4 xv[S::kSteps][2];
 #pragma unroll
@@ -234,12 +333,12 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
           for (int u = 0; u < S::kSteps && k + u < k1; ++u) {
             uint32_t xv[2][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) load_row<8>(xv[h], x[h], 32 * (k + u) + 8 * quarter, a.n, a.n_vector);
+            for (int h = 0; h < 2; ++h) load_row<8>(xv[h], x[h], 32 * (k + u) + 8 * quarter, a.n, a.n, a.n_vector);
 #pragma unroll
             for (int j = 0; j < kNT; ++j) {
               if (8 * j < rank) {
                 uint32_t wv[4];
-                load_row<8>(wv, Aa + min(8 * j + row8, rank - 1) * a.n, 32 * (k + u) + 8 * quarter, a.n, a.n_vector);
+                load_row<8>(wv, Aa + min(8 * j + row8, rank - 1) * a.n, 32 * (k + u) + 8 * quarter, a.n, a.n, a.n_vector);
                 product(j, xv[0], xv[1], wv);
               }
             }
@@ -317,43 +416,89 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
 
     // 3. The outputs, 32 columns at a time: block j of a product has the columns 8 t + 2 j + e, so a lane
     // ends with 8 neighbouring ones of its rows.
+    // Up to 64 ranks of B for a block. A lane takes neighbouring ranks of its column (16 of 64, 8 of 32, 4
+    // of 16), so that a warp's load asks for whole lines of memory: as many 32-byte pieces leave most of
+    // the SM's requests in flight empty.
+    constexpr int kK = S::kR < 64 ? S::kR / 16 : 4;
+    constexpr int kLoad = kK == 1 ? 4 : 8;  // ranks of a load
+    auto load_b = [&](int64_t b, int from, uint32_t (&w)[4][2 * kK]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // (Columns past the last take the last one's elements: they are not stored. Ranks past the stored
+        // ones take others, which clear_b sets to zero: nothing here waits for a load.)
+        const uint16_t* row = Ba + min(32 * b + 8 * (row8 / 2) + 2 * j + row8 % 2, a.m - 1) * a.rank;
+        const int r = from + 4 * kK * quarter;
+#pragma unroll
+        for (int u = 0; u < 4 * kK / kLoad; ++u) {
+          uint32_t* to = &w[j][kLoad / 2 * u];
+          if (a.rank_vector) {
+            const uint16_t* at = row + min(r + kLoad * u, a.rank - kLoad);
+            if constexpr (kLoad == 8) {
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
+              to[0] = v.x;
+              to[1] = v.y;
+              to[2] = v.z;
+              to[3] = v.w;
+            } else {
+              const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+              to[0] = v.x;
+              to[1] = v.y;
+            }
+          } else {
+            load_row<kLoad>(*reinterpret_cast<uint32_t(*)[kLoad / 2]>(to), row, r + kLoad * u, rank, rank, false);
+          }
+        }
+      }
+    };
+    auto clear_b = [&](int from, uint32_t (&w)[4][2 * kK]) {
+      if (rank >= from + 16 * kK) return;
+      const int keep = rank - from - 4 * kK * quarter;  // of this lane's ranks
+#pragma unroll
+      for (int i = 0; i < 2 * kK; ++i) {
+        const uint32_t mask = 2 * i + 1 < keep ? 0xffffffffu : 2 * i < keep ? 0xffffu : 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j][i] &= mask;
+      }
+    };
+    // y of this lane's rows and columns; the next block's is on its way during a product.
+    auto load_y = [&](int64_t b, float4 (&y)[2][2]) {
+      const int64_t c0 = 32 * b + 8 * quarter;
+      if (a.y_vector && c0 + 8 <= a.m) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if ((active | copied) >> (row8 + 8 * h) & 1u) {
+            const float4* from = reinterpret_cast<const float4*>(a.y + (row0 + 16 * sub + row8 + 8 * h) * a.y_stride + c0);
+            y[h][0] = from[0];
+            y[h][1] = from[1];
+          }
+        }
+      }
+    };
+    uint32_t w[4][2 * kK];
+    float4 yv[2][2], next[2][2];
+    constexpr bool kAhead = kNT <= 4;  // (the registers of more ranks leave no room for it)
+    if (kAhead && m0 + share < m1 && (active | copied)) load_y(m0 + share, yv);
     for (int64_t b = m0 + share; b < m1 && (active | copied); b += S::kSplit) {
+      const int64_t c0 = 32 * b + 8 * quarter;
+      const bool vector = a.y_vector && c0 + 8 <= a.m;
+      if (active) load_b(b, 0, w);
+      if (!kAhead) load_y(b, yv);
+      if (kAhead && b + S::kSplit < m1) load_y(b + S::kSplit, next);
       float acc[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-      // (Columns past the last take the last one's elements: they are not stored.)
-      const uint16_t* rows_of_b[4];
+      for (int k0 = 0; k0 < rank && active; k0 += 16 * kK) {
+        if (k0 > 0) load_b(b, k0, w);
+        clear_b(k0, w);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        rows_of_b[j] = Ba + min(32 * b + 8 * (row8 / 2) + 2 * j + row8 % 2, a.m - 1) * a.rank + 4 * quarter;
-      }
-      for (int k0 = 0; k0 < rank; k0 += 64) {
-        uint32_t w[4][4][2];
+        for (int k = 0; k < kK; ++k) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (k0 + 16 * k + 16 <= rank && a.rank_vector) {
+          for (int t = 0; t < kTerms; ++t) {
+            const uint16_t* from = terms + (t * S::kM + 16 * sub + row8) * S::kStride + k0 + 4 * kK * quarter + 4 * k;
+            const uint2 x0 = *reinterpret_cast<const uint2*>(from);
+            const uint2 x1 = *reinterpret_cast<const uint2*>(from + 8 * S::kStride);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint2 v = __ldg(reinterpret_cast<const uint2*>(rows_of_b[j] + k0 + 16 * k));
-              w[k][j][0] = v.x;
-              w[k][j][1] = v.y;
-            }
-          } else if (k0 + 16 * k < rank) {  // the last ranks: what lies past them may be anything
-#pragma unroll
-            for (int j = 0; j < 4; ++j) load_row<4>(w[k][j], rows_of_b[j] - 4 * quarter, k0 + 16 * k + 4 * quarter, rank, a.rank_vector);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (k0 + 16 * k < rank) {
-#pragma unroll
-            for (int t = 0; t < kTerms; ++t) {
-              const uint16_t* from = terms + (t * S::kM + 16 * sub + row8) * S::kStride + k0 + 16 * k + 4 * quarter;
-              const uint2 x0 = *reinterpret_cast<const uint2*>(from);
-              const uint2 x1 = *reinterpret_cast<const uint2*>(from + 8 * S::kStride);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) lora_mma<T>(acc[j], x0.x, x1.x, x0.y, x1.y, w[k][j][0], w[k][j][1]);
-            }
+            for (int j = 0; j < 4; ++j) lora_mma<T>(acc[j], x0.x, x1.x, x0.y, x1.y, w[j][2 * k], w[j][2 * k + 1]);
           }
         }
       }
@@ -366,22 +511,26 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = on && rank > 0 ? acc[i / 2][2 * h + i % 2] * by : 0.0f;
-        const int64_t c = 32 * b + 8 * quarter;
-        const float* y = a.y + (row0 + 16 * sub + r) * a.y_stride + c;
-        float* out = a.out + (row0 + 16 * sub + r) * a.out_stride + c;
-        if (a.y_vector && c + 8 <= a.m) {
+        float* out = a.out + (row0 + 16 * sub + r) * a.out_stride + c0;
+        if (vector) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float4 from = reinterpret_cast<const float4*>(y)[i];
+            const float4 from = yv[h][i];
             reinterpret_cast<float4*>(out)[i] =
                 make_float4(from.x + v[4 * i], from.y + v[4 * i + 1], from.z + v[4 * i + 2], from.w + v[4 * i + 3]);
           }
         } else {
+          const float* y = a.y + (row0 + 16 * sub + r) * a.y_stride + c0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            if (c + i < a.m) out[i] = y[i] + v[i];
+            if (c0 + i < a.m) out[i] = y[i] + v[i];
           }
         }
+      }
+#pragma unroll
+      for (int h = 0; kAhead && h < 2; ++h) {
+        yv[h][0] = next[h][0];
+        yv[h][1] = next[h][1];
       }
     }
     if (rank > 0) {
@@ -432,7 +581,7 @@ cudaError_t launch_rank(const LoraArgs& a, int tiles, int items, int ctas, cudaS
 }
 
 // Up to 256 rows are taken as a decode batch: tiles of 16, an item for each of its rows' adapters, many
-// CTAs an item. More are taken as prompts: tiles of 64, four items at a time (a tile meets one or two),
+// CTAs an item. More are taken as prompts: tiles of 64, two items at a time (a tile rarely meets more),
 // and as many CTAs an item as give the SMs two each. (Ranks over 128 leave no room for the sums of 64 rows.)
 template <typename T>
 cudaError_t launch_tokens(const LoraArgs& a, cudaStream_t s) {
@@ -444,7 +593,7 @@ cudaError_t launch_tokens(const LoraArgs& a, cudaStream_t s) {
   const int tiles = static_cast<int>((a.tokens + 63) / 64);
   int ctas = 8;
   while (ctas > 1 && tiles * ctas > 2 * 148) ctas /= 2;
-  return launch_rank<T, 4>(a, tiles, 4, ctas, s);
+  return launch_rank<T, 4>(a, tiles, 2, ctas, s);
 }
 
 }  // namespace
@@ -486,7 +635,8 @@ extern "C" int pck_lora_add(const void* x, int dtype, int64_t tokens, int64_t n,
   a.count = static_cast<int32_t>(count);
   a.rank = static_cast<int32_t>(rank);
   a.n_vector = aligned_to(x, 16) && aligned_to(A, 16) && x_stride % 8 == 0 && n % 8 == 0;
-  a.rank_vector = aligned_to(B, 8) && rank % 4 == 0;
+  const int piece = rank <= 16 ? 4 : 8;  // ranks that a load takes
+  a.rank_vector = aligned_to(B, 2 * piece) && rank % piece == 0;
   a.y_vector = aligned_to(y, 16) && aligned_to(out, 16) && y_stride % 4 == 0 && out_stride % 4 == 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t err = dtype == PCK_LOGITS_BF16 ? launch_tokens<__nv_bfloat16>(a, s) : launch_tokens<__half>(a, s);
