@@ -412,7 +412,8 @@ int pck_peer_all_gather(const pck_peer_gather* gather, void* stream);
 
 /*
  * The operators below have no counterpart in the reference and are not part of the trusted
- * path. Element types are PCK_LOGITS_F32, _BF16 and _F16. Indices that they read from device
+ * path. Each takes a descriptor (every field 8 bytes wide, read during the call) and a stream.
+ * Element types are PCK_LOGITS_F32, _BF16 and _F16. Indices that they read from device
  * memory (slots, pages, adapters, token ids) are checked by the kernels: a page, slot or
  * adapter beyond its range is left out and sets bit 1 of pck_device_status.
  *
@@ -436,10 +437,19 @@ int pck_peer_all_gather(const pck_peer_gather* gather, void* stream);
  * and v_values (both or neither) get the values that the codes stand for, (tokens, kv_heads, dim)
  * of `dtype`, whatever the slot.
  */
-int pck_kv4_append(void* cache, int64_t pages, int64_t kv_heads, int64_t page_tiles, int64_t dim, const void* k,
-                   const void* v, int dtype, int64_t tokens, int64_t k_token_stride, int64_t k_head_stride,
-                   int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots, void* k_values, void* v_values,
-                   void* stream);
+typedef struct pck_kv4_append_desc {
+  void* cache;
+  int64_t pages, kv_heads, page_tiles, dim;
+  const void* k;
+  const void* v;
+  int64_t dtype;
+  int64_t tokens;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const int64_t* slots;
+  void* k_values;
+  void* v_values;
+} pck_kv4_append_desc;
+int pck_kv4_append(const pck_kv4_append_desc* desc, void* stream);
 
 /*
  * Attention over the cache: q (batch, queries, heads, dim) bfloat16 or float16 by its strides (the
@@ -454,11 +464,23 @@ int pck_kv4_append(void* cache, int64_t pages, int64_t kv_heads, int64_t page_ti
  */
 int64_t pck_kv4_attention_scratch(int64_t batch, int64_t queries, int64_t heads, int64_t kv_heads, int64_t dim,
                                   int64_t max_tokens);
-int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_t queries, int64_t heads, int64_t dim,
-                      int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride, const void* cache,
-                      int64_t pages, int64_t kv_heads, int64_t page_tiles, const int32_t* page_table,
-                      int64_t table_stride, int64_t table_pages, const int32_t* lengths, double scale, int64_t window,
-                      void* out, void* scratch, int64_t scratch_bytes, void* stream);
+typedef struct pck_kv4_attention_desc {
+  const void* q;
+  int64_t dtype;
+  int64_t batch, queries, heads, dim;
+  int64_t q_batch_stride, q_token_stride, q_head_stride;
+  const void* cache;
+  int64_t pages, kv_heads, page_tiles;
+  const int32_t* page_table;
+  int64_t table_stride, table_pages;
+  const int32_t* lengths;
+  double scale;
+  int64_t window;
+  void* out;
+  void* scratch;
+  int64_t scratch_bytes;
+} pck_kv4_attention_desc;
+int pck_kv4_attention(const pck_kv4_attention_desc* desc, void* stream);
 
 /*
  * Low-rank adapters of many requests beside a shared projection: out = y + s_a B_a (A_a x) for
@@ -468,9 +490,22 @@ int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_t queries, 
  * [0, rank] (the rest of A and B is not used) or is NULL. rank in [1, 256]. The intermediate A x is
  * held in binary32.
  */
-int pck_lora_add(const void* x, int dtype, int64_t tokens, int64_t n, int64_t x_stride, const float* y, int64_t m,
-                 int64_t y_stride, const void* A, const void* B, int64_t count, int64_t rank, const int32_t* adapters,
-                 const float* scales, const int32_t* ranks, float* out, int64_t out_stride, void* stream);
+typedef struct pck_lora_desc {
+  const void* x;
+  int64_t dtype;
+  int64_t tokens, n, x_stride;
+  const float* y;
+  int64_t m, y_stride;
+  const void* A;
+  const void* B;
+  int64_t count, rank;
+  const int32_t* adapters;
+  const float* scales;
+  const int32_t* ranks;
+  float* out;
+  int64_t out_stride;
+} pck_lora_desc;
+int pck_lora_add(const pck_lora_desc* desc, void* stream);
 
 /*
  * Logits (rows, vocab) of `dtype` to binary32 `out` (which may be the logits), in this order, each
@@ -486,11 +521,27 @@ int pck_lora_add(const void* x, int dtype, int64_t tokens, int64_t n, int64_t x_
  * (`biases` entries in all). Ids outside the vocabulary are skipped. tokens, each penalty (rows),
  * bias_starts and mask may be NULL.
  */
-int pck_process_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
-                       const int64_t* tokens, int64_t token_stride, int64_t max_tokens, const int32_t* prompt_lengths,
-                       const int32_t* lengths, const float* repetition, const float* frequency, const float* presence,
-                       const int32_t* bias_starts, const int64_t* bias_ids, const float* bias_values, int64_t biases,
-                       const int32_t* mask, int64_t mask_stride, float* out, int64_t out_stride, void* stream);
+typedef struct pck_logits_desc {
+  const void* logits;
+  int64_t dtype;
+  int64_t rows, vocab, row_stride;
+  const int64_t* tokens;
+  int64_t token_stride, max_tokens;
+  const int32_t* prompt_lengths;
+  const int32_t* lengths;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  const int32_t* bias_starts;
+  const int64_t* bias_ids;
+  const float* bias_values;
+  int64_t biases;
+  const int32_t* mask;
+  int64_t mask_stride;
+  float* out;
+  int64_t out_stride;
+} pck_logits_desc;
+int pck_process_logits(const pck_logits_desc* desc, void* stream);
 
 #ifdef __cplusplus
 }

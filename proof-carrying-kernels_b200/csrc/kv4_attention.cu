@@ -1064,12 +1064,10 @@ extern "C" int64_t pck_kv4_attention_scratch(int64_t batch, int64_t queries, int
   return pck::scratch_size(parts, rows, dim, batch * kv_heads * blocks);
 }
 
-extern "C" int pck_kv4_attention(const void* q, int dtype, int64_t batch, int64_t queries, int64_t heads, int64_t dim,
-                                 int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride, const void* cache,
-                                 int64_t pages, int64_t kv_heads, int64_t page_tiles, const int32_t* page_table,
-                                 int64_t table_stride, int64_t table_pages, const int32_t* lengths, double scale,
-                                 int64_t window, void* out, void* scratch, int64_t scratch_bytes, void* stream) {
+extern "C" int pck_kv4_attention(const pck_kv4_attention_desc* desc, void* stream) {
   using namespace pck;
+  if (!desc) return report_error(PCK_ERR_ARGUMENT, "attention: NULL descriptor");
+  const auto& [q, dtype, batch, queries, heads, dim, q_batch_stride, q_token_stride, q_head_stride, cache, pages, kv_heads, page_tiles, page_table, table_stride, table_pages, lengths, scale, window, out, scratch, scratch_bytes] = *desc;
   if (dim != 64 && dim != 128 && dim != 256) return report_error(PCK_ERR_ARGUMENT, "attention: dim must be 64, 128 or 256");
   if (dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) return report_error(PCK_ERR_ARGUMENT, "attention: q must be bfloat16 or float16");
   if (batch < 0 || queries < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || heads > 0xffff ||

@@ -105,13 +105,10 @@ cudaError_t launch_logits(LogitsArgs a, int64_t rows, cudaStream_t stream) {
 }  // namespace
 }  // namespace pck
 
-extern "C" int pck_process_logits(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
-                                  const int64_t* tokens, int64_t token_stride, int64_t max_tokens,
-                                  const int32_t* prompt_lengths, const int32_t* lengths, const float* repetition,
-                                  const float* frequency, const float* presence, const int32_t* bias_starts,
-                                  const int64_t* bias_ids, const float* bias_values, int64_t biases, const int32_t* mask,
-                                  int64_t mask_stride, float* out, int64_t out_stride, void* stream) {
+extern "C" int pck_process_logits(const pck_logits_desc* desc, void* stream) {
   using namespace pck;
+  if (!desc) return report_error(PCK_ERR_ARGUMENT, "logits: NULL descriptor");
+  const auto& [logits, dtype, rows, vocab, row_stride, tokens, token_stride, max_tokens, prompt_lengths, lengths, repetition, frequency, presence, bias_starts, bias_ids, bias_values, biases, mask, mask_stride, out, out_stride] = *desc;
   if (dtype != PCK_LOGITS_F32 && dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) {
     return report_error(PCK_ERR_ARGUMENT, "logits: unknown dtype");
   }

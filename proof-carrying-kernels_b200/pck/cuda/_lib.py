@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().parent.parent / "_lib" / "libpck_b200.so"
@@ -66,6 +67,14 @@ class PeerGather(ctypes.Structure):
     ]  # fmt: skip
 
 
+# Descriptors of the serving operators: 8-byte fields in the header's order, packed by one call (a
+# ctypes structure, or as many arguments, costs a decode step several times as much). Pointers are
+# addresses, 0 for NULL.
+KV4_APPEND = struct.Struct("@16q")  # pck_kv4_append_desc
+KV4_ATTENTION = struct.Struct("@17qd4q")  # pck_kv4_attention_desc
+LORA = struct.Struct("@17q")  # pck_lora_desc
+LOGITS = struct.Struct("@21q")  # pck_logits_desc
+
 _SIGNATURES = {
     "pck_last_error": ([], ctypes.c_char_p),
     "pck_abi_version": ([], _int),
@@ -96,13 +105,11 @@ _SIGNATURES = {
     "pck_peer_import": ([_p, ctypes.POINTER(_p)], _int),
     "pck_peer_close": ([_p], _int),
     "pck_peer_all_gather": ([ctypes.POINTER(PeerGather), _p], _int),
-    "pck_kv4_append": ([_p, _i64, _i64, _i64, _i64, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p], _int),
+    "pck_kv4_append": ([ctypes.c_char_p, _p], _int),  # packed descriptors, see KV4_APPEND and the others
     "pck_kv4_attention_scratch": ([_i64, _i64, _i64, _i64, _i64, _i64], _i64),
-    "pck_kv4_attention": ([_p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p,
-                           _f64, _i64, _p, _p, _i64, _p], _int),
-    "pck_lora_add": ([_p, _int, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _p, _i64, _p], _int),
-    "pck_process_logits": ([_p, _int, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64,
-                            _p, _i64, _p], _int),
+    "pck_kv4_attention": ([ctypes.c_char_p, _p], _int),
+    "pck_lora_add": ([ctypes.c_char_p, _p], _int),
+    "pck_process_logits": ([ctypes.c_char_p, _p], _int),
 }
 
 EXPORTED = tuple(_SIGNATURES)

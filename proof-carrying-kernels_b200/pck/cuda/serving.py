@@ -18,7 +18,7 @@ import functools
 import torch
 
 from pck.cuda import _lib
-from pck.cuda._ext import on_device, type_name
+from pck.cuda._ext import type_name
 
 KV4_TILE = 16
 """Tokens of a cache tile; a page holds a whole number of them."""
@@ -27,31 +27,51 @@ KV4_GROUP = 64
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PCK_LOGITS_*
 _HALF = {torch.bfloat16: 1, torch.float16: 2}
+_CONTIGUOUS = torch.contiguous_format
+
+# A decode step makes many of these calls, each shorter on the GPU than a dozen Python calls, so the
+# checks use the cheapest accessors and the arguments travel as one packed descriptor.
 
 
-def _tensor(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> int:
-    """Pointer of a contiguous tensor of the given type on the device."""
+def _tensor(t: torch.Tensor, name: str, dtype: torch.dtype, index: int) -> int:
+    """Pointer of a contiguous tensor of the given type on CUDA device `index`."""
     if t.dtype is not dtype:
         raise RuntimeError(f"{name} must be {type_name(dtype)}, got {type_name(t.dtype)}")
-    if t.device != device:
-        raise RuntimeError(f"{name} must be on {device}")
+    if t.get_device() != index:
+        raise RuntimeError(f"{name} must be on cuda:{index}")
     if not t.is_contiguous():
         raise RuntimeError(f"{name} must be contiguous")
     return t.data_ptr()
 
 
-def _cuda(t: torch.Tensor, name: str) -> torch.device:
+def _per_row(t: torch.Tensor | None, name: str, dtype: torch.dtype, index: int, count: int) -> int:
+    """Pointer of one value per row (0 for none)."""
+    if t is None:
+        return 0
+    if t.shape != (count,):
+        raise RuntimeError(f"{name} must have shape ({count},)")
+    return _tensor(t, name, dtype, index)
+
+
+def _index(t: torch.Tensor, name: str) -> int:
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
-    return t.device
+    return t.get_device()
 
 
-def _call(fn: str, device: torch.device, *args) -> None:
-    lib = _lib.library()
-    with on_device(device):
-        rc = getattr(lib, fn)(*args, torch._C._cuda_getCurrentRawStream(device.index))
+@functools.cache
+def _entry(name: str):
+    return getattr(_lib.library(), name)
+
+
+def _call(name: str, index: int, descriptor: bytes) -> None:
+    if torch._C._cuda_getDevice() == index:
+        rc = _entry(name)(descriptor, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = _entry(name)(descriptor, torch._C._cuda_getCurrentRawStream(index))
     if rc:
-        _lib.check(rc, fn)
+        _lib.check(rc, name)
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -83,13 +103,14 @@ def kv4_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, device: 
     return torch.zeros(pages, kv_heads, page_size // KV4_TILE, 18 * head_dim, dtype=torch.uint8, device=device)
 
 
-def _cache(cache: torch.Tensor, device: torch.device) -> tuple[int, int, int, int]:
+def _cache(cache: torch.Tensor, index: int) -> tuple[int, int, int, int]:
     """(pages, kv_heads, tiles of a page, dim) of a cache."""
-    if cache.dim() != 4 or cache.dtype is not torch.uint8 or cache.size(3) not in (1152, 2304, 4608):
+    shape = cache.shape
+    if len(shape) != 4 or cache.dtype is not torch.uint8 or shape[3] not in (1152, 2304, 4608):
         raise RuntimeError("cache must be uint8 (pages, kv_heads, page_size / 16, 18 * dim) with dim 64, 128 or 256")
-    if cache.device != device or not cache.is_contiguous():
-        raise RuntimeError(f"cache must be contiguous on {device}")
-    pages, heads, tiles, size = cache.shape
+    if cache.get_device() != index or not cache.is_contiguous():
+        raise RuntimeError(f"cache must be contiguous on cuda:{index}")
+    pages, heads, tiles, size = shape
     return pages, heads, tiles, size // 18
 
 
@@ -104,29 +125,34 @@ def kv4_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: tor
     group that holds a NaN or an infinity is stored, and read back, as NaN. With ``values`` the
     call returns (k, v) as the cache holds them, in the input's type, left-out tokens included: an
     attention over the fresh prompt with these sees what later decode steps will see."""
-    device = _cuda(k, "k")
-    pages, heads, tiles, dim = _cache(cache, device)
+    index = _index(k, "k")
+    pages, heads, tiles, dim = _cache(cache, index)
     code = _TYPES.get(k.dtype)
     if code is None or v.dtype is not k.dtype:
         raise RuntimeError("k and v must both be float32, bfloat16 or float16")
-    if k.dim() != 3 or k.shape != v.shape or k.size(1) != heads or k.size(2) != dim:
-        raise RuntimeError(f"expected k and v of shape (tokens, {heads}, {dim}), got {list(k.shape)} and {list(v.shape)}")
-    if v.device != device or k.stride(2) != 1 or v.stride(2) != 1:
-        raise RuntimeError(f"k and v must be on {device} with unit channel stride")
-    tokens = k.size(0)
-    if slots.dim() != 1 or slots.size(0) != tokens:
-        raise RuntimeError(f"slots must have shape ({tokens},)")
-    out = (torch.empty(k.shape, dtype=k.dtype, device=device), torch.empty(k.shape, dtype=k.dtype, device=device)) if values else None
-    _call("pck_kv4_append", device, cache.data_ptr(), pages, heads, tiles, dim, k.data_ptr(), v.data_ptr(), code, tokens,
-          k.stride(0), k.stride(1), v.stride(0), v.stride(1), _tensor(slots, "slots", torch.int64, device),
-          out[0].data_ptr() if out else None, out[1].data_ptr() if out else None)  # fmt: skip
+    shape = k.shape
+    if len(shape) != 3 or v.shape != shape or shape[1] != heads or shape[2] != dim:
+        raise RuntimeError(f"expected k and v of shape (tokens, {heads}, {dim}), got {list(shape)} and {list(v.shape)}")
+    (kt, kh, kc), (vt, vh, vc) = k.stride(), v.stride()
+    if v.get_device() != index or kc != 1 or vc != 1:
+        raise RuntimeError(f"k and v must be on cuda:{index} with unit channel stride")
+    tokens = shape[0]
+    slot_ptr = _per_row(slots, "slots", torch.int64, index, tokens)
+    out = None
+    k_ptr = v_ptr = 0
+    if values:
+        out = (torch.empty_like(k, memory_format=_CONTIGUOUS), torch.empty_like(v, memory_format=_CONTIGUOUS))
+        k_ptr, v_ptr = out[0].data_ptr(), out[1].data_ptr()
+    _call("pck_kv4_append", index, _lib.KV4_APPEND.pack(
+        cache.data_ptr(), pages, heads, tiles, dim, k.data_ptr(), v.data_ptr(), code, tokens, kt, kh, vt, vh, slot_ptr, k_ptr,
+        v_ptr))  # fmt: skip
     return out
 
 
 @functools.lru_cache(maxsize=4096)
-def _scratch_bytes(device: int, batch: int, queries: int, heads: int, kv_heads: int, dim: int, max_tokens: int) -> int:
-    with on_device(torch.device("cuda", device)):
-        return _lib.library().pck_kv4_attention_scratch(batch, queries, heads, kv_heads, dim, max_tokens)
+def _scratch_bytes(index: int, batch: int, queries: int, heads: int, kv_heads: int, dim: int, max_tokens: int) -> int:
+    with torch.cuda.device(index):
+        return _entry("pck_kv4_attention_scratch")(batch, queries, heads, kv_heads, dim, max_tokens)
 
 
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -140,38 +166,49 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     length are not read). Query token t sees tokens up to its own; with ``window`` > 0 the last
     ``window`` of those. One that sees nothing (an empty request) gives zeros. heads is a multiple
     of the cache's kv_heads; ``scale`` is dim**-0.5 by default."""
-    device = _cuda(q, "q")
-    pages, kv_heads, tiles, dim = _cache(cache, device)
-    code = _HALF.get(q.dtype)
+    index = _index(q, "q")
+    pages, kv_heads, tiles, dim = _cache(cache, index)
+    dtype = q.dtype
+    code = _HALF.get(dtype)
     if code is None:
-        raise RuntimeError(f"q must be bfloat16 or float16, got {type_name(q.dtype)}")
-    shape = q.shape
-    if q.dim() == 3:
-        q = q.unsqueeze(1)
-    if q.dim() != 4 or q.size(3) != dim or q.size(2) % kv_heads or q.size(2) == 0 or q.size(1) == 0:
+        raise RuntimeError(f"q must be bfloat16 or float16, got {type_name(dtype)}")
+    shape, strides = q.shape, q.stride()
+    if len(shape) == 4:
+        batch, queries, heads, channels = shape
+        qb, qt, qh, qc = strides
+    elif len(shape) == 3:
+        batch, heads, channels = shape
+        queries = 1
+        qb, qh, qc = strides
+        qt = 0
+    else:
+        heads = channels = 0
+    if channels != dim or heads == 0 or heads % kv_heads or queries == 0:
         raise RuntimeError(f"expected q of shape (batch, queries, heads, {dim}) with heads a multiple of {kv_heads}, got {list(shape)}")
-    if q.stride(3) != 1:
+    if qc != 1:
         raise RuntimeError("q must have unit channel stride")
-    batch, queries, heads = q.size(0), q.size(1), q.size(2)
-    if page_table.dim() != 2 or page_table.size(0) != batch or lengths.dim() != 1 or lengths.size(0) != batch:
+    table_shape = page_table.shape
+    if len(table_shape) != 2 or table_shape[0] != batch or lengths.shape != (batch,):
         raise RuntimeError(f"page_table must have shape ({batch}, pages) and lengths ({batch},)")
-    if page_table.dtype is not torch.int32 or page_table.device != device or (page_table.size(1) > 1 and page_table.stride(1) != 1):
-        raise RuntimeError(f"page_table must be Int on {device} with unit column stride")
+    table_pages = table_shape[1]
+    table_stride, column = page_table.stride()
+    if page_table.dtype is not torch.int32 or page_table.get_device() != index or (table_pages > 1 and column != 1):
+        raise RuntimeError(f"page_table must be Int on cuda:{index} with unit column stride")
     if window < 0:
         raise RuntimeError("window must be 0 (none) or positive")
-    table_pages = page_table.size(1)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=device)
+        out = torch.empty_like(q, memory_format=_CONTIGUOUS)
     elif out.shape != shape:
         raise RuntimeError(f"out must have shape {list(shape)}")
     elif _overlaps(out, q) or _overlaps(out, cache):
         raise RuntimeError("out must not share memory with q or the cache")
-    bytes_ = _scratch_bytes(device.index, batch, queries, heads, kv_heads, dim, table_pages * tiles * KV4_TILE)
-    scratch = torch.empty(bytes_, dtype=torch.uint8, device=device) if bytes_ > 0 else None
-    _call("pck_kv4_attention", device, q.data_ptr(), code, batch, queries, heads, dim, q.stride(0), q.stride(1), q.stride(2),
-          cache.data_ptr(), pages, kv_heads, tiles, page_table.data_ptr(), max(page_table.stride(0), table_pages), table_pages,
-          _tensor(lengths, "lengths", torch.int32, device), dim**-0.5 if scale is None else float(scale), window,
-          _tensor(out, "out", q.dtype, device), scratch.data_ptr() if scratch is not None else None, bytes_)  # fmt: skip
+    size = _scratch_bytes(index, batch, queries, heads, kv_heads, dim, table_pages * tiles * KV4_TILE)
+    scratch = cache.new_empty((size,)) if size > 0 else None
+    _call("pck_kv4_attention", index, _lib.KV4_ATTENTION.pack(
+        q.data_ptr(), code, batch, queries, heads, dim, qb, qt, qh, cache.data_ptr(), pages, kv_heads, tiles,
+        page_table.data_ptr(), table_stride if table_stride > table_pages else table_pages, table_pages,
+        _tensor(lengths, "lengths", torch.int32, index), dim**-0.5 if scale is None else scale, window,
+        _tensor(out, "out", dtype, index), 0 if scratch is None else scratch.data_ptr(), size))  # fmt: skip
     return out
 
 
@@ -190,42 +227,42 @@ def lora_add(x: torch.Tensor, y: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     (default 1) multiplies, ``ranks`` (count,) int32 gives an adapter's own rank (at most the
     stored one; the rest is not used). rank is at most 256. The result is ``out`` (float32; may be
     y) or a new tensor. A checked y must have been decided before it is overwritten."""
-    device = _cuda(x, "x")
-    code = _HALF.get(x.dtype)
-    if code is None or A.dtype is not x.dtype or B.dtype is not x.dtype:
+    index = _index(x, "x")
+    dtype = x.dtype
+    code = _HALF.get(dtype)
+    if code is None or A.dtype is not dtype or B.dtype is not dtype:
         raise RuntimeError("x, A and B must all be bfloat16 or all float16")
-    if x.dim() != 2 or y.dim() != 2 or A.dim() != 3 or B.dim() != 3:
+    x_shape, y_shape, a_shape = x.shape, y.shape, A.shape
+    if len(x_shape) != 2 or len(y_shape) != 2 or len(a_shape) != 3:
         raise RuntimeError("expected x (tokens, n), y (tokens, m), A (count, rank, n) and B (count, m, rank)")
-    tokens, n = x.shape
-    m = y.size(1)
-    count, rank = A.size(0), A.size(1)
-    if y.size(0) != tokens or A.size(2) != n or tuple(B.shape) != (count, m, rank):
-        raise RuntimeError(f"expected x (tokens, n), y (tokens, m), A (count, rank, n) and B (count, m, rank), got {list(x.shape)}, "
-                           f"{list(y.shape)}, {list(A.shape)} and {list(B.shape)}")  # fmt: skip
-    if y.dtype is not torch.float32 or y.device != device:
-        raise RuntimeError(f"y must be Float on {device}")
-    if (n > 1 and x.stride(1) != 1) or (m > 1 and y.stride(1) != 1):
+    tokens, n = x_shape
+    m = y_shape[1]
+    count, rank, _ = a_shape
+    if y_shape[0] != tokens or a_shape[2] != n or B.shape != (count, m, rank):
+        raise RuntimeError(f"expected x (tokens, n), y (tokens, m), A (count, rank, n) and B (count, m, rank), got {list(x_shape)}, "
+                           f"{list(y_shape)}, {list(a_shape)} and {list(B.shape)}")  # fmt: skip
+    if y.dtype is not torch.float32 or y.get_device() != index:
+        raise RuntimeError(f"y must be Float on cuda:{index}")
+    (x_stride, x_column), (y_stride, y_column) = x.stride(), y.stride()
+    if (n > 1 and x_column != 1) or (m > 1 and y_column != 1):
         raise RuntimeError("x and y must have unit column stride")
-    if tuple(adapters.shape) != (tokens,):
-        raise RuntimeError(f"adapters must have shape ({tokens},)")
-    for t, name in ((scales, "scales"), (ranks, "ranks")):
-        if t is not None and tuple(t.shape) != (count,):
-            raise RuntimeError(f"{name} must have shape ({count},)")
     if out is None:
-        out = torch.empty((tokens, m), dtype=torch.float32, device=device)
+        out = torch.empty_like(y, memory_format=_CONTIGUOUS)
+        out_stride = m
     else:
-        if tuple(out.shape) != (tokens, m) or out.dtype is not torch.float32 or out.device != device or (m > 1 and out.stride(1) != 1):
-            raise RuntimeError(f"out must be Float ({tokens}, {m}) on {device} with unit column stride")
-        if tokens > 1 and out.stride(0) < m:
+        if out.shape != y_shape or out.dtype is not torch.float32 or out.get_device() != index or (m > 1 and out.stride(1) != 1):
+            raise RuntimeError(f"out must be Float ({tokens}, {m}) on cuda:{index} with unit column stride")
+        out_stride = out.stride(0)
+        if tokens > 1 and out_stride < m:
             raise RuntimeError("out must not overlap itself")
         same = out.data_ptr() == y.data_ptr() and out.stride() == y.stride()
         if (not same and _overlaps(out, y)) or any(_overlaps(out, t) for t in (x, A, B, adapters)):
             raise RuntimeError("out must be y itself or share no memory with the inputs")
-    _call("pck_lora_add", device, x.data_ptr(), code, tokens, n, max(x.stride(0), n), y.data_ptr(), m, max(y.stride(0), m),
-          _tensor(A, "A", x.dtype, device), _tensor(B, "B", x.dtype, device), count, rank,
-          _tensor(adapters, "adapters", torch.int32, device),
-          None if scales is None else _tensor(scales, "scales", torch.float32, device),
-          None if ranks is None else _tensor(ranks, "ranks", torch.int32, device), out.data_ptr(), max(out.stride(0), m))  # fmt: skip
+    _call("pck_lora_add", index, _lib.LORA.pack(
+        x.data_ptr(), code, tokens, n, x_stride if x_stride > n else n, y.data_ptr(), m, y_stride if y_stride > m else m,
+        _tensor(A, "A", dtype, index), _tensor(B, "B", dtype, index), count, rank,
+        _per_row(adapters, "adapters", torch.int32, index, tokens), _per_row(scales, "scales", torch.float32, index, count),
+        _per_row(ranks, "ranks", torch.int32, index, count), out.data_ptr(), out_stride if out_stride > m else m))  # fmt: skip
     return out
 
 
@@ -250,69 +287,83 @@ def process_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, 
     twice the last counts. ``mask`` (rows, ceil(vocab / 32)) int32: a token whose bit is 0 becomes
     -inf, whatever its logit was. Ids outside the vocabulary are skipped. ``out`` may be the logits
     themselves (float32)."""
-    device = _cuda(logits, "logits")
+    index = _index(logits, "logits")
     code = _TYPES.get(logits.dtype)
     if code is None:
         raise RuntimeError(f"logits must be float32, bfloat16 or float16, got {type_name(logits.dtype)}")
-    if logits.dim() != 2 or logits.size(1) == 0:
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] == 0:
         raise RuntimeError("expected logits of shape (rows, vocab)")
-    rows, vocab = logits.shape
-    if vocab > 1 and logits.stride(1) != 1:
+    rows, vocab = shape
+    stride, column = logits.stride()
+    if vocab > 1 and column != 1:
         raise RuntimeError("logits must have unit column stride")
-    history = [None, 0, 0]
+    history = history_stride = most = prompts = counts = rep = freq = pres = 0
     if tokens is not None:
-        if tokens.dim() != 2 or tokens.size(0) != rows or tokens.dtype is not torch.int64 or tokens.device != device:
-            raise RuntimeError(f"tokens must be Long ({rows}, max_tokens) on {device}")
-        if tokens.size(1) > 1 and tokens.stride(1) != 1:
+        t_shape = tokens.shape
+        if len(t_shape) != 2 or t_shape[0] != rows or tokens.dtype is not torch.int64 or tokens.get_device() != index:
+            raise RuntimeError(f"tokens must be Long ({rows}, max_tokens) on cuda:{index}")
+        most = t_shape[1]
+        history_stride, column = tokens.stride()
+        if most > 1 and column != 1:
             raise RuntimeError("tokens must have unit column stride")
         if lengths is None:
             raise RuntimeError("tokens need lengths")
-        history = [tokens.data_ptr() if tokens.numel() else None, max(tokens.stride(0), tokens.size(1)), tokens.size(1)]
-    elif any(t is not None for t in (lengths, prompt_lengths, repetition, frequency, presence)):
+        if history_stride < most:
+            history_stride = most
+        prompts = _per_row(prompt_lengths, "prompt_lengths", torch.int32, index, rows)
+        counts = _per_row(lengths, "lengths", torch.int32, index, rows)
+        rep = _per_row(repetition, "repetition", torch.float32, index, rows)
+        freq = _per_row(frequency, "frequency", torch.float32, index, rows)
+        pres = _per_row(presence, "presence", torch.float32, index, rows)
+        if most:
+            history = tokens.data_ptr()
+        else:
+            prompts = counts = rep = freq = pres = 0
+    elif lengths is not None or prompt_lengths is not None or repetition is not None or frequency is not None or presence is not None:
         raise RuntimeError("lengths and penalties need tokens")
-    per_row = []
-    for t, name, dtype in ((prompt_lengths, "prompt_lengths", torch.int32), (lengths, "lengths", torch.int32),
-                           (repetition, "repetition", torch.float32), (frequency, "frequency", torch.float32),
-                           (presence, "presence", torch.float32)):  # fmt: skip
-        if t is None or history[0] is None:
-            per_row.append(None)
-            continue
-        if tuple(t.shape) != (rows,):
-            raise RuntimeError(f"{name} must have shape ({rows},)")
-        per_row.append(_tensor(t, name, dtype, device))
-    bias = [None, None, None, 0]
+    starts = ids = amounts = biases = 0
     if bias_starts is not None:
         if bias_ids is None or bias_values is None:
             raise RuntimeError("bias_starts needs bias_ids and bias_values")
-        if tuple(bias_starts.shape) != (rows + 1,) or bias_ids.dim() != 1 or bias_ids.shape != bias_values.shape:
+        b_shape = bias_ids.shape
+        if bias_starts.shape != (rows + 1,) or len(b_shape) != 1 or bias_values.shape != b_shape:
             raise RuntimeError(f"bias_starts must have shape ({rows + 1},), bias_ids and bias_values one length")
-        bias = [_tensor(bias_starts, "bias_starts", torch.int32, device), _tensor(bias_ids, "bias_ids", torch.int64, device),
-                _tensor(bias_values, "bias_values", torch.float32, device), bias_ids.numel()]  # fmt: skip
-        if bias[3] == 0:
-            bias = [None, None, None, 0]
+        starts = _tensor(bias_starts, "bias_starts", torch.int32, index)
+        ids = _tensor(bias_ids, "bias_ids", torch.int64, index)
+        amounts = _tensor(bias_values, "bias_values", torch.float32, index)
+        biases = b_shape[0]
+        if biases == 0:
+            starts = 0
     elif bias_ids is not None or bias_values is not None:
         raise RuntimeError("biases need bias_starts")
-    words = -(-vocab // 32)
-    mask_ptr, mask_stride = None, 0
+    mask_ptr = mask_stride = 0
     if mask is not None:
-        if tuple(mask.shape) != (rows, words) or mask.dtype is not torch.int32 or mask.device != device:
-            raise RuntimeError(f"mask must be Int ({rows}, {words}) on {device}")
-        if words > 1 and mask.stride(1) != 1:
+        words = -(-vocab // 32)
+        if mask.shape != (rows, words) or mask.dtype is not torch.int32 or mask.get_device() != index:
+            raise RuntimeError(f"mask must be Int ({rows}, {words}) on cuda:{index}")
+        mask_stride, column = mask.stride()
+        if words > 1 and column != 1:
             raise RuntimeError("mask must have unit column stride")
-        mask_ptr, mask_stride = mask.data_ptr(), max(mask.stride(0), words)
+        mask_ptr, mask_stride = mask.data_ptr(), mask_stride if mask_stride > words else words
     if out is None:
-        out = torch.empty((rows, vocab), dtype=torch.float32, device=device)
+        out = torch.empty_like(logits, dtype=torch.float32, memory_format=_CONTIGUOUS)
+        out_stride = vocab
     else:
-        if tuple(out.shape) != (rows, vocab) or out.dtype is not torch.float32 or out.device != device:
-            raise RuntimeError(f"out must be Float ({rows}, {vocab}) on {device}")
-        if (vocab > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < vocab):
+        if out.shape != shape or out.dtype is not torch.float32 or out.get_device() != index:
+            raise RuntimeError(f"out must be Float ({rows}, {vocab}) on cuda:{index}")
+        out_stride, column = out.stride()
+        if (vocab > 1 and column != 1) or (rows > 1 and out_stride < vocab):
             raise RuntimeError("out must have unit column stride and rows of their own")
         same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride() and out.dtype is logits.dtype
         inputs = [t for t in (tokens, bias_ids, bias_values, mask) if t is not None]
         if (not same and _overlaps(out, logits)) or any(_overlaps(out, t) for t in inputs):
             raise RuntimeError("out must be the logits themselves or share no memory with the inputs")
-    _call("pck_process_logits", device, logits.data_ptr(), code, rows, vocab, max(logits.stride(0), vocab), *history, *per_row,
-          *bias, mask_ptr, mask_stride, out.data_ptr(), max(out.stride(0), vocab))  # fmt: skip
+        if out_stride < vocab:
+            out_stride = vocab
+    _call("pck_process_logits", index, _lib.LOGITS.pack(
+        logits.data_ptr(), code, rows, vocab, stride if stride > vocab else vocab, history, history_stride, most, prompts, counts,
+        rep, freq, pres, starts, ids, amounts, biases, mask_ptr, mask_stride, out.data_ptr(), out_stride))  # fmt: skip
     return out
 
 

@@ -53,28 +53,48 @@ def test_the_library_rejects_bad_arguments() -> None:
     from pck.cuda import _lib
 
     lib = _lib.library()
+    call = lambda fn, layout, args: fn(layout.pack(*(a or 0 for a in args)), None)  # noqa: E731
     err = lambda: lib.pck_last_error().decode()  # noqa: E731
-    ok = [16, 4, 2, 1, 128, 16, 16, 0, 3, 256, 128, 256, 128, 16, None, None, None]
+    ok = [16, 4, 2, 1, 128, 16, 16, 0, 3, 256, 128, 256, 128, 16, None, None]
     for at, value, message in ((4, 96, "dim"), (2, 0, "kv_heads"), (3, 0, "page_tiles"), (7, 3, "dtype"), (5, None, "NULL"),
                                (13, None, "NULL"), (0, 8, "aligned"), (14, 16, "together")):  # fmt: skip
         args = list(ok)
         args[at] = value
-        assert lib.pck_kv4_append(*args) == 1 and message in err(), (at, err())
+        assert call(lib.pck_kv4_append, _lib.KV4_APPEND, args) == 1 and message in err(), (at, err())
     args = list(ok)
     args[8] = 0
-    assert lib.pck_kv4_append(*args) == 0  # nothing to write
-    ok = [16, 1, 2, 1, 8, 128, 1024, 1024, 128, 16, 4, 2, 1, 16, 4, 4, 16, 0.1, 0, 16, None, 0, None]
+    assert call(lib.pck_kv4_append, _lib.KV4_APPEND, args) == 0  # nothing to write
+    ok = [16, 1, 2, 1, 8, 128, 1024, 1024, 128, 16, 4, 2, 1, 16, 4, 4, 16, 0.1, 0, 16, None, 0]
     for at, value, message in ((5, 80, "dim"), (1, 0, "bfloat16"), (3, 0, "queries"), (4, 7, "multiple"), (12, 0, "page_tiles"),
                                (14, 3, "whole rows"), (18, -1, "window"), (17, 0.0, "scale"), (17, float("nan"), "scale"),
                                (0, None, "NULL"), (13, None, "NULL"), (9, 8, "aligned")):  # fmt: skip
         args = list(ok)
         args[at] = value
-        assert lib.pck_kv4_attention(*args) == 1 and message in err(), (at, err())
+        assert call(lib.pck_kv4_attention, _lib.KV4_ATTENTION, args) == 1 and message in err(), (at, err())
     args = list(ok)
     args[2] = 0
-    assert lib.pck_kv4_attention(*args) == 0
+    assert call(lib.pck_kv4_attention, _lib.KV4_ATTENTION, args) == 0
     assert lib.pck_kv4_attention_scratch(1, 0, 8, 8, 128, 64) == -1
     assert isinstance(ctypes.c_int64(lib.pck_kv4_attention_scratch(1, 1, 8, 8, 128, 64)).value, int)
+
+
+def test_packed_descriptors_have_the_headers_fields() -> None:
+    """Every field of a serving descriptor is 8 bytes, and the binding packs as many, doubles where they are."""
+    import re
+    from pathlib import Path
+
+    from pck.cuda import _lib
+
+    text = (Path(__file__).resolve().parents[1] / "include" / "pck_b200.h").read_text()
+    for name, layout in (("kv4_append", _lib.KV4_APPEND), ("kv4_attention", _lib.KV4_ATTENTION), ("lora", _lib.LORA),
+                         ("logits", _lib.LOGITS)):  # fmt: skip
+        body = re.search(rf"typedef struct pck_{name}_desc {{(.*?)}}", text, re.S).group(1)
+        kinds = ""
+        for line in filter(None, (x.strip() for x in body.split(";"))):
+            assert "*" in line or line.startswith(("int64_t", "double")), line
+            kinds += ("d" if line.startswith("double") else "q") * len(line.split(","))
+        want = "".join(k * int(n or 1) for n, k in re.findall(r"(\d*)([qd])", layout.format))
+        assert kinds == want and layout.size == 8 * len(kinds), name
 
 
 def test_cpu_tensors_and_bad_sizes_are_refused() -> None:

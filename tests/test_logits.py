@@ -49,16 +49,17 @@ def test_the_library_rejects_bad_arguments() -> None:
     from pck.cuda import _lib
 
     lib = _lib.library()
-    ok = [16, 0, 2, 100, 100, 16, 8, 8, None, 16, 16, None, None, 16, 16, 16, 4, 16, 4, 16, 100, None]
+    call = lambda fn, layout, args: fn(layout.pack(*(a or 0 for a in args)), None)  # noqa: E731
+    ok = [16, 0, 2, 100, 100, 16, 8, 8, None, 16, 16, None, None, 16, 16, 16, 4, 16, 4, 16, 100]
     for at, value, message in ((1, 3, "dtype"), (3, 0, "vocab"), (4, 99, "strides"), (20, 99, "strides"), (9, None, "lengths"),
                                (6, 7, "whole rows"), (5, None, "need a history"), (14, None, "ids and values"),
                                (18, 3, "words"), (0, None, "NULL"), (19, None, "NULL")):  # fmt: skip
         args = list(ok)
         args[at] = value
-        assert lib.pck_process_logits(*args) == 1 and message in lib.pck_last_error().decode(), at
+        assert call(lib.pck_process_logits, _lib.LOGITS, args) == 1 and message in lib.pck_last_error().decode(), at
     args = list(ok)
     args[2] = 0
-    assert lib.pck_process_logits(*args) == 0
+    assert call(lib.pck_process_logits, _lib.LOGITS, args) == 0
 
 
 class TestLogits:

@@ -37,17 +37,18 @@ def test_the_library_rejects_bad_arguments() -> None:
     from pck.cuda import _lib
 
     lib = _lib.library()
-    ok = [16, 1, 3, 64, 64, 16, 32, 32, 16, 16, 2, 8, 16, None, None, 16, 32, None]
+    call = lambda fn, layout, args: fn(layout.pack(*(a or 0 for a in args)), None)  # noqa: E731
+    ok = [16, 1, 3, 64, 64, 16, 32, 32, 16, 16, 2, 8, 16, None, None, 16, 32]
     for at, value, message in ((1, 0, "bfloat16"), (3, 0, "n >= 1"), (4, 63, "strides"), (7, 31, "strides"), (16, 31, "strides"),
                                (11, 0, "rank"), (11, 257, "rank"), (10, -1, "number"), (0, None, "NULL"), (8, None, "NULL"),
                                (15, None, "NULL")):  # fmt: skip
         args = list(ok)
         args[at] = value
-        assert lib.pck_lora_add(*args) == 1 and message in lib.pck_last_error().decode(), at
+        assert call(lib.pck_lora_add, _lib.LORA, args) == 1 and message in lib.pck_last_error().decode(), at
     for at in (2, 6):
         args = list(ok)
         args[at] = 0
-        assert lib.pck_lora_add(*args) == 0
+        assert call(lib.pck_lora_add, _lib.LORA, args) == 0
 
 
 class TestLora:
