@@ -435,7 +435,7 @@ int pck_peer_all_gather(const pck_peer_gather* gather, void* stream);
  * < 2^-126), code = clamp(rint((x - zero) * inv), 0, 15), each step one binary32 operation. A
  * group whose scale or zero is not finite (it held a NaN or an infinity) is stored as NaN (0x7fc0, codes 0). k_values
  * and v_values (both or neither) get the values that the codes stand for, (tokens, kv_heads, dim)
- * of `dtype`, whatever the slot.
+ * of `dtype`, 16-byte aligned, whatever the slot.
  */
 typedef struct pck_kv4_append_desc {
   void* cache;

@@ -5,8 +5,11 @@
 // are the same wherever the same formula is evaluated. The division by 15 is a product with the
 // binary32 nearest 1/15 and the division by the scale one with its rounded reciprocal.
 //
-// One warp per (token, head, keys or values): a lane holds two neighbouring channels of each group,
-// which is one byte of codes. Bound by memory: the inputs are read once, the codes written once.
+// A warp takes 8 tokens of one head's keys or values, a lane a quarter of each group's channels of one
+// token, so that a lane's key codes are one 16-byte piece of the tile. Value codes of two neighbouring
+// tokens share 32-bit words: where the next token's slot is the next one, the two lanes exchange halves
+// and write 16 bytes each; single 16-bit pieces remain for decode steps and the ends of prompts. Bound
+// by memory: the inputs are read once, the codes written once, in whole 32-byte sectors.
 #include "kv4_layout.cuh"
 #include "serving_common.cuh"
 
@@ -24,78 +27,191 @@ struct AppendArgs {
   int64_t total_slots;
   int32_t heads;
   int32_t page_tiles;
+  int32_t vector;  // rows of k and v are 16-byte aligned
 };
 
+// 16 channels of a row as binary32.
+template <typename T>
+__device__ __forceinline__ void load16(float (&v)[16], const T* from, bool vector) {
+  if (vector) {
+    uint4 w[sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+    const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = to_float(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = to_float(from[i]);
+  }
+}
+
 template <typename T, int kDim>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
-  const int lane = threadIdx.x % kWarp;
+__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int kPlanes = kDim > 128 ? kDim / 128 : 1, kWidth = kv4_plane_groups(kDim);
+  const int lane = threadIdx.x % kWarp, row = lane / 4, quarter = lane % 4;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x / kWarp) + threadIdx.x / kWarp;
-  if (item >= a.tokens * a.heads * 2) return;
-  const int side = static_cast<int>(item % 2);
-  const int head = static_cast<int>(item / 2 % a.heads);
-  const int64_t token = item / 2 / a.heads;
-  int64_t slot = a.slots[token];
+  wait_for_producers();
+  allow_dependents();
+  const int64_t blocks = (a.tokens + 7) / 8;
+  if (item >= blocks * a.heads * 2 * kPlanes) return;
+  const int plane = static_cast<int>(item % kPlanes);
+  const int side = static_cast<int>(item / kPlanes % 2);
+  const int head = static_cast<int>(item / kPlanes / 2 % a.heads);
+  const int64_t token = item / kPlanes / 2 / a.heads * 8 + row;
+  const bool there = token < a.tokens;
+  int64_t slot = there ? a.slots[token] : -1;
   if (slot >= a.total_slots) {
-    if (lane == 0) report(kDevIndex);
+    if (quarter == 0) report(kDevIndex);
     slot = -1;
   }
-  uint8_t* tile = nullptr;
+  // The lane that holds the other token of this one's pair of slots, if it is in this warp.
+  const int other = slot % 2 == 0 ? lane + 4 : lane - 4;
+  const int64_t other_slot = __shfl_sync(kFullMask, slot, other & 31);
+  const bool paired = slot >= 0 && other >= 0 && other < kWarp && other_slot == (slot ^ 1);
   const int at = static_cast<int>(slot % kKv4Tile);
+  uint8_t* tile = nullptr;
   if (slot >= 0) {
     const int64_t page_tokens = static_cast<int64_t>(a.page_tiles) * kKv4Tile;
     const int64_t page = slot / page_tokens, in_page = slot % page_tokens;
     tile = a.cache + ((page * a.heads + head) * a.page_tiles + in_page / kKv4Tile) * kv4_tile_bytes(kDim);
   }
   const T* x = static_cast<const T*>(a.x[side]) + token * a.token_stride[side] + head * a.head_stride[side];
-  T* values = static_cast<T*>(a.values[side]);
+  float v[kWidth][16];
+  if (there) {
 #pragma unroll
-  for (int g = 0; g < kv4_groups(kDim); ++g) {
-    const int c = g * kKv4Group + 2 * lane;
-    const float v0 = to_float(x[c]), v1 = to_float(x[c + 1]);
-    bool nan = v0 != v0 || v1 != v1;
-    float low = fminf(v0, v1), high = fmaxf(v0, v1);
+    for (int g = 0; g < kWidth; ++g) load16(v[g], x + (plane * kWidth + g) * kKv4Group + 16 * quarter, a.vector);
+  } else {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
+    for (int g = 0; g < kWidth; ++g) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[g][i] = 0.0f;
+    }
+  }
+  uint32_t codes[kWidth][2], pairs[kWidth];
+#pragma unroll
+  for (int g = 0; g < kWidth; ++g) {
+    bool nan = false;
+    float low = v[g][0], high = v[g][0];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      nan = nan || v[g][i] != v[g][i];
+      low = fminf(low, v[g][i]);
+      high = fmaxf(high, v[g][i]);
+    }
+    int any = nan;
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
       low = fminf(low, __shfl_xor_sync(kFullMask, low, o));
       high = fmaxf(high, __shfl_xor_sync(kFullMask, high, o));
+      any |= __shfl_xor_sync(kFullMask, any, o);
     }
-    nan = __any_sync(kFullMask, nan);
-    __nv_bfloat16 scale_b = __float2bfloat16_rn((high - low) * (1.0f / 15.0f));
-    __nv_bfloat16 zero_b = __float2bfloat16_rn(low);
+    const __nv_bfloat16 scale_b = __float2bfloat16_rn((high - low) * (1.0f / 15.0f)), zero_b = __float2bfloat16_rn(low);
     float scale = __bfloat162float(scale_b), zero = __bfloat162float(zero_b);
-    if (nan || !isfinite(scale) || !isfinite(zero)) {  // nothing finite stands for such a group
+    pairs[g] = __bfloat16_as_ushort(scale_b) | static_cast<uint32_t>(__bfloat16_as_ushort(zero_b)) << 16;
+    if (any || !isfinite(scale) || !isfinite(zero)) {  // nothing finite stands for such a group
       scale = zero = __int_as_float(0x7fc00000);
-      scale_b = zero_b = __ushort_as_bfloat16(0x7fc0);
+      pairs[g] = 0x7fc07fc0u;
     }
     const float inv = scale >= 0x1p-126f ? 1.0f / scale : 0.0f;
-    const float q0 = fminf(fmaxf(rintf((v0 - zero) * inv), 0.0f), 15.0f);  // NaN gives 0
-    const float q1 = fminf(fmaxf(rintf((v1 - zero) * inv), 0.0f), 15.0f);
-    if (tile) {
-      const uint8_t byte = static_cast<uint8_t>(static_cast<int>(q0) | static_cast<int>(q1) << 4);
-      tile[side ? kv4_value_byte(kDim, at, c) : kv4_key_byte(kDim, at, c)] = byte;
-      if (lane == 0) {
-        const uint32_t pair = __bfloat16_as_ushort(scale_b) | static_cast<uint32_t>(__bfloat16_as_ushort(zero_b)) << 16;
-        *reinterpret_cast<uint32_t*>(tile + (side ? kv4_value_scale(kDim, at, g) : kv4_key_scale(kDim, at, g))) = pair;
+    codes[g][0] = codes[g][1] = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float q = fminf(fmaxf(rintf((v[g][i] - zero) * inv), 0.0f), 15.0f);  // NaN gives 0
+      codes[g][i / 8] |= static_cast<uint32_t>(q) << (4 * (i % 8));
+      v[g][i] = q * scale + zero;
+    }
+  }
+  // The exchange: the token of the even slot writes the pair's first 8 channels of its quarter, the
+  // other the second.
+  const int mine = slot & 1;
+  uint32_t theirs[kWidth];
+#pragma unroll
+  for (int g = 0; g < kWidth; ++g) theirs[g] = __shfl_sync(kFullMask, mine ? codes[g][0] : codes[g][1], other & 31);
+  if (tile) {
+    uint8_t* const plane_at = tile + plane * 512 * kWidth;
+    if (side == 0) {
+      uint8_t* to = plane_at + at * 32 * kWidth + quarter * 8 * kWidth;
+      if constexpr (kWidth == 2) {
+        *reinterpret_cast<uint4*>(to) = make_uint4(codes[0][0], codes[0][1], codes[1][0], codes[1][1]);
+      } else {
+        *reinterpret_cast<uint2*>(to) = make_uint2(codes[0][0], codes[0][1]);
+      }
+    } else {
+      uint8_t* to = plane_at + 9 * kDim + at / 8 * 256 * kWidth + at % 8 / 2 * 8 * kWidth;
+      if (paired) {
+        uint32_t w[2 * kWidth];
+#pragma unroll
+        for (int g = 0; g < kWidth; ++g) {
+          const uint32_t own = mine ? codes[g][1] : codes[g][0];
+          const uint32_t even = mine ? theirs[g] : own, odd = mine ? own : theirs[g];
+          w[2 * g] = __byte_perm(even, odd, 0x5410);
+          w[2 * g + 1] = __byte_perm(even, odd, 0x7632);
+        }
+        to += (2 * quarter + mine) * 32 * kWidth;
+        if constexpr (kWidth == 2) {
+          *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+          *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        }
+      } else {
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+#pragma unroll
+          for (int g = 0; g < kWidth; ++g) {
+            uint16_t* piece = reinterpret_cast<uint16_t*>(to + (2 * quarter + o) * 32 * kWidth + g * 8) + mine;
+            piece[0] = static_cast<uint16_t>(codes[g][o]);
+            piece[2] = static_cast<uint16_t>(codes[g][o] >> 16);
+          }
+        }
       }
     }
-    if (values) {
-      T* to = values + (token * a.heads + head) * kDim + c;
-      to[0] = from_float<T>(q0 * scale + zero);
-      to[1] = from_float<T>(q1 * scale + zero);
+    if (quarter == 0) {
+      uint32_t* to = reinterpret_cast<uint32_t*>(tile + (side ? kv4_value_scale(kDim, at, 0) : kv4_key_scale(kDim, at, 0)));
+#pragma unroll
+      for (int g = 0; g < kWidth; ++g) to[plane * kWidth + g] = pairs[g];
+    }
+  }
+  T* values = static_cast<T*>(a.values[side]);
+  if (values && there) {
+#pragma unroll
+    for (int g = 0; g < kWidth; ++g) {
+      T* to = values + (token * a.heads + head) * kDim + (plane * kWidth + g) * kKv4Group + 16 * quarter;
+      T e[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) e[i] = from_float<T>(v[g][i]);
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(e)[i];
     }
   }
 }
 
-template <typename T>
-cudaError_t launch_append(const AppendArgs& a, int dim, cudaStream_t stream) {
-  constexpr int kWarps = 8;
-  const int64_t blocks = (a.tokens * a.heads * 2 + kWarps - 1) / kWarps;
+template <typename T, int kDim>
+cudaError_t launch_dim(const AppendArgs& a, cudaStream_t stream) {
+  constexpr int kPlanes = kDim > 128 ? kDim / 128 : 1;
+  const int64_t warps = (a.tokens + 7) / 8 * a.heads * 2 * kPlanes;
+  // Few tokens: a warp a CTA, on as many SMs as there are.
+  const int per = warps >= 2048 ? 8 : 1;
+  const int64_t blocks = (warps + per - 1) / per;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const unsigned grid = static_cast<unsigned>(blocks);
-  if (dim == 64) append_kernel<T, 64><<<grid, kWarps * kWarp, 0, stream>>>(a);
-  if (dim == 128) append_kernel<T, 128><<<grid, kWarps * kWarp, 0, stream>>>(a);
-  if (dim == 256) append_kernel<T, 256><<<grid, kWarps * kWarp, 0, stream>>>(a);
-  return cudaGetLastError();
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(static_cast<unsigned>(per * kWarp));
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, append_kernel<T, kDim>, a);
+}
+
+template <typename T>
+cudaError_t launch_append(AppendArgs a, int64_t dim, cudaStream_t stream) {
+  const int64_t e = 16 / sizeof(T);
+  a.vector = aligned_to(a.x[0], 16) && aligned_to(a.x[1], 16) && a.token_stride[0] % e == 0 && a.head_stride[0] % e == 0 &&
+             a.token_stride[1] % e == 0 && a.head_stride[1] % e == 0;
+  return dim == 64 ? launch_dim<T, 64>(a, stream) : dim == 128 ? launch_dim<T, 128>(a, stream) : launch_dim<T, 256>(a, stream);
 }
 
 }  // namespace
@@ -118,7 +234,9 @@ extern "C" int pck_kv4_append(const pck_kv4_append_desc* desc, void* stream) {
   if (tokens == 0) return PCK_OK;
   if ((pages > 0 && !cache) || !k || !v || !slots) return report_error(PCK_ERR_ARGUMENT, "append: NULL cache, k, v or slots");
   if (!k_values != !v_values) return report_error(PCK_ERR_ARGUMENT, "append: k_values and v_values go together");
-  if (!aligned_to(cache, 16)) return report_error(PCK_ERR_ARGUMENT, "append: the cache must be 16-byte aligned");
+  if (!aligned_to(cache, 16) || !aligned_to(k_values, 16) || !aligned_to(v_values, 16)) {
+    return report_error(PCK_ERR_ARGUMENT, "append: the cache and the values must be 16-byte aligned");
+  }
   AppendArgs a{};
   a.cache = static_cast<uint8_t*>(cache);
   a.x[0] = k;
@@ -134,10 +252,9 @@ extern "C" int pck_kv4_append(const pck_kv4_append_desc* desc, void* stream) {
   a.total_slots = pages * page_tiles * kKv4Tile;
   a.heads = static_cast<int32_t>(kv_heads);
   a.page_tiles = static_cast<int32_t>(page_tiles);
-  const int d = static_cast<int>(dim);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = dtype == PCK_LOGITS_F32    ? launch_append<float>(a, d, s)
-                          : dtype == PCK_LOGITS_BF16 ? launch_append<__nv_bfloat16>(a, d, s)
-                                                     : launch_append<__half>(a, d, s);
+  const cudaError_t err = dtype == PCK_LOGITS_F32    ? launch_append<float>(a, dim, s)
+                          : dtype == PCK_LOGITS_BF16 ? launch_append<__nv_bfloat16>(a, dim, s)
+                                                     : launch_append<__half>(a, dim, s);
   return err == cudaSuccess ? PCK_OK : report_cuda("append kernel", err);
 }
