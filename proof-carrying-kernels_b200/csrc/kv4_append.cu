@@ -30,37 +30,60 @@ struct AppendArgs {
   int32_t vector;  // rows of k and v are 16-byte aligned
 };
 
-// 16 channels of a row as binary32.
-template <typename T>
-__device__ __forceinline__ void load16(float (&v)[16], const T* from, bool vector) {
-  if (vector) {
-    uint4 w[sizeof(T)];
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
-    const T* e = reinterpret_cast<const T*>(w);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = to_float(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = to_float(from[i]);
-  }
+// Smaller and larger of two, NaN if either is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 16 channels of a row, as they lie.
+template <typename T>
+struct Raw16 {
+  uint4 w[sizeof(T)];
+  __device__ __forceinline__ void load(const T* from, bool vector) {
+    if (vector) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+    } else {
+      T e[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) e[i] = from[i];
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return to_float(reinterpret_cast<const T*>(w)[i]); }
+};
 
 template <typename T, int kDim>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int kPlanes = kDim > 128 ? kDim / 128 : 1, kWidth = kv4_plane_groups(kDim);
   const int lane = threadIdx.x % kWarp, row = lane / 4, quarter = lane % 4;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (blockDim.x / kWarp) + threadIdx.x / kWarp;
+  const int plane = static_cast<int>(blockIdx.y) % kPlanes, side = static_cast<int>(blockIdx.y) / kPlanes % 2;
+  const int head = static_cast<int>(blockIdx.y) / kPlanes / 2;
+  const int64_t token = (static_cast<int64_t>(blockIdx.x) * (blockDim.x / kWarp) + threadIdx.x / kWarp) * 8 + row;
   wait_for_producers();
   allow_dependents();
-  const int64_t blocks = (a.tokens + 7) / 8;
-  if (item >= blocks * a.heads * 2 * kPlanes) return;
-  const int plane = static_cast<int>(item % kPlanes);
-  const int side = static_cast<int>(item / kPlanes % 2);
-  const int head = static_cast<int>(item / kPlanes / 2 % a.heads);
-  const int64_t token = item / kPlanes / 2 / a.heads * 8 + row;
   const bool there = token < a.tokens;
   int64_t slot = there ? a.slots[token] : -1;
+  // The inputs are on their way before anything waits for the slot.
+  const T* x = static_cast<const T*>(a.x[side]) + token * a.token_stride[side] + head * a.head_stride[side];
+  Raw16<T> raw[kWidth];
+#pragma unroll
+  for (int g = 0; g < kWidth; ++g) {
+    if (there) {
+      raw[g].load(x + (plane * kWidth + g) * kKv4Group + 16 * quarter, a.vector);
+    } else {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) raw[g].w[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
   if (slot >= a.total_slots) {
     if (quarter == 0) report(kDevIndex);
     slot = -1;
@@ -72,54 +95,49 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
   const int at = static_cast<int>(slot % kKv4Tile);
   uint8_t* tile = nullptr;
   if (slot >= 0) {
-    const int64_t page_tokens = static_cast<int64_t>(a.page_tiles) * kKv4Tile;
-    const int64_t page = slot / page_tokens, in_page = slot % page_tokens;
-    tile = a.cache + ((page * a.heads + head) * a.page_tiles + in_page / kKv4Tile) * kv4_tile_bytes(kDim);
+    // (A 64-bit division takes several times a 32-bit one; caches of 2^32 slots are rare.)
+    const int64_t index = slot / kKv4Tile;
+    const int64_t page = a.total_slots < int64_t{1} << 32
+                             ? static_cast<uint32_t>(index) / static_cast<uint32_t>(a.page_tiles) : index / a.page_tiles;
+    tile = a.cache + ((page * a.heads + head) * a.page_tiles + (index - page * a.page_tiles)) * kv4_tile_bytes(kDim);
   }
-  const T* x = static_cast<const T*>(a.x[side]) + token * a.token_stride[side] + head * a.head_stride[side];
   float v[kWidth][16];
-  if (there) {
 #pragma unroll
-    for (int g = 0; g < kWidth; ++g) load16(v[g], x + (plane * kWidth + g) * kKv4Group + 16 * quarter, a.vector);
-  } else {
+  for (int g = 0; g < kWidth; ++g) {
 #pragma unroll
-    for (int g = 0; g < kWidth; ++g) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[g][i] = 0.0f;
-    }
+    for (int i = 0; i < 16; ++i) v[g][i] = raw[g].at(i);
   }
   uint32_t codes[kWidth][2], pairs[kWidth];
 #pragma unroll
   for (int g = 0; g < kWidth; ++g) {
-    bool nan = false;
     float low = v[g][0], high = v[g][0];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      nan = nan || v[g][i] != v[g][i];
-      low = fminf(low, v[g][i]);
-      high = fmaxf(high, v[g][i]);
+    for (int i = 1; i < 16; ++i) {
+      low = min_nan(low, v[g][i]);
+      high = max_nan(high, v[g][i]);
     }
-    int any = nan;
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-      low = fminf(low, __shfl_xor_sync(kFullMask, low, o));
-      high = fmaxf(high, __shfl_xor_sync(kFullMask, high, o));
-      any |= __shfl_xor_sync(kFullMask, any, o);
+      low = min_nan(low, __shfl_xor_sync(kFullMask, low, o));
+      high = max_nan(high, __shfl_xor_sync(kFullMask, high, o));
     }
     const __nv_bfloat16 scale_b = __float2bfloat16_rn((high - low) * (1.0f / 15.0f)), zero_b = __float2bfloat16_rn(low);
     float scale = __bfloat162float(scale_b), zero = __bfloat162float(zero_b);
     pairs[g] = __bfloat16_as_ushort(scale_b) | static_cast<uint32_t>(__bfloat16_as_ushort(zero_b)) << 16;
-    if (any || !isfinite(scale) || !isfinite(zero)) {  // nothing finite stands for such a group
+    if (!isfinite(scale) || !isfinite(zero)) {  // nothing finite stands for such a group
       scale = zero = __int_as_float(0x7fc00000);
       pairs[g] = 0x7fc07fc0u;
     }
     const float inv = scale >= 0x1p-126f ? 1.0f / scale : 0.0f;
-    codes[g][0] = codes[g][1] = 0;
+    // rint of a number in [0, 15] by a sum with 1.5 2^23, which leaves it in the low bits (the codes are
+    // added up with the rest of that number's bits, taken off at once below). q * scale is exact, so the
+    // value's one rounding is that of the sum.
+    codes[g][0] = codes[g][1] = 0u - 0x4b400000u * 0x11111111u;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float q = fminf(fmaxf(rintf((v[g][i] - zero) * inv), 0.0f), 15.0f);  // NaN gives 0
-      codes[g][i / 8] |= static_cast<uint32_t>(q) << (4 * (i % 8));
-      v[g][i] = q * scale + zero;
+      const float y = fminf(fmaxf((v[g][i] - zero) * inv, 0.0f), 15.0f) + 12582912.0f;  // NaN gives 0
+      codes[g][i / 8] += __float_as_uint(y) << (4 * (i % 8));
+      v[g][i] = fmaf(y - 12582912.0f, scale, zero);
     }
   }
   // The exchange: the token of the even slot writes the pair's first 8 channels of its quarter, the
@@ -189,16 +207,16 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 template <typename T, int kDim>
 cudaError_t launch_dim(const AppendArgs& a, cudaStream_t stream) {
   constexpr int kPlanes = kDim > 128 ? kDim / 128 : 1;
-  const int64_t warps = (a.tokens + 7) / 8 * a.heads * 2 * kPlanes;
+  const int64_t warps = (a.tokens + 7) / 8, sides = static_cast<int64_t>(a.heads) * 2 * kPlanes;
   // Few tokens: a warp a CTA, on as many SMs as there are.
-  const int per = warps >= 2048 ? 8 : 1;
+  const int per = warps * sides >= 2048 ? 8 : 1;
   const int64_t blocks = (warps + per - 1) / per;
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (blocks > 0x7fffffffLL || sides > 0xffff) return cudaErrorInvalidValue;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(sides));
   config.blockDim = dim3(static_cast<unsigned>(per * kWarp));
   config.stream = stream;
   config.attrs = &attr;
@@ -225,8 +243,8 @@ extern "C" int pck_kv4_append(const pck_kv4_append_desc* desc, void* stream) {
   if (!desc) return report_error(PCK_ERR_ARGUMENT, "append: NULL descriptor");
   const auto& [cache, pages, kv_heads, page_tiles, dim, k, v, dtype, tokens, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, k_values, v_values] = *desc;
   if (dim != 64 && dim != 128 && dim != 256) return report_error(PCK_ERR_ARGUMENT, "append: dim must be 64, 128 or 256");
-  if (pages < 0 || kv_heads < 1 || kv_heads > 0x7fffffff || page_tiles < 1 || page_tiles > 0x7fffffff || tokens < 0) {
-    return report_error(PCK_ERR_ARGUMENT, "append: need pages >= 0, kv_heads >= 1, page_tiles >= 1 and tokens >= 0");
+  if (pages < 0 || kv_heads < 1 || kv_heads > 0x3fff || page_tiles < 1 || page_tiles > 0x7fffffff || tokens < 0) {
+    return report_error(PCK_ERR_ARGUMENT, "append: need pages >= 0, kv_heads in [1, 16383], page_tiles >= 1 and tokens >= 0");
   }
   if (dtype != PCK_LOGITS_F32 && dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) {
     return report_error(PCK_ERR_ARGUMENT, "append: unknown dtype");
