@@ -1,26 +1,30 @@
 // pck_process_logits: penalties for repeated tokens, biases and grammar masks on a batch of logits,
 // written as the binary32 logits that the sampler and the membership check take.
 //
-// Bound by memory: the logits are read once and written once. A CTA takes a slice of a row's vocabulary
-// and asks for all of it, in registers, before it looks at the history. What the history holds of the
-// slice is counted in shared memory, a word for each token (integer atomics: the counts do not depend on
-// their order). Up to eight CTAs of a row form a cluster that reads the history once, each its share, and
-// counts into one another's shared memory: without it every slice would read the whole history, half
-// as much again as the logits for 64 rows of 128,256 with 3,000 tokens each. A second word for each
-// token holds the last bias that names it. What decides the time beside the bytes is the chain of
-// dependent reads (lengths, ids, counts), so each is asked for as early as it can be. Each step is a
-// separate binary32 operation, so the result is the formula's wherever it is evaluated.
-#include <cooperative_groups.h>
-
+// Bound by memory: the logits are read once and written once. Two kernels, since few tokens of a row are
+// in its history or its biases and what they need is a chain of dependent reads:
+//   - the pass writes every logit, or -inf by the mask, at the memory's rate, and looks at nothing else;
+//   - the marks, a programmatic dependent that counts while the pass runs: a CTA takes 16,384 tokens of
+//     a row's vocabulary, reads the row's history, and keeps a word of counts for each of its tokens in
+//     shared memory (integer atomics: their order does not matter) and a list of those that it met. Then
+//     it waits for the pass and computes the listed tokens' logits; biases are added after that, the last
+//     entry of a token found by the largest entry number in the token's word.
+//   (One kernel that did both held its registers and its memory requests through that chain: 31 us for 64
+//   rows of 128,256, where the bytes take 10. A hash table of a row's tokens, a CTA a row, took as long:
+//   text repeats its words, and their counts wait for one another.)
+// In place the marks come first and the pass, which then only writes the mask's -inf, second. Each step is
+// a separate binary32 operation, so the result is the formula's wherever it is evaluated.
 #include "serving_common.cuh"
 
 namespace pck {
 namespace {
 
-namespace cg = cooperative_groups;
-
-constexpr int kLogitsThreads = 512;
-constexpr int kLogitsWarps = kLogitsThreads / kWarp;
+constexpr int kPassThreads = 256;
+constexpr int kPassPer = 16;                          // tokens of a thread
+constexpr int kPassChunk = kPassThreads * kPassPer;   // tokens of a CTA's step
+constexpr int kPassCtas = 32;                         // of an SM at most; then a CTA takes several steps
+constexpr int kMarkThreads = 512;
+constexpr int kMarkSlice = 16384;                     // tokens of a marking CTA
 constexpr uint32_t kInPrompt = 0x80000000u;
 
 struct LogitsArgs {
@@ -43,148 +47,168 @@ struct LogitsArgs {
   int64_t mask_stride;
   float* out;
   int64_t out_stride;
-  int32_t clusters;  // of a row
+  int64_t rows;
+  int32_t in_place;
 };
 
-// kPer: tokens of a thread; token j of thread t is j * kLogitsThreads + t of the slice, so a warp meets
-// one word of the mask.
-template <typename T, int kPer>
-__global__ void __launch_bounds__(kLogitsThreads, 3) logits_kernel(const __grid_constant__ LogitsArgs a) {
-  constexpr int kSlice = kPer * kLogitsThreads;
-  extern __shared__ uint32_t counts[];     // how often the token was put out; kInPrompt: in the prompt
-  uint32_t* const bias = counts + kSlice;  // 1 + the last of the row's biases that names the token
-  cg::cluster_group cluster = cg::this_cluster();
-  const int cta = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
+// Every logit as binary32, or -inf where the mask says so (in place: only those).
+template <typename T>
+__global__ void __launch_bounds__(kPassThreads) pass_kernel(const __grid_constant__ LogitsArgs a) {
   const int tid = threadIdx.x, lane = tid % kWarp, warp = tid / kWarp;
-  const int64_t row = blockIdx.x / ctas / a.clusters;
-  const int64_t first = static_cast<int64_t>(blockIdx.x / ctas % a.clusters) * ctas * kSlice;  // of the cluster
-  const int64_t base = first + static_cast<int64_t>(cta) * kSlice;
-  const int size = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(kSlice), a.vocab - base)));
   wait_for_producers();
   allow_dependents();
+  const int64_t chunks = (a.vocab + kPassChunk - 1) / kPassChunk;
+  for (int64_t c = blockIdx.x; c < chunks * a.rows; c += gridDim.x) {
+    const int64_t row = c / chunks, base = c % chunks * kPassChunk;
+    const int size = static_cast<int>(min(static_cast<int64_t>(kPassChunk), a.vocab - base));
+    // Token j of thread t is j * kPassThreads + t, so a warp meets one word of the mask, which lane j holds.
+    const T* in = static_cast<const T*>(a.logits) + row * a.row_stride + base;
+    T raw[kPassPer];
+    if (!a.in_place) {
+#pragma unroll
+      for (int j = 0; j < kPassPer; ++j) {
+        if (j * kPassThreads + tid < size) raw[j] = in[j * kPassThreads + tid];
+      }
+    }
+    uint32_t words = 0xffffffffu;
+    const int first = (lane * (kPassThreads / kWarp) + warp) * kWarp;
+    if (a.mask && lane < kPassPer && first < size) {
+      words = static_cast<uint32_t>(a.mask[row * a.mask_stride + (base + first) / 32]);
+    }
+    float* out = a.out + row * a.out_stride + base;
+#pragma unroll
+    for (int j = 0; j < kPassPer; ++j) {
+      const int i = j * kPassThreads + tid;
+      const bool shown = __shfl_sync(kFullMask, words, j) >> lane & 1u;
+      if (i < size && !(a.in_place && shown)) out[i] = shown ? to_float(raw[j]) : -INFINITY;
+    }
+  }
+}
+
+// The logits of the tokens in a row's history or biases.
+template <typename T>
+__global__ void __launch_bounds__(kMarkThreads) mark_kernel(const __grid_constant__ LogitsArgs a) {
+  extern __shared__ uint32_t counts[];  // times put out, kInPrompt
+  uint16_t* const listed = reinterpret_cast<uint16_t*>(counts + kMarkSlice);  // tokens with a count
+  __shared__ uint32_t met;
+  const int tid = threadIdx.x;
+  const int64_t slices = (a.vocab + kMarkSlice - 1) / kMarkSlice;
+  const int64_t row = blockIdx.x / slices, base = blockIdx.x % slices * kMarkSlice;
+  const int64_t size = min(static_cast<int64_t>(kMarkSlice), a.vocab - base);
+  if (a.in_place) wait_for_producers();  // else this call's pass comes before, and it has waited
+  allow_dependents();
   int64_t length = 0, prompt = 0, bias0 = 0, bias1 = 0;
+  float rep = 1.0f, freq = 0.0f, pres = 0.0f;
   if (a.tokens) {
     length = min(static_cast<int64_t>(a.lengths[row]), a.max_tokens);
     if (a.prompt_lengths) prompt = a.prompt_lengths[row];
+    if (a.repetition) rep = a.repetition[row];
+    if (a.frequency) freq = a.frequency[row];
+    if (a.presence) pres = a.presence[row];
   }
   if (a.bias_starts) {
     bias0 = max(static_cast<int64_t>(a.bias_starts[row]), int64_t{0});
     bias1 = min(static_cast<int64_t>(a.bias_starts[row + 1]), a.biases);
   }
+  if (a.tokens) {
+#pragma unroll
+    for (int j = 0; j < kMarkSlice / 4 / kMarkThreads; ++j) {
+      reinterpret_cast<uint4*>(counts)[j * kMarkThreads + tid] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  if (tid == 0) met = 0;
+  constexpr int kAhead = 8;
+  const int64_t* const tokens = a.tokens + row * a.token_stride;
+  int64_t id[kAhead];
+  auto load = [&](int64_t i) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) id[u] = i + u * kMarkThreads < length ? tokens[i + u * kMarkThreads] : -1;
+  };
+  load(tid);
+  int64_t bias_id = bias0 + tid < bias1 ? a.bias_ids[bias0 + tid] : -1;
+  __syncthreads();
+  for (int64_t i = tid; i < length; i += kAhead * kMarkThreads) {
+    if (i > tid) load(i);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t at = id[u] - base;
+      if (id[u] < 0 || at < 0 || at >= size) continue;
+      const uint32_t before = i + u * kMarkThreads < prompt ? atomicOr(&counts[at], kInPrompt) : atomicAdd(&counts[at], 1u);
+      if (before == 0) listed[atomicAdd(&met, 1u)] = static_cast<uint16_t>(at);
+    }
+  }
+  __syncthreads();
+  if (!a.in_place) wait_for_producers();  // the pass has written its logits
   const T* in = static_cast<const T*>(a.logits) + row * a.row_stride + base;
-  T raw[kPer];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    if (j * kLogitsThreads + tid < size) raw[j] = in[j * kLogitsThreads + tid];
-  }
-  uint32_t words = 0xffffffffu;  // lane j: the mask of the warp's j-th 32 tokens
-  if (a.mask && lane < kPer && (lane * kLogitsWarps + warp) * kWarp < size) {
-    words = static_cast<uint32_t>(a.mask[row * a.mask_stride + base / 32 + lane * kLogitsWarps + warp]);
-  }
-  const float rep = a.repetition ? a.repetition[row] : 1.0f;
-  const float freq = a.frequency ? a.frequency[row] : 0.0f;
-  const float pres = a.presence ? a.presence[row] : 0.0f;
-  const bool marked = a.tokens || a.bias_starts;
-  if (marked) {
-#pragma unroll
-    for (int j = 0; j < 2 * kPer / 4; ++j) {
-      reinterpret_cast<uint4*>(counts)[j * kLogitsThreads + tid] = make_uint4(0, 0, 0, 0);
-    }
-    cluster.barrier_arrive();
-    const int64_t* t = a.tokens + row * a.token_stride;
-    constexpr int kAhead = 4;
-    const int64_t step = static_cast<int64_t>(ctas) * kLogitsThreads;
-    const int64_t start = static_cast<int64_t>(cta) * kLogitsThreads + tid;
-    int64_t id[kAhead];
-    auto load = [&](int64_t i) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) id[u] = i + u * step < length ? t[i + u * step] : -1;
-    };
-    load(start);
-    int64_t bias_id = bias0 + tid < bias1 ? a.bias_ids[bias0 + tid] : -1;
-    cluster.barrier_wait();  // every CTA's words are zero
-    for (int64_t i = start; i < length; i += kAhead * step) {
-      if (i > start) load(i);
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int64_t at = id[u] - first;
-        if (id[u] < 0 || at < 0 || at >= static_cast<int64_t>(ctas) * kSlice) continue;  // (past the vocabulary: no one reads it)
-        uint32_t* count = cluster.map_shared_rank(counts, static_cast<int>(at / kSlice)) + at % kSlice;
-        if (i + u * step < prompt) {
-          atomicOr(count, kInPrompt);
-        } else {
-          atomicAdd(count, 1u);
-        }
-      }
-    }
-    for (int64_t i = bias0 + tid; i < bias1; i += kLogitsThreads) {
-      if (i > bias0 + tid) bias_id = a.bias_ids[i];
-      const int64_t at = bias_id - base;
-      if (bias_id >= 0 && at >= 0 && at < size) atomicMax(&bias[at], static_cast<uint32_t>(i - bias0 + 1));
-    }
-    cluster.sync();
-  }
   float* out = a.out + row * a.out_stride + base;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int i = j * kLogitsThreads + tid;
-    const uint32_t word = __shfl_sync(kFullMask, words, j);
-    if (i >= size) continue;
-    float l = to_float(raw[j]);
-    if (marked) {
-      const uint32_t c = counts[i], entry = bias[i];
-      if (c) {
-        l = l > 0.0f ? l / rep : l * rep;
-        const uint32_t said = c & ~kInPrompt;
-        if (said) l = l - freq * static_cast<float>(said) - pres;
-      }
-      if (entry) l += a.bias_values[bias0 + entry - 1];
-    }
-    out[i] = word >> lane & 1u ? l : -INFINITY;
+  auto hidden = [&](int at) {
+    return a.mask && !(static_cast<uint32_t>(a.mask[row * a.mask_stride + (base + at) / 32]) >> (at % 32) & 1u);
+  };
+  const int count = static_cast<int>(met);
+  for (int k = tid; k < count; k += kMarkThreads) {
+    const int at = listed[k];
+    float l = to_float(in[at]);
+    if (hidden(at)) continue;
+    l = l > 0.0f ? l / rep : l * rep;
+    const uint32_t said = counts[at] & ~kInPrompt;
+    if (said) l = l - freq * static_cast<float>(said) - pres;
+    out[at] = l;
   }
+  if (bias0 >= bias1) return;
+  // Biases: the last entry that names a token counts.
+  auto each = [&](auto&& f) {
+    for (int64_t i = bias0 + tid; i < bias1; i += kMarkThreads) {
+      const int64_t b = i == bias0 + tid ? bias_id : a.bias_ids[i];
+      if (b >= base && b - base < size) f(i, static_cast<int>(b - base));
+    }
+  };
+  __syncthreads();
+  each([&](int64_t, int at) { counts[at] = 0; });
+  __syncthreads();
+  each([&](int64_t i, int at) { atomicMax(&counts[at], static_cast<uint32_t>(i - bias0 + 1)); });
+  __syncthreads();
+  each([&](int64_t i, int at) {
+    if (counts[at] == static_cast<uint32_t>(i - bias0 + 1) && !hidden(at)) out[at] += a.bias_values[i];
+  });
 }
 
-template <typename T, int kPer>
-cudaError_t launch_slices(LogitsArgs a, int64_t rows, cudaStream_t stream) {
-  const int64_t slices = (a.vocab + kPer * kLogitsThreads - 1) / (kPer * kLogitsThreads);
-  // The fewest clusters of up to eight, all of the same size.
-  a.clusters = static_cast<int32_t>((slices + 7) / 8);
-  const int64_t ctas = (slices + a.clusters - 1) / a.clusters;
-  const int64_t blocks = rows * a.clusters * ctas;
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  constexpr int kSmem = 2 * kPer * kLogitsThreads * 4;
+template <typename T>
+cudaError_t launch_logits(const LogitsArgs& a, cudaStream_t stream) {
+  constexpr int kSmem = kMarkSlice * 6;
   static bool configured[64] = {};
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    const cudaError_t err =
-        cudaFuncSetAttribute(logits_kernel<T, kPer>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    const cudaError_t err = cudaFuncSetAttribute(mark_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (err != cudaSuccess) return err;
     configured[dev] = true;
   }
-  cudaLaunchAttribute attr[2]{};
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(blocks));
-  config.blockDim = dim3(kLogitsThreads);
-  config.dynamicSmemBytes = kSmem;
   config.stream = stream;
-  config.attrs = attr;
-  config.numAttrs = 2;
-  return cudaLaunchKernelEx(&config, logits_kernel<T, kPer>, a);
-}
-
-// The longest slices that still give every SM two CTAs: 8192, 4096 or 1024 tokens.
-template <typename T>
-cudaError_t launch_logits(const LogitsArgs& a, int64_t rows, cudaStream_t stream) {
-  if (rows * a.vocab >= int64_t{2 * 148} * 16 * kLogitsThreads) return launch_slices<T, 16>(a, rows, stream);
-  if (rows * a.vocab >= int64_t{2 * 148} * 8 * kLogitsThreads) return launch_slices<T, 8>(a, rows, stream);
-  return launch_slices<T, 2>(a, rows, stream);
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  auto pass = [&] {
+    if (a.in_place && !a.mask) return cudaSuccess;
+    const int64_t chunks = (a.vocab + kPassChunk - 1) / kPassChunk * a.rows;
+    config.gridDim = dim3(static_cast<unsigned>(chunks < 148 * kPassCtas ? chunks : 148 * kPassCtas));
+    config.blockDim = dim3(kPassThreads);
+    config.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&config, pass_kernel<T>, a);
+  };
+  auto marks = [&] {
+    if (!a.tokens && !a.bias_starts) return cudaSuccess;
+    config.blockDim = dim3(kMarkThreads);
+    const int64_t blocks = (a.vocab + kMarkSlice - 1) / kMarkSlice * a.rows;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    config.gridDim = dim3(static_cast<unsigned>(blocks));
+    config.dynamicSmemBytes = kSmem;
+    return cudaLaunchKernelEx(&config, mark_kernel<T>, a);
+  };
+  const cudaError_t err = a.in_place ? marks() : pass();
+  return err != cudaSuccess ? err : a.in_place ? pass() : marks();
 }
 
 }  // namespace
@@ -197,7 +221,7 @@ extern "C" int pck_process_logits(const pck_logits_desc* desc, void* stream) {
   if (dtype != PCK_LOGITS_F32 && dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) {
     return report_error(PCK_ERR_ARGUMENT, "logits: unknown dtype");
   }
-  if (rows < 0 || vocab < 1 || vocab > 0x7fffffffLL || row_stride < vocab || out_stride < vocab) {
+  if (rows < 0 || rows > 0x7fffffffLL || vocab < 1 || vocab > 0x7fffffffLL || row_stride < vocab || out_stride < vocab) {
     return report_error(PCK_ERR_ARGUMENT, "logits: need rows >= 0, vocab in [1, 2^31) and strides of whole rows");
   }
   if (tokens && (!lengths || max_tokens < 0 || token_stride < max_tokens)) {
@@ -210,11 +234,12 @@ extern "C" int pck_process_logits(const pck_logits_desc* desc, void* stream) {
   if (mask && mask_stride < (vocab + 31) / 32) return report_error(PCK_ERR_ARGUMENT, "logits: a mask row has ceil(vocab / 32) words");
   if (rows == 0) return PCK_OK;
   if (!logits || !out) return report_error(PCK_ERR_ARGUMENT, "logits: NULL logits or out");
-  LogitsArgs a{logits, row_stride, vocab, tokens, token_stride, max_tokens, prompt_lengths, lengths, repetition, frequency,
-               presence, bias_starts, bias_ids, bias_values, biases, mask, mask_stride, out, out_stride, 0};
+  const int32_t in_place = out == logits && out_stride == row_stride && dtype == PCK_LOGITS_F32;
+  const LogitsArgs a{logits, row_stride, vocab, tokens, token_stride, max_tokens, prompt_lengths, lengths, repetition, frequency,
+                     presence, bias_starts, bias_ids, bias_values, biases, mask, mask_stride, out, out_stride, rows, in_place};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = dtype == PCK_LOGITS_F32    ? launch_logits<float>(a, rows, s)
-                          : dtype == PCK_LOGITS_BF16 ? launch_logits<__nv_bfloat16>(a, rows, s)
-                                                     : launch_logits<__half>(a, rows, s);
+  const cudaError_t err = dtype == PCK_LOGITS_F32    ? launch_logits<float>(a, s)
+                          : dtype == PCK_LOGITS_BF16 ? launch_logits<__nv_bfloat16>(a, s)
+                                                     : launch_logits<__half>(a, s);
   return err == cudaSuccess ? PCK_OK : report_cuda("logits kernel", err);
 }
