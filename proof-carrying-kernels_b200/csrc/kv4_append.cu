@@ -241,8 +241,11 @@ PCK_STATUS_READER(append_status)
 extern "C" int pck_kv4_append(const pck_kv4_append_desc* desc, void* stream) {
   using namespace pck;
   if (!desc) return report_error(PCK_ERR_ARGUMENT, "append: NULL descriptor");
-  const auto& [cache, pages, kv_heads, page_tiles, dim, k, v, dtype, tokens, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, k_values, v_values] = *desc;
-  if (dim != 64 && dim != 128 && dim != 256) return report_error(PCK_ERR_ARGUMENT, "append: dim must be 64, 128 or 256");
+  const auto& [cache, pages, kv_heads, page_tiles, dim, k, v, dtype, tokens, k_token_stride, k_head_stride,
+               v_token_stride, v_head_stride, slots, k_values, v_values] = *desc;
+  if (dim != 64 && dim != 128 && dim != 256) {
+    return report_error(PCK_ERR_ARGUMENT, "append: dim must be 64, 128 or 256");
+  }
   if (pages < 0 || kv_heads < 1 || kv_heads > 0x3fff || page_tiles < 1 || page_tiles > 0x7fffffff || tokens < 0) {
     return report_error(PCK_ERR_ARGUMENT, "append: need pages >= 0, kv_heads in [1, 16383], page_tiles >= 1 and tokens >= 0");
   }

@@ -322,7 +322,8 @@ __device__ __forceinline__ void store_row(T* to, float4 o, float l) {
     const T x = from_float<T>(l == 0.0f ? 0.0f : v[i] / l);
     u[i] = *reinterpret_cast<const uint16_t*>(&x);
   }
-  *reinterpret_cast<uint2*>(to) = make_uint2(u[0] | static_cast<uint32_t>(u[1]) << 16, u[2] | static_cast<uint32_t>(u[3]) << 16);
+  *reinterpret_cast<uint2*>(to) =
+      make_uint2(u[0] | static_cast<uint32_t>(u[1]) << 16, u[2] | static_cast<uint32_t>(u[3]) << 16);
 }
 
 template <typename T, int kDim, int kRows>
@@ -368,7 +369,8 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     filled = __shfl_sync(kFullMask, filled, 0) * items;
     const bool pieces = 2 * filled <= a.parts;
     // Tiles of a piece, at most: with this many the pieces are no more than the CTAs.
-    const int piece = pieces ? static_cast<int>(max(int64_t{kMinPiece}, divide(tiles * items, a.parts - filled) + 1)) : 1;
+    const int64_t even = pieces ? divide(tiles * items, a.parts - filled) + 1 : 1;
+    const int piece = static_cast<int>(max(int64_t{kMinPiece}, even));
     auto places = [&](int n) -> int64_t { return pieces ? (n + piece - 1) / piece : item_length(n); };
     int64_t begin = blockIdx.x, end = begin + 1;
     if (!pieces) {
@@ -423,8 +425,9 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     const int64_t row_size = static_cast<int64_t>(a.queries) * a.heads * kDim;
     for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
       if (request_tiles(a, b).tiles == 0) {
-        for (int64_t i = tid - kWarp; i < row_size; i += kAttnThreads - kWarp) out[b * row_size + i] = from_float<T>(0.0f);
-        for (int64_t i = tid - kWarp; a.parts > 1 && i < items; i += kAttnThreads - kWarp) a.split[b * items + i] = make_int2(0, 0);
+        constexpr int kRest = kAttnThreads - kWarp;
+        for (int64_t i = tid - kWarp; i < row_size; i += kRest) out[b * row_size + i] = from_float<T>(0.0f);
+        for (int64_t i = tid - kWarp; a.parts > 1 && i < items; i += kRest) a.split[b * items + i] = make_int2(0, 0);
       }
     }
   }
@@ -1032,7 +1035,8 @@ cudaError_t launch(const AttentionArgs& a, cudaStream_t stream) {
   config.numAttrs = 1;
   cudaError_t err = cudaLaunchKernelEx(&config, attention_kernel<T, kDim, kRows>, a);
   if (err != cudaSuccess || a.parts == 1) return err;  // one part: nothing is split
-  const int64_t joins = a.batch * a.kv_heads * a.row_blocks * ((std::min(kRows, a.queries * a.group) + kJoinRows - 1) / kJoinRows);
+  const int chunks = (std::min(kRows, a.queries * a.group) + kJoinRows - 1) / kJoinRows;
+  const int64_t joins = a.batch * a.kv_heads * a.row_blocks * chunks;
   if (joins > 0x7fffffffLL) return cudaErrorInvalidValue;
   config.gridDim = dim3(static_cast<unsigned>(joins));
   config.blockDim = dim3(kJoinThreads);
@@ -1067,9 +1071,15 @@ extern "C" int64_t pck_kv4_attention_scratch(int64_t batch, int64_t queries, int
 extern "C" int pck_kv4_attention(const pck_kv4_attention_desc* desc, void* stream) {
   using namespace pck;
   if (!desc) return report_error(PCK_ERR_ARGUMENT, "attention: NULL descriptor");
-  const auto& [q, dtype, batch, queries, heads, dim, q_batch_stride, q_token_stride, q_head_stride, cache, pages, kv_heads, page_tiles, page_table, table_stride, table_pages, lengths, scale, window, out, scratch, scratch_bytes] = *desc;
-  if (dim != 64 && dim != 128 && dim != 256) return report_error(PCK_ERR_ARGUMENT, "attention: dim must be 64, 128 or 256");
-  if (dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) return report_error(PCK_ERR_ARGUMENT, "attention: q must be bfloat16 or float16");
+  const auto& [q, dtype, batch, queries, heads, dim, q_batch_stride, q_token_stride, q_head_stride, cache, pages,
+               kv_heads, page_tiles, page_table, table_stride, table_pages, lengths, scale, window, out, scratch,
+               scratch_bytes] = *desc;
+  if (dim != 64 && dim != 128 && dim != 256) {
+    return report_error(PCK_ERR_ARGUMENT, "attention: dim must be 64, 128 or 256");
+  }
+  if (dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) {
+    return report_error(PCK_ERR_ARGUMENT, "attention: q must be bfloat16 or float16");
+  }
   if (batch < 0 || queries < 1 || kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || heads > 0xffff ||
       queries > 0x7fff) {
     return report_error(PCK_ERR_ARGUMENT, "attention: need batch >= 0, queries in [1, 32767] and heads a multiple of kv_heads");

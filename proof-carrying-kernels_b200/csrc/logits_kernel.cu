@@ -217,7 +217,9 @@ cudaError_t launch_logits(const LogitsArgs& a, cudaStream_t stream) {
 extern "C" int pck_process_logits(const pck_logits_desc* desc, void* stream) {
   using namespace pck;
   if (!desc) return report_error(PCK_ERR_ARGUMENT, "logits: NULL descriptor");
-  const auto& [logits, dtype, rows, vocab, row_stride, tokens, token_stride, max_tokens, prompt_lengths, lengths, repetition, frequency, presence, bias_starts, bias_ids, bias_values, biases, mask, mask_stride, out, out_stride] = *desc;
+  const auto& [logits, dtype, rows, vocab, row_stride, tokens, token_stride, max_tokens, prompt_lengths, lengths,
+               repetition, frequency, presence, bias_starts, bias_ids, bias_values, biases, mask, mask_stride, out,
+               out_stride] = *desc;
   if (dtype != PCK_LOGITS_F32 && dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) {
     return report_error(PCK_ERR_ARGUMENT, "logits: unknown dtype");
   }

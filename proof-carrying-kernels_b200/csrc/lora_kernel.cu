@@ -605,8 +605,11 @@ PCK_STATUS_READER(lora_status)
 extern "C" int pck_lora_add(const pck_lora_desc* desc, void* stream) {
   using namespace pck;
   if (!desc) return report_error(PCK_ERR_ARGUMENT, "adapters: NULL descriptor");
-  const auto& [x, dtype, tokens, n, x_stride, y, m, y_stride, A, B, count, rank, adapters, scales, ranks, out, out_stride] = *desc;
-  if (dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) return report_error(PCK_ERR_ARGUMENT, "adapters: x must be bfloat16 or float16");
+  const auto& [x, dtype, tokens, n, x_stride, y, m, y_stride, A, B, count, rank, adapters, scales, ranks, out,
+               out_stride] = *desc;
+  if (dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) {
+    return report_error(PCK_ERR_ARGUMENT, "adapters: x must be bfloat16 or float16");
+  }
   if (tokens < 0 || tokens > 1 << 30 || n < 1 || m < 0 || x_stride < n || y_stride < m || out_stride < m) {
     return report_error(PCK_ERR_ARGUMENT, "adapters: need tokens >= 0, n >= 1, m >= 0 and strides of whole rows");
   }
