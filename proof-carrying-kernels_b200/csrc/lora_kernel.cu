@@ -1,8 +1,10 @@
 // pck_lora_add: out = y + s_a B_a (A_a x) for rows that each name their adapter a.
 //
-// A tile of 16 or 64 rows is walked through the distinct adapters that its rows name, an item each,
-// so rows may come in any order: a decode batch where every row has its own adapter, or prompts whose
-// rows share one. A cluster of CTAs takes an item:
+// Rows come in any order and are taken by their adapters, an item being some rows of one adapter:
+//   - decode batches, where nearly every row has its own: up to 16 rows of one adapter, gathered from 256
+//     rows, so an adapter's weights are read once for all of them;
+//   - prompts, whose rows share one: the rows of one adapter in a tile of 64.
+// A cluster of CTAs takes an item:
 //   1. h = A x for the item's rows: the CTAs and their warps split the columns n, and each product
 //      (mma.sync, binary32 sums) takes x and A straight from memory in 16-byte loads, since nothing in
 //      a warp reads them twice;
@@ -11,8 +13,7 @@
 //   3. out = y + s B h: the CTAs and warps split the outputs m. h enters the products as three (bfloat16)
 //      or two (binary16, scaled by a power of two of its row) terms whose sum is h to binary32's
 //      precision, so nothing is lost against a binary32 product.
-// Bound by the adapters' bytes for decode batches (each read once per tile that names it) and by x, y and
-// out for prompts; with few rows by the latency of the two dependent passes, which is why a single row
+// Bound by the adapters' bytes for decode batches and by x, y and out for prompts; with few rows by the latency of the two dependent passes, which is why a single row
 // is spread over a cluster of eight CTAs.
 #include <cooperative_groups.h>
 
@@ -205,39 +206,71 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
   const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
   const int row8 = lane / 4, quarter = lane % 4;
   const int sub = warp % kSub, share = warp / kSub;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x / ctas) * S::kM;
+  constexpr int kSpan = kSub == 1 ? kLoraThreads : S::kM;  // rows that a cluster's items come from
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x / ctas) * kSpan;
+  __shared__ int members[16];  // of an item of a decode batch: its rows
   wait_for_producers();
   allow_dependents();
 
-  // The rows' adapters: lane i has row i (and 32 + i); -1 for none, -2 past the last row.
-  int owner[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 32 * i + lane;
-    owner[i] = r < S::kM && row0 + r < a.tokens ? max(a.adapters[row0 + r], -1) : -2;
-    if (owner[i] >= a.count) {
-      if (warp == 0 && cta == 0 && blockIdx.y == 0) report(kDevIndex);
-      owner[i] = -1;
+  // A row's adapter: -1 for none, -2 past the last row.
+  auto owner_of = [&](int r) {
+    int owner = row0 + r < a.tokens ? max(a.adapters[row0 + r], -1) : -2;
+    if (owner >= a.count) {
+      if (cta == 0 && blockIdx.y == 0) report(kDevIndex);
+      owner = -1;
     }
+    return owner;
+  };
+  int owner[2] = {-2, -2};
+  if constexpr (kSub > 1) {  // lane i has row i and row 32 + i of the tile
+    owner[0] = owner_of(lane);
+    owner[1] = owner_of(32 + lane);
   }
   for (int item = blockIdx.y;; item += gridDim.y) {
-    // The item-th distinct adapter, in the order of the rows, and its rows.
+    // The item's adapter and its rows, as bits.
     uint32_t rows[2] = {0, 0};
     int adapter = -1;
     if constexpr (kSub == 1) {
-      const uint32_t like = __match_any_sync(kFullMask, owner[0]);
-      uint32_t firsts = __ballot_sync(kFullMask, owner[0] >= 0 && __ffs(like) - 1 == lane);
-      for (int i = 0; i < item; ++i) firsts &= firsts - 1;
-      if (firsts) {
-        adapter = __shfl_sync(kFullMask, owner[0], __ffs(firsts) - 1);
-        rows[0] = __shfl_sync(kFullMask, like, __ffs(firsts) - 1);
+      // Groups of 16 rows of one adapter (rows without one are another), numbered by their first rows.
+      __shared__ __align__(16) int owners[kLoraThreads];
+      __shared__ int firsts[kLoraWarps];
+      __shared__ int found[2];
+      const int tid = threadIdx.x;
+      owners[tid] = owner_of(tid);
+      if (tid == 0) found[0] = -2;
+      __syncthreads();
+      const int own = owners[tid];
+      int before = 0;  // rows of the same adapter before this one
+      const int upto = own == -2 ? 0 : (warp + 1) * kWarp;
+      for (int k = 0; k < upto; k += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(owners + k);
+        before += (v.x == own && k < tid) + (v.y == own && k + 1 < tid);
+        before += (v.z == own && k + 2 < tid) + (v.w == own && k + 3 < tid);
       }
+      const bool first = own >= -1 && before % 16 == 0;
+      const unsigned ballot = __ballot_sync(kFullMask, first);
+      if (lane == 0) firsts[warp] = __popc(ballot);
+      __syncthreads();
+      int number = __popc(ballot & ((1u << lane) - 1));
+      for (int w = 0; w < warp; ++w) number += firsts[w];
+      if (first && number == item) {
+        found[0] = own;
+        found[1] = before;
+      }
+      __syncthreads();
+      if (found[0] == -2) return;  // there are fewer groups
+      adapter = found[0];
+      const int place = before - found[1];
+      const bool member = own == adapter && place >= 0 && place < 16;
+      if (member) members[place] = tid;
+      rows[0] = (1u << __syncthreads_count(member)) - 1;
     } else {
       uint32_t left[2] = {__ballot_sync(kFullMask, owner[0] >= 0), __ballot_sync(kFullMask, owner[1] >= 0)};
       for (int i = 0; left[0] | left[1]; ++i) {
         const int first = left[0] ? __shfl_sync(kFullMask, owner[0], __ffs(left[0]) - 1)
                                   : __shfl_sync(kFullMask, owner[1], __ffs(left[1]) - 1);
-        const uint32_t in0 = __ballot_sync(kFullMask, owner[0] == first), in1 = __ballot_sync(kFullMask, owner[1] == first);
+        const uint32_t in0 = __ballot_sync(kFullMask, owner[0] == first);
+        const uint32_t in1 = __ballot_sync(kFullMask, owner[1] == first);
         if (i == item) {
           adapter = first;
           rows[0] = in0;
@@ -247,16 +280,26 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
         left[0] &= ~in0;
         left[1] &= ~in1;
       }
+      if (adapter < 0 && item > 0) return;
     }
-    if (adapter < 0 && item > 0) return;
-    // Rows without an adapter go with the first item.
-    uint32_t plain[2] = {__ballot_sync(kFullMask, owner[0] == -1), __ballot_sync(kFullMask, owner[1] == -1)};
-    if (item > 0) plain[0] = plain[1] = 0;
+    // Rows without an adapter: a group of their own, or with the tile's first item.
+    uint32_t plain[2] = {0, 0};
+    if constexpr (kSub == 1) {
+      if (adapter < 0) {
+        plain[0] = rows[0];
+        rows[0] = 0;
+      }
+    } else if (item == 0) {
+      plain[0] = __ballot_sync(kFullMask, owner[0] == -1);
+      plain[1] = __ballot_sync(kFullMask, owner[1] == -1);
+    }
     const int rank = adapter < 0 ? 0 : a.ranks ? min(max(a.ranks[adapter], 0), a.rank) : a.rank;
     const float scale = adapter >= 0 && a.scales ? a.scales[adapter] : 1.0f;
     // This warp's 16 rows of the item.
     const uint32_t active = (sub < 2 ? rows[0] >> 16 * sub : rows[1] >> 16 * (sub - 2)) & 0xffffu;
     const uint32_t copied = (sub < 2 ? plain[0] >> 16 * sub : plain[1] >> 16 * (sub - 2)) & 0xffffu;
+    // Where row r of the block lies.
+    auto row_of = [&](int r) { return row0 + (kSub == 1 ? members[r] : 16 * sub + r); };
     const int64_t m_blocks = (a.m + 31) / 32;
     const int64_t m0 = m_blocks * cta / ctas, m1 = m_blocks * (cta + 1) / ctas;
     const uint16_t* const Ba = static_cast<const uint16_t*>(a.B) + static_cast<int64_t>(max(adapter, 0)) * a.m * a.rank;
@@ -287,7 +330,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = active >> (row8 + 8 * h) & 1u ? row8 + 8 * h : other;
-          x[h] = static_cast<const uint16_t*>(a.x) + (row0 + 16 * sub + r) * a.x_stride;
+          x[h] = static_cast<const uint16_t*>(a.x) + row_of(r) * a.x_stride;
         }
         const uint16_t* const Aa = static_cast<const uint16_t*>(a.A) + static_cast<int64_t>(adapter) * a.rank * a.n;
         auto product = [&](int j, const uint32_t (&x0)[4], const uint32_t (&x1)[4], const uint32_t (&w)[4]) {
@@ -467,7 +510,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if ((active | copied) >> (row8 + 8 * h) & 1u) {
-            const float4* from = reinterpret_cast<const float4*>(a.y + (row0 + 16 * sub + row8 + 8 * h) * a.y_stride + c0);
+            const float4* from = reinterpret_cast<const float4*>(a.y + row_of(row8 + 8 * h) * a.y_stride + c0);
             y[h][0] = from[0];
             y[h][1] = from[1];
           }
@@ -511,7 +554,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = on && rank > 0 ? acc[i / 2][2 * h + i % 2] * by : 0.0f;
-        float* out = a.out + (row0 + 16 * sub + r) * a.out_stride + c0;
+        float* out = a.out + row_of(r) * a.out_stride + c0;
         if (vector) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -520,7 +563,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
                 make_float4(from.x + v[4 * i], from.y + v[4 * i + 1], from.z + v[4 * i + 2], from.w + v[4 * i + 3]);
           }
         } else {
-          const float* y = a.y + (row0 + 16 * sub + r) * a.y_stride + c0;
+          const float* y = a.y + row_of(r) * a.y_stride + c0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if (c0 + i < a.m) out[i] = y[i] + v[i];
@@ -537,6 +580,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
       if (ctas > 1) cluster.barrier_wait();  // the peers have read this CTA's sums
       __syncthreads();
     }
+    if (kSub == 1) return;  // (the grid has a place for every group)
   }
 }
 
@@ -580,19 +624,19 @@ cudaError_t launch_rank(const LoraArgs& a, int tiles, int items, int ctas, cudaS
   return launch_lora<T, kSub, 16>(a, tiles, items, ctas, s);
 }
 
-// Up to 256 rows are taken as a decode batch: tiles of 16, an item for each of its rows' adapters, many
-// CTAs an item. More are taken as prompts: tiles of 64, two items at a time (a tile rarely meets more),
-// and as many CTAs an item as give the SMs two each. (Ranks over 128 leave no room for the sums of 64 rows.)
+// Up to 256 rows are taken as a decode batch: as many places for groups as there are rows, a cluster each.
+// More are taken as prompts: two items of a tile at a time (it rarely meets more), and as many CTAs an item
+// as run at once. (Ranks over 128 leave no room for the sums of 64 rows.)
 template <typename T>
 cudaError_t launch_tokens(const LoraArgs& a, cudaStream_t s) {
   if (a.tokens <= 256 || a.rank > 128) {
-    const int tiles = static_cast<int>((a.tokens + 15) / 16);
-    const int items = static_cast<int>(a.tokens < 16 ? a.tokens : 16);
-    return launch_rank<T, 1>(a, tiles, items, a.tokens <= 32 ? 8 : 4, s);
+    const int spans = static_cast<int>((a.tokens + kLoraThreads - 1) / kLoraThreads);
+    const int items = static_cast<int>(a.tokens < kLoraThreads ? a.tokens : kLoraThreads);
+    return launch_rank<T, 1>(a, spans, items, a.tokens <= 32 ? 8 : 4, s);
   }
   const int tiles = static_cast<int>((a.tokens + 63) / 64);
   int ctas = 8;
-  while (ctas > 1 && tiles * ctas > 2 * 148) ctas /= 2;
+  while (ctas > 1 && tiles * ctas > 148 * (a.rank <= 64 ? 2 : 1)) ctas /= 2;
   return launch_rank<T, 4>(a, tiles, 2, ctas, s);
 }
 
