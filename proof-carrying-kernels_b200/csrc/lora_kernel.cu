@@ -45,8 +45,10 @@ struct LoraArgs {
   int64_t out_stride;
   int64_t n, m, tokens;
   int32_t count, rank;
+  int32_t rank0;      // first rank of this launch, which takes up to `taken` of them
+  int32_t taken;
   int32_t n_vector;   // rows of x and A are 16-byte aligned
-  int32_t rank_vector;  // rows of B are aligned to a load's ranks
+  int32_t rank_vector;  // ranks that the rows of B are aligned to: 8, 4 or 0
   int32_t y_vector;   // rows of y and out are 16-byte aligned
 };
 
@@ -136,7 +138,7 @@ __device__ __forceinline__ int64_t staged_steps(const LoraArgs& a, uint8_t* smem
   const int lane = threadIdx.x % kWarp, warp = threadIdx.x / kWarp;
   const int row8 = lane / 4, quarter = lane % 4, sub = warp % kSub, share = warp / kSub;
   const int other = rows[0] ? __ffs(rows[0]) - 1 : 31 + __ffs(rows[1]);
-  const uint16_t* const Aa = static_cast<const uint16_t*>(a.A) + static_cast<int64_t>(adapter) * a.rank * a.n;
+  const uint16_t* const Aa = static_cast<const uint16_t*>(a.A) + (static_cast<int64_t>(adapter) * a.rank + a.rank0) * a.n;
   // The pieces that this thread copies: row i / 8, piece i % 8 of 128 bytes.
   constexpr int kPieces = (S::kM + S::kR) * 8;
   constexpr int kMine = (kPieces + kLoraThreads - 1) / kLoraThreads;
@@ -293,7 +295,15 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
       plain[0] = __ballot_sync(kFullMask, owner[0] == -1);
       plain[1] = __ballot_sync(kFullMask, owner[1] == -1);
     }
-    const int rank = adapter < 0 ? 0 : a.ranks ? min(max(a.ranks[adapter], 0), a.rank) : a.rank;
+    int rank = adapter < 0 ? 0 : a.ranks ? min(max(a.ranks[adapter], 0), a.rank) : a.rank;
+    rank = min(max(rank - a.rank0, 0), a.taken);
+    if (a.rank0 > 0) {  // a later launch on the same rows: out already has what these add to
+      if (rank == 0) {
+        if (kSub == 1) return;
+        continue;
+      }
+      plain[0] = plain[1] = 0;
+    }
     const float scale = adapter >= 0 && a.scales ? a.scales[adapter] : 1.0f;
     // This warp's 16 rows of the item.
     const uint32_t active = (sub < 2 ? rows[0] >> 16 * sub : rows[1] >> 16 * (sub - 2)) & 0xffffu;
@@ -302,7 +312,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
     auto row_of = [&](int r) { return row0 + (kSub == 1 ? members[r] : 16 * sub + r); };
     const int64_t m_blocks = (a.m + 31) / 32;
     const int64_t m0 = m_blocks * cta / ctas, m1 = m_blocks * (cta + 1) / ctas;
-    const uint16_t* const Ba = static_cast<const uint16_t*>(a.B) + static_cast<int64_t>(max(adapter, 0)) * a.m * a.rank;
+    const uint16_t* const Ba = static_cast<const uint16_t*>(a.B) + static_cast<int64_t>(max(adapter, 0)) * a.m * a.rank + a.rank0;
     if (kSub == 1 && rank > 0) {  // B is not needed before h: have it on its way
       const char* from = reinterpret_cast<const char*>(Ba + 32 * m0 * a.rank);
       const int64_t bytes = (min(32 * m1, a.m) - 32 * m0) * a.rank * 2;
@@ -332,7 +342,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
           const int r = active >> (row8 + 8 * h) & 1u ? row8 + 8 * h : other;
           x[h] = static_cast<const uint16_t*>(a.x) + row_of(r) * a.x_stride;
         }
-        const uint16_t* const Aa = static_cast<const uint16_t*>(a.A) + static_cast<int64_t>(adapter) * a.rank * a.n;
+        const uint16_t* const Aa = static_cast<const uint16_t*>(a.A) + (static_cast<int64_t>(adapter) * a.rank + a.rank0) * a.n;
         auto product = [&](int j, const uint32_t (&x0)[4], const uint32_t (&x1)[4], const uint32_t (&w)[4]) {
           lora_mma<T>(acc[j], x0[0], x1[0], x0[1], x1[1], w[0], w[1]);
           lora_mma<T>(acc[j], x0[2], x1[2], x0[3], x1[3], w[2], w[3]);
@@ -464,6 +474,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
     // the SM's requests in flight empty.
     constexpr int kK = S::kR < 64 ? S::kR / 16 : 4;
     constexpr int kLoad = kK == 1 ? 4 : 8;  // ranks of a load
+    const int held = a.rank - a.rank0;      // of a row of B from here on
     auto load_b = [&](int64_t b, int from, uint32_t (&w)[4][2 * kK]) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -474,18 +485,18 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
 #pragma unroll
         for (int u = 0; u < 4 * kK / kLoad; ++u) {
           uint32_t* to = &w[j][kLoad / 2 * u];
-          if (a.rank_vector) {
-            const uint16_t* at = row + min(r + kLoad * u, a.rank - kLoad);
-            if constexpr (kLoad == 8) {
-              const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
-              to[0] = v.x;
-              to[1] = v.y;
-              to[2] = v.z;
-              to[3] = v.w;
-            } else {
-              const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
-              to[0] = v.x;
-              to[1] = v.y;
+          if (kLoad == 8 && a.rank_vector == 8) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + min(r + 8 * u, held - 8)));
+            to[0] = v.x;
+            to[1] = v.y;
+            to[kLoad / 2 - 2] = v.z;
+            to[kLoad / 2 - 1] = v.w;
+          } else if (a.rank_vector) {
+#pragma unroll
+            for (int h = 0; h < kLoad / 4; ++h) {
+              const uint2 v = __ldg(reinterpret_cast<const uint2*>(row + min(r + kLoad * u + 4 * h, held - 4)));
+              to[2 * h] = v.x;
+              to[2 * h + 1] = v.y;
             }
           } else {
             load_row<kLoad>(*reinterpret_cast<uint32_t(*)[kLoad / 2]>(to), row, r + kLoad * u, rank, rank, false);
@@ -615,29 +626,35 @@ cudaError_t launch_lora(const LoraArgs& a, int tiles, int items, int ctas, cudaS
 
 template <typename T, int kSub>
 cudaError_t launch_rank(const LoraArgs& a, int tiles, int items, int ctas, cudaStream_t s) {
-  if (a.rank <= 16) return launch_lora<T, kSub, 2>(a, tiles, items, ctas, s);
-  if (a.rank <= 32) return launch_lora<T, kSub, 4>(a, tiles, items, ctas, s);
-  if (a.rank <= 64) return launch_lora<T, kSub, 8>(a, tiles, items, ctas, s);
+  if (a.taken <= 16) return launch_lora<T, kSub, 2>(a, tiles, items, ctas, s);
+  if (a.taken <= 32) return launch_lora<T, kSub, 4>(a, tiles, items, ctas, s);
   if constexpr (kSub == 1) {
-    if (a.rank > 128) return launch_lora<T, kSub, 32>(a, tiles, items, ctas, s);
+    if (a.taken > 128) return launch_lora<T, kSub, 32>(a, tiles, items, ctas, s);
+    if (a.taken > 64) return launch_lora<T, kSub, 16>(a, tiles, items, ctas, s);
   }
-  return launch_lora<T, kSub, 16>(a, tiles, items, ctas, s);
+  return launch_lora<T, kSub, 8>(a, tiles, items, ctas, s);
 }
 
 // Up to 256 rows are taken as a decode batch: as many places for groups as there are rows, a cluster each.
 // More are taken as prompts: two items of a tile at a time (it rarely meets more), and as many CTAs an item
-// as run at once. (Ranks over 128 leave no room for the sums of 64 rows.)
+// as run at once; 64 ranks a launch, the later ones adding to out: the sums of 64 rows and more ranks leave
+// an SM one CTA and its registers no room for loads in flight (2,000 rows of rank 100: 145 us so, 135 us in
+// two launches).
 template <typename T>
-cudaError_t launch_tokens(const LoraArgs& a, cudaStream_t s) {
-  if (a.tokens <= 256 || a.rank > 128) {
-    const int spans = static_cast<int>((a.tokens + kLoraThreads - 1) / kLoraThreads);
-    const int items = static_cast<int>(a.tokens < kLoraThreads ? a.tokens : kLoraThreads);
-    return launch_rank<T, 1>(a, spans, items, a.tokens <= 32 ? 8 : 4, s);
+cudaError_t launch_tokens(LoraArgs a, cudaStream_t s) {
+  if (a.tokens <= kLoraThreads) {
+    return launch_rank<T, 1>(a, 1, static_cast<int>(a.tokens), a.tokens <= 32 ? 8 : 4, s);
   }
   const int tiles = static_cast<int>((a.tokens + 63) / 64);
-  int ctas = 8;
-  while (ctas > 1 && tiles * ctas > 148 * (a.rank <= 64 ? 2 : 1)) ctas /= 2;
-  return launch_rank<T, 4>(a, tiles, 2, ctas, s);
+  int ctas = kLoraMaxCtas;
+  while (ctas > 1 && tiles * ctas > 148 * 2) ctas /= 2;
+  for (const int all = a.rank; a.rank0 < all; a.rank0 += 64) {
+    a.taken = all - a.rank0 < 64 ? all - a.rank0 : 64;
+    if (const cudaError_t err = launch_rank<T, 4>(a, tiles, 2, ctas, s); err != cudaSuccess) return err;
+    a.y = a.out;
+    a.y_stride = a.out_stride;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace
@@ -679,10 +696,9 @@ extern "C" int pck_lora_add(const pck_lora_desc* desc, void* stream) {
   a.m = m;
   a.tokens = tokens;
   a.count = static_cast<int32_t>(count);
-  a.rank = static_cast<int32_t>(rank);
+  a.rank = a.taken = static_cast<int32_t>(rank);
   a.n_vector = aligned_to(x, 16) && aligned_to(A, 16) && x_stride % 8 == 0 && n % 8 == 0;
-  const int piece = rank <= 16 ? 4 : 8;  // ranks that a load takes
-  a.rank_vector = aligned_to(B, 2 * piece) && rank % piece == 0;
+  a.rank_vector = aligned_to(B, 16) && rank % 8 == 0 ? 8 : aligned_to(B, 8) && rank % 4 == 0 ? 4 : 0;
   a.y_vector = aligned_to(y, 16) && aligned_to(out, 16) && y_stride % 4 == 0 && out_stride % 4 == 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t err = dtype == PCK_LOGITS_BF16 ? launch_tokens<__nv_bfloat16>(a, s) : launch_tokens<__half>(a, s);

@@ -58,7 +58,8 @@ class TestLora:
     @pytest.mark.parametrize("tokens,n,m,count,rank", [
         (1, 1, 1, 1, 1), (1, 4096, 512, 3, 16), (7, 72, 33, 2, 8), (16, 128, 128, 1, 64), (17, 520, 130, 5, 13),
         (33, 1000, 257, 40, 32), (64, 136, 64, 48, 128), (5, 64, 65, 2, 256), (70, 37, 50, 3, 5), (200, 256, 96, 4, 48),
-        (300, 512, 200, 2, 24), (65, 2048, 1024, 3, 7)])  # fmt: skip
+        (300, 512, 200, 2, 24), (65, 2048, 1024, 3, 7),
+        (270, 96, 70, 3, 68), (330, 160, 129, 2, 131), (260, 64, 96, 4, 256), (290, 100, 64, 3, 100)])  # fmt: skip
     def test_against_binary64(self, tokens, n, m, count, rank, dtype) -> None:
         from pck.cuda import device_status, lora_add
 
@@ -80,19 +81,20 @@ class TestLora:
         check(got, args, 256, 16)
         assert torch.equal(got.cpu()[adapters < 0], y[adapters < 0])
 
-    def test_strided_rows_in_place_and_unaligned(self) -> None:
+    @pytest.mark.parametrize("tokens,rank", [(21, 16), (280, 96)])
+    def test_strided_rows_in_place_and_unaligned(self, tokens, rank) -> None:
         from pck.cuda import lora_add
 
         for shift in (0, 1, 8):
-            x, y, A, B, adapters, scales, ranks = problem(21, 264, 72, 4, 16, torch.bfloat16)
-            wx = torch.zeros(21, 264 + 32, dtype=torch.bfloat16, device="cuda")
-            wy = torch.full((21, 72 + 9), 7.0, device="cuda")
+            x, y, A, B, adapters, scales, ranks = problem(tokens, 264, 72, 4, rank, torch.bfloat16)
+            wx = torch.zeros(tokens, 264 + 32, dtype=torch.bfloat16, device="cuda")
+            wy = torch.full((tokens, 72 + 9), 7.0, device="cuda")
             xs, ys = wx[:, shift : shift + 264], wy[:, shift : shift + 72]
             xs.copy_(x)
             ys.copy_(y)
             rest = [t.cuda() for t in (A, B, adapters, scales, ranks)]
             fresh = lora_add(xs, ys, *rest)
-            check(fresh, (x, y, A, B, adapters, scales, ranks), 264, 16)
+            check(fresh, (x, y, A, B, adapters, scales, ranks), 264, rank)
             assert lora_add(xs, ys, *rest, out=ys) is ys
             assert torch.equal(ys, fresh)
             keep = torch.ones(81, dtype=torch.bool)
