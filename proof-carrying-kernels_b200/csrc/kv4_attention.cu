@@ -344,8 +344,8 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     fence_barrier_init();
   }
   __syncwarp();
-  allow_dependents();
   wait_for_producers();
+  allow_dependents();
 
   T* const out = static_cast<T*>(a.out);
   const int64_t items = static_cast<int64_t>(a.kv_heads) * a.row_blocks;  // of a request
@@ -739,12 +739,20 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
-        // Keep the largest scale within 2^4 of the unit; a NaN scale leaves the unit alone.
+        // Keep the largest scale within 2^4 of the unit.
         uint32_t largest = 0;
 #pragma unroll
         for (int j = 0; j < kJ; ++j) largest = max(largest, pairs[j][g] << 16);
-        const uint32_t field = __reduce_max_sync(kFullMask, largest) >> 23;
-        if (field + 4 - unit[g] > 8 && field != 0 && field < 255) {
+        uint32_t field = __reduce_max_sync(kFullMask, largest) >> 23;
+        if (field == 255) {  // a token's NaN, which must not hide the others' size
+          largest = 0;
+#pragma unroll
+          for (int j = 0; j < kJ; ++j) {
+            if (pairs[j][g] << 16 < 0x7f800000u) largest = max(largest, pairs[j][g] << 16);
+          }
+          field = __reduce_max_sync(kFullMask, largest) >> 23;
+        }
+        if (field + 4 - unit[g] > 8 && field != 0) {
           const uint32_t next = min(field, 253u);
           const float ratio = __uint_as_float((254u - next) << 23) * __uint_as_float(unit[g] << 23);
           unit[g] = next;

@@ -353,6 +353,41 @@ class TestAttention:
             assert torch.equal(out.isnan().any(-1), seen)
             assert not bool(seen[0, :, 2:].any()) and not bool(seen[0, :5, :2].any()) and bool(seen[0, 5:, :2].all())
 
+    @pytest.mark.parametrize("size", [1e-12, 1.0, 1e12])
+    def test_values_of_any_size_beside_a_nan(self, size) -> None:
+        """Values far from 1 (binary16 holds neither), the last token's NaN: the earlier rows do not see it."""
+        from pck.cuda import kv4_append, kv4_attention, kv4_cache
+
+        gen = torch.Generator().manual_seed(7)
+        k, v = torch.randn(2, 30, 1, 64, generator=gen)
+        v *= size
+        v[29, 0, 3] = float("nan")
+        cache = kv4_cache(2, 16, 1, 64)
+        kv4_append(cache, k.cuda(), v.cuda(), torch.arange(30, device="cuda"))
+        q = torch.randn(1, 4, 2, 64, generator=gen).bfloat16()
+        table, lens = torch.tensor([[0, 1]], dtype=torch.int32), torch.tensor([30], dtype=torch.int32)
+        out = kv4_attention(q.cuda(), cache, table.cuda(), lens.cuda()).cpu()
+        assert bool(out[0, 3].isnan().all())
+        want, big = ref.attention(q[:, :3], cache.cpu(), table, torch.tensor([29], dtype=torch.int32))
+        tol = UNIT[torch.bfloat16] * want.abs() + (4 * 2.0**-9 + 2.0**-16) * big
+        assert bool(((out[:, :3].double() - want).abs() <= tol).all())
+
+    def test_values_of_changing_size(self) -> None:
+        """The values' scales rise and fall by 2^40 along the tokens, past what one power of two covers."""
+        from pck.cuda import kv4_append, kv4_attention, kv4_cache
+
+        gen = torch.Generator().manual_seed(8)
+        k, v = torch.randn(2, 400, 1, 128, generator=gen)
+        v *= torch.exp2(40 * torch.sin(torch.arange(400) / 20))[:, None, None]
+        cache = kv4_cache(25, 16, 1, 128)
+        kv4_append(cache, k.cuda(), v.cuda(), torch.arange(400, device="cuda"))
+        q = torch.randn(1, 1, 5, 128, generator=gen).half()
+        table, lens = torch.arange(25, dtype=torch.int32)[None], torch.tensor([400], dtype=torch.int32)
+        out = kv4_attention(q.bfloat16().cuda(), cache, table.cuda(), lens.cuda()).cpu()
+        want, big = ref.attention(q.bfloat16(), cache.cpu(), table, lens)
+        tol = UNIT[torch.bfloat16] * want.abs() + (4 * 2.0**-9 + 2.0**-16) * big
+        assert bool(((out.double() - want).abs() <= tol).all())
+
     def test_refusals(self) -> None:
         from pck.cuda import kv4_attention, kv4_cache
 
