@@ -13,8 +13,10 @@
 //   3. out = y + s B h: the CTAs and warps split the outputs m. h enters the products as three (bfloat16)
 //      or two (binary16, scaled by a power of two of its row) terms whose sum is h to binary32's
 //      precision, so nothing is lost against a binary32 product.
-// Bound by the adapters' bytes for decode batches and by x, y and out for prompts; with few rows by the latency of the two dependent passes, which is why a single row
-// is spread over a cluster of eight CTAs.
+// The floor is the adapters' bytes for decode batches and x, y and out for prompts. Few rows are bound by the
+// latency of the two dependent passes (one row of rank 16, 4096 x 4096: 7.2 us), which is why a row is spread
+// over a cluster. Prompts run their passes one after the other (4,099 rows, 14336 to 4096: 80 us against
+// a floor of 39; A x 28 us, x alone at 4.1 TB/s, and the outputs 30 us, y and out at 4.5 TB/s).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -636,6 +638,10 @@ cudaError_t launch_rank(const LoraArgs& a, int tiles, int items, int ctas, cudaS
 }
 
 // Up to 256 rows are taken as a decode batch: as many places for groups as there are rows, a cluster each.
+// Clusters of eight CTAs shorten the two passes while there are SMs for them, four take fewer turns after
+// that (4096 x 4096, 48 adapters of rank 64, us with eight and with four: 1 row 10.7 and 14.6, 32 rows 15.8
+// and 15.5, 64 rows 18.2 and 19.4, 128 rows 29.5 and 21.8; of rank 16: 7.3 and 10.6, 8.7 and 10.5, 10.6
+// and 12.1, 17.7 and 13.5).
 // More are taken as prompts: two items of a tile at a time (it rarely meets more), and as many CTAs an item
 // as run at once; 64 ranks a launch, the later ones adding to out: the sums of 64 rows and more ranks leave
 // an SM one CTA and its registers no room for loads in flight (2,000 rows of rank 100: 145 us so, 135 us in
@@ -643,7 +649,7 @@ cudaError_t launch_rank(const LoraArgs& a, int tiles, int items, int ctas, cudaS
 template <typename T>
 cudaError_t launch_tokens(LoraArgs a, cudaStream_t s) {
   if (a.tokens <= kLoraThreads) {
-    return launch_rank<T, 1>(a, 1, static_cast<int>(a.tokens), a.tokens <= 32 ? 8 : 4, s);
+    return launch_rank<T, 1>(a, 1, static_cast<int>(a.tokens), a.tokens <= 64 ? 8 : 4, s);
   }
   const int tiles = static_cast<int>((a.tokens + 63) / 64);
   int ctas = kLoraMaxCtas;
