@@ -51,7 +51,6 @@ struct LoraArgs {
   int32_t taken;
   int32_t n_vector;   // rows of x and A are 16-byte aligned
   int32_t rank_vector;  // ranks that the rows of B are aligned to: 8, 4 or 0
-  int32_t y_vector;   // rows of y and out are 16-byte aligned
 };
 
 template <typename T>
@@ -195,7 +194,8 @@ __device__ __forceinline__ int64_t staged_steps(const LoraArgs& a, uint8_t* smem
   return k0 + 2 * stages;
 }
 
-template <typename T, int kSub, int kNT>
+// kWhole: rows of y and out are 16-byte aligned.
+template <typename T, int kSub, int kNT, bool kWhole>
 __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(const __grid_constant__ LoraArgs a) {
   using S = LoraShape<kSub, kNT>;
   constexpr int kTerms = std::is_same_v<T, __half> ? 2 : 3;
@@ -470,7 +470,11 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
     }
 
     // 3. The outputs, 32 columns at a time: block j of a product has the columns 8 t + 2 j + e, so a lane
-    // ends with 8 neighbouring ones of its rows.
+    // ends with 8 neighbouring ones of its rows. Where rows are not 16-byte aligned (!kWhole) it has the
+    // columns 4 (2 j + e) + t, so that a load or store of single elements meets neighbouring ones in a quad
+    // (2,000 rows of rank 32, 4096 to 4097: 94 us with a lane's columns neighbouring and their y loaded last,
+    // 54 so; a choice in one kernel instead of two cost the aligned rows 40 to 45 us at 4096 to 4096).
+    const int first = kWhole ? 8 * quarter : quarter;
     // Up to 64 ranks of B for a block. A lane takes neighbouring ranks of its column (16 of 64, 8 of 32, 4
     // of 16), so that a warp's load asks for whole lines of memory: as many 32-byte pieces leave most of
     // the SM's requests in flight empty.
@@ -482,7 +486,8 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
       for (int j = 0; j < 4; ++j) {
         // (Columns past the last take the last one's elements: they are not stored. Ranks past the stored
         // ones take others, which clear_b sets to zero: nothing here waits for a load.)
-        const uint16_t* row = Ba + min(32 * b + 8 * (row8 / 2) + 2 * j + row8 % 2, a.m - 1) * a.rank;
+        const int column = kWhole ? 8 * (row8 / 2) + 2 * j + row8 % 2 : 4 * (2 * j + row8 % 2) + row8 / 2;
+        const uint16_t* row = Ba + min(32 * b + column, a.m - 1) * a.rank;
         const int r = from + 4 * kK * quarter;
 #pragma unroll
         for (int u = 0; u < 4 * kK / kLoad; ++u) {
@@ -518,14 +523,22 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
     };
     // y of this lane's rows and columns; the next block's is on its way during a product.
     auto load_y = [&](int64_t b, float4 (&y)[2][2]) {
-      const int64_t c0 = 32 * b + 8 * quarter;
-      if (a.y_vector && c0 + 8 <= a.m) {
+      const int64_t c0 = 32 * b + first;
+      if (!kWhole || c0 + 8 <= a.m) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if ((active | copied) >> (row8 + 8 * h) & 1u) {
-            const float4* from = reinterpret_cast<const float4*>(a.y + row_of(row8 + 8 * h) * a.y_stride + c0);
-            y[h][0] = from[0];
-            y[h][1] = from[1];
+            const float* from = a.y + row_of(row8 + 8 * h) * a.y_stride + c0;
+            if constexpr (kWhole) {
+              y[h][0] = reinterpret_cast<const float4*>(from)[0];
+              y[h][1] = reinterpret_cast<const float4*>(from)[1];
+            } else {
+              float v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = c0 + 4 * i < a.m ? from[4 * i] : 0.0f;
+              y[h][0] = make_float4(v[0], v[1], v[2], v[3]);
+              y[h][1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
           }
         }
       }
@@ -535,8 +548,8 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
     constexpr bool kAhead = kNT <= 4;  // (the registers of more ranks leave no room for it)
     if (kAhead && m0 + share < m1 && (active | copied)) load_y(m0 + share, yv);
     for (int64_t b = m0 + share; b < m1 && (active | copied); b += S::kSplit) {
-      const int64_t c0 = 32 * b + 8 * quarter;
-      const bool vector = a.y_vector && c0 + 8 <= a.m;
+      const int64_t c0 = 32 * b + first;
+      const bool vector = kWhole && c0 + 8 <= a.m;
       if (active) load_b(b, 0, w);
       if (!kAhead) load_y(b, yv);
       if (kAhead && b + S::kSplit < m1) load_y(b + S::kSplit, next);
@@ -575,6 +588,13 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
             reinterpret_cast<float4*>(out)[i] =
                 make_float4(from.x + v[4 * i], from.y + v[4 * i + 1], from.z + v[4 * i + 2], from.w + v[4 * i + 3]);
           }
+        } else if constexpr (!kWhole) {
+          const float y[8] = {yv[h][0].x, yv[h][0].y, yv[h][0].z, yv[h][0].w,
+                              yv[h][1].x, yv[h][1].y, yv[h][1].z, yv[h][1].w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (c0 + 4 * i < a.m) out[4 * i] = y[i] + v[i];
+          }
         } else {
           const float* y = a.y + row_of(r) * a.y_stride + c0;
 #pragma unroll
@@ -597,7 +617,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
   }
 }
 
-template <typename T, int kSub, int kNT>
+template <typename T, int kSub, int kNT, bool kWhole>
 cudaError_t launch_lora(const LoraArgs& a, int tiles, int items, int ctas, cudaStream_t stream) {
   using S = LoraShape<kSub, kNT>;
   static bool configured[64] = {};
@@ -605,7 +625,7 @@ cudaError_t launch_lora(const LoraArgs& a, int tiles, int items, int ctas, cudaS
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
     const cudaError_t err =
-        cudaFuncSetAttribute(lora_kernel<T, kSub, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        cudaFuncSetAttribute(lora_kernel<T, kSub, kNT, kWhole>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (err != cudaSuccess) return err;
     configured[dev] = true;
   }
@@ -623,18 +643,18 @@ cudaError_t launch_lora(const LoraArgs& a, int tiles, int items, int ctas, cudaS
   config.stream = stream;
   config.attrs = attr;
   config.numAttrs = 2;
-  return cudaLaunchKernelEx(&config, lora_kernel<T, kSub, kNT>, a);
+  return cudaLaunchKernelEx(&config, lora_kernel<T, kSub, kNT, kWhole>, a);
 }
 
-template <typename T, int kSub>
+template <typename T, int kSub, bool kWhole>
 cudaError_t launch_rank(const LoraArgs& a, int tiles, int items, int ctas, cudaStream_t s) {
-  if (a.taken <= 16) return launch_lora<T, kSub, 2>(a, tiles, items, ctas, s);
-  if (a.taken <= 32) return launch_lora<T, kSub, 4>(a, tiles, items, ctas, s);
+  if (a.taken <= 16) return launch_lora<T, kSub, 2, kWhole>(a, tiles, items, ctas, s);
+  if (a.taken <= 32) return launch_lora<T, kSub, 4, kWhole>(a, tiles, items, ctas, s);
   if constexpr (kSub == 1) {
-    if (a.taken > 128) return launch_lora<T, kSub, 32>(a, tiles, items, ctas, s);
-    if (a.taken > 64) return launch_lora<T, kSub, 16>(a, tiles, items, ctas, s);
+    if (a.taken > 128) return launch_lora<T, kSub, 32, kWhole>(a, tiles, items, ctas, s);
+    if (a.taken > 64) return launch_lora<T, kSub, 16, kWhole>(a, tiles, items, ctas, s);
   }
-  return launch_lora<T, kSub, 8>(a, tiles, items, ctas, s);
+  return launch_lora<T, kSub, 8, kWhole>(a, tiles, items, ctas, s);
 }
 
 // Up to 256 rows are taken as a decode batch: as many places for groups as there are rows, a cluster each.
@@ -644,19 +664,19 @@ cudaError_t launch_rank(const LoraArgs& a, int tiles, int items, int ctas, cudaS
 // and 12.1, 17.7 and 13.5).
 // More are taken as prompts: two items of a tile at a time (it rarely meets more), and as many CTAs an item
 // as run at once; 64 ranks a launch, the later ones adding to out: the sums of 64 rows and more ranks leave
-// an SM one CTA and its registers no room for loads in flight (2,000 rows of rank 100: 145 us so, 135 us in
+// an SM one CTA and its registers no room for loads in flight (2,000 rows of rank 100: 145 us so, 125 us in
 // two launches).
-template <typename T>
+template <typename T, bool kWhole>
 cudaError_t launch_tokens(LoraArgs a, cudaStream_t s) {
   if (a.tokens <= kLoraThreads) {
-    return launch_rank<T, 1>(a, 1, static_cast<int>(a.tokens), a.tokens <= 64 ? 8 : 4, s);
+    return launch_rank<T, 1, kWhole>(a, 1, static_cast<int>(a.tokens), a.tokens <= 64 ? 8 : 4, s);
   }
   const int tiles = static_cast<int>((a.tokens + 63) / 64);
   int ctas = kLoraMaxCtas;
   while (ctas > 1 && tiles * ctas > 148 * 2) ctas /= 2;
   for (const int all = a.rank; a.rank0 < all; a.rank0 += 64) {
     a.taken = all - a.rank0 < 64 ? all - a.rank0 : 64;
-    if (const cudaError_t err = launch_rank<T, 4>(a, tiles, 2, ctas, s); err != cudaSuccess) return err;
+    if (const cudaError_t err = launch_rank<T, 4, kWhole>(a, tiles, 2, ctas, s); err != cudaSuccess) return err;
     a.y = a.out;
     a.y_stride = a.out_stride;
   }
@@ -705,8 +725,11 @@ extern "C" int pck_lora_add(const pck_lora_desc* desc, void* stream) {
   a.rank = a.taken = static_cast<int32_t>(rank);
   a.n_vector = aligned_to(x, 16) && aligned_to(A, 16) && x_stride % 8 == 0 && n % 8 == 0;
   a.rank_vector = aligned_to(B, 16) && rank % 8 == 0 ? 8 : aligned_to(B, 8) && rank % 4 == 0 ? 4 : 0;
-  a.y_vector = aligned_to(y, 16) && aligned_to(out, 16) && y_stride % 4 == 0 && out_stride % 4 == 0;
+  const bool whole = aligned_to(y, 16) && aligned_to(out, 16) && y_stride % 4 == 0 && out_stride % 4 == 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = dtype == PCK_LOGITS_BF16 ? launch_tokens<__nv_bfloat16>(a, s) : launch_tokens<__half>(a, s);
+  const cudaError_t err =
+      dtype == PCK_LOGITS_BF16
+          ? (whole ? launch_tokens<__nv_bfloat16, true>(a, s) : launch_tokens<__nv_bfloat16, false>(a, s))
+          : (whole ? launch_tokens<__half, true>(a, s) : launch_tokens<__half, false>(a, s));
   return err == cudaSuccess ? PCK_OK : report_cuda("adapter kernel", err);
 }

@@ -81,6 +81,22 @@ class TestLora:
         check(got, args, 256, 16)
         assert torch.equal(got.cpu()[adapters < 0], y[adapters < 0])
 
+    @pytest.mark.parametrize("m", [1, 31, 33, 257])
+    @pytest.mark.parametrize("tokens", [40, 300])
+    def test_rows_whose_outputs_are_not_aligned(self, tokens, m) -> None:
+        """Single elements at the ends of the rows, and rows without an adapter beside them, in place too."""
+        from pck.cuda import lora_add
+
+        x, y, A, B, _, scales, ranks = problem(tokens, 128, m, 3, 40, torch.bfloat16)
+        adapters = torch.tensor([(i // 23) % 4 - 1 for i in range(tokens)], dtype=torch.int32)
+        args = (x, y, A, B, adapters, scales, ranks)
+        on = [t.cuda() for t in args]
+        got = lora_add(*on)
+        check(got, args, 128, 40)
+        assert torch.equal(got.cpu()[adapters < 0], y[adapters < 0])
+        lora_add(*on, out=on[1])
+        assert torch.equal(on[1], got)
+
     @pytest.mark.parametrize("tokens,rank", [(21, 16), (280, 96)])
     def test_strided_rows_in_place_and_unaligned(self, tokens, rank) -> None:
         from pck.cuda import lora_add
