@@ -14,7 +14,7 @@
 //      or two (binary16, scaled by a power of two of its row) terms whose sum is h to binary32's
 //      precision, so nothing is lost against a binary32 product.
 // The floor is the adapters' bytes for decode batches and x, y and out for prompts. Few rows are bound by the
-// latency of the two dependent passes (one row of rank 16, 4096 x 4096: 7.2 us), which is why a row is spread
+// latency of the two dependent passes (one row of rank 16, 4096 x 4096: 7.1 us), which is why a row is spread
 // over a cluster. Prompts run their passes one after the other (4,099 rows, 14336 to 4096: 80 us against
 // a floor of 39; A x 28 us, x alone at 4.1 TB/s, and the outputs 30 us, y and out at 4.5 TB/s).
 #include <cooperative_groups.h>
