@@ -415,7 +415,9 @@ int pck_peer_all_gather(const pck_peer_gather* gather, void* stream);
  * path. Each takes a descriptor (every field 8 bytes wide, read during the call) and a stream.
  * Element types are PCK_LOGITS_F32, _BF16 and _F16. Indices that they read from device
  * memory (slots, pages, adapters, token ids) are checked by the kernels: a page, slot or
- * adapter beyond its range is left out and sets bit 1 of pck_device_status.
+ * adapter beyond its range is left out and sets bit 1 of pck_device_status. Row strides of what
+ * they read (logits, history, mask, x, y, page table) are 0, the same row for all, or at least a
+ * row; those of `out` are at least a row.
  *
  * The 4-bit cache: `cache` is (pages, kv_heads, page_tiles, 18 * dim) bytes, contiguous and
  * 16-byte aligned, dim 64, 128 or 256. A page holds 16 * page_tiles tokens of every head. A tile
@@ -486,7 +488,7 @@ int pck_kv4_attention(const pck_kv4_attention_desc* desc, void* stream);
  * Low-rank adapters of many requests beside a shared projection: out = y + s_a B_a (A_a x) for
  * every row, a = adapters[row] (negative: none, out = y). x (tokens, n) bfloat16 or float16, A
  * (count, rank, n) and B (count, m, rank) contiguous of x's type, y and out (tokens, m) binary32
- * (out may be y). scales (count) may be NULL (1); ranks (count) gives each adapter's own rank in
+ * (out may be y, with its stride). scales (count) may be NULL (1); ranks (count) gives each adapter's own rank in
  * [0, rank] (the rest of A and B is not used) or is NULL. rank in [1, 256]. The intermediate A x is
  * held in binary32.
  */
@@ -508,7 +510,7 @@ typedef struct pck_lora_desc {
 int pck_lora_add(const pck_lora_desc* desc, void* stream);
 
 /*
- * Logits (rows, vocab) of `dtype` to binary32 `out` (which may be the logits), in this order, each
+ * Logits (rows, vocab) of `dtype` to binary32 `out` (which may be the logits, with their stride), in this order, each
  * step one binary32 operation:
  *   repetition: l > 0 ? l / r : l * r for tokens in the row's history;
  *   frequency:  l - f * (times put out) for tokens that were put out;

@@ -1098,7 +1098,7 @@ extern "C" int pck_kv4_attention(const pck_kv4_attention_desc* desc, void* strea
     return report_error(PCK_ERR_ARGUMENT, "attention: need batch >= 0, queries in [1, 32767] and heads a multiple of kv_heads");
   }
   if (pages < 0 || pages > 0x7fffffff || page_tiles < 1 || page_tiles > 0x7fffff || table_pages < 0 || table_pages > 0x7fffffff ||
-      table_stride < table_pages) {
+      !rows_apart(table_stride, table_pages)) {
     return report_error(PCK_ERR_ARGUMENT, "attention: need pages >= 0, page_tiles >= 1 and a page table of whole rows");
   }
   if (window < 0) return report_error(PCK_ERR_ARGUMENT, "attention: window must be 0 (none) or positive");

@@ -224,17 +224,17 @@ extern "C" int pck_process_logits(const pck_logits_desc* desc, void* stream) {
   if (dtype != PCK_LOGITS_F32 && dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) {
     return report_error(PCK_ERR_ARGUMENT, "logits: unknown dtype");
   }
-  if (rows < 0 || rows > 0x7fffffffLL || vocab < 1 || vocab > 0x7fffffffLL || row_stride < vocab || out_stride < vocab) {
+  if (rows < 0 || rows > 0x7fffffffLL || vocab < 1 || vocab > 0x7fffffffLL || !rows_apart(row_stride, vocab) || out_stride < vocab) {
     return report_error(PCK_ERR_ARGUMENT, "logits: need rows >= 0, vocab in [1, 2^31) and strides of whole rows");
   }
-  if (tokens && (!lengths || max_tokens < 0 || token_stride < max_tokens)) {
+  if (tokens && (!lengths || max_tokens < 0 || !rows_apart(token_stride, max_tokens))) {
     return report_error(PCK_ERR_ARGUMENT, "logits: a history needs lengths and a stride of whole rows");
   }
   if (!tokens && (repetition || frequency || presence)) return report_error(PCK_ERR_ARGUMENT, "logits: penalties need a history");
   if (bias_starts && (biases < 0 || biases > 0x7fffffffLL || (biases > 0 && (!bias_ids || !bias_values)))) {
     return report_error(PCK_ERR_ARGUMENT, "logits: biases need ids and values");
   }
-  if (mask && mask_stride < (vocab + 31) / 32) return report_error(PCK_ERR_ARGUMENT, "logits: a mask row has ceil(vocab / 32) words");
+  if (mask && !rows_apart(mask_stride, (vocab + 31) / 32)) return report_error(PCK_ERR_ARGUMENT, "logits: a mask of whole rows has ceil(vocab / 32) words");
   if (rows == 0) return PCK_OK;
   if (!logits || !out) return report_error(PCK_ERR_ARGUMENT, "logits: NULL logits or out");
   const int32_t in_place = out == logits && out_stride == row_stride && dtype == PCK_LOGITS_F32;

@@ -697,7 +697,8 @@ extern "C" int pck_lora_add(const pck_lora_desc* desc, void* stream) {
   if (dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) {
     return report_error(PCK_ERR_ARGUMENT, "adapters: x must be bfloat16 or float16");
   }
-  if (tokens < 0 || tokens > 1 << 30 || n < 1 || m < 0 || x_stride < n || y_stride < m || out_stride < m) {
+  if (tokens < 0 || tokens > 1 << 30 || n < 1 || m < 0 || !rows_apart(x_stride, n) || !rows_apart(y_stride, m) ||
+      out_stride < m) {
     return report_error(PCK_ERR_ARGUMENT, "adapters: need tokens >= 0, n >= 1, m >= 0 and strides of whole rows");
   }
   if (count < 0 || count > 0x7fffffffLL) return report_error(PCK_ERR_ARGUMENT, "adapters: bad number of adapters");

@@ -26,6 +26,9 @@ inline int report_cuda(const char* what, cudaError_t err) {
   return report_error(PCK_ERR_CUDA, msg);
 }
 
+// Row strides of an input: rows of their own, or one row for all.
+inline bool rows_apart(int64_t stride, int64_t width) { return stride >= width || stride == 0; }
+
 inline bool aligned_to(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 __device__ __forceinline__ float to_float(float v) { return v; }

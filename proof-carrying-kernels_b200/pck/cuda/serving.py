@@ -53,6 +53,12 @@ def _per_row(t: torch.Tensor | None, name: str, dtype: torch.dtype, index: int, 
     return _tensor(t, name, dtype, index)
 
 
+def _row_stride(stride: int, rows: int, width: int) -> int:
+    """What the library is told of a row stride: the tensor's own (0 for expanded rows, which the kernels
+    read as they are; it refuses rows that overlap in part), but a whole row where there is only one."""
+    return stride if rows > 1 else width
+
+
 def _index(t: torch.Tensor, name: str) -> int:
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
@@ -206,7 +212,7 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
     scratch = cache.new_empty((size,)) if size > 0 else None
     _call("pck_kv4_attention", index, _lib.KV4_ATTENTION.pack(
         q.data_ptr(), code, batch, queries, heads, dim, qb, qt, qh, cache.data_ptr(), pages, kv_heads, tiles,
-        page_table.data_ptr(), table_stride if table_stride > table_pages else table_pages, table_pages,
+        page_table.data_ptr(), _row_stride(table_stride, batch, table_pages), table_pages,
         _tensor(lengths, "lengths", torch.int32, index), dim**-0.5 if scale is None else scale, window,
         _tensor(out, "out", dtype, index), 0 if scratch is None else scratch.data_ptr(), size))  # fmt: skip
     return out
@@ -259,10 +265,10 @@ def lora_add(x: torch.Tensor, y: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
         if (not same and _overlaps(out, y)) or any(_overlaps(out, t) for t in (x, A, B, adapters)):
             raise RuntimeError("out must be y itself or share no memory with the inputs")
     _call("pck_lora_add", index, _lib.LORA.pack(
-        x.data_ptr(), code, tokens, n, x_stride if x_stride > n else n, y.data_ptr(), m, y_stride if y_stride > m else m,
+        x.data_ptr(), code, tokens, n, _row_stride(x_stride, tokens, n), y.data_ptr(), m, _row_stride(y_stride, tokens, m),
         _tensor(A, "A", dtype, index), _tensor(B, "B", dtype, index), count, rank,
         _per_row(adapters, "adapters", torch.int32, index, tokens), _per_row(scales, "scales", torch.float32, index, count),
-        _per_row(ranks, "ranks", torch.int32, index, count), out.data_ptr(), out_stride if out_stride > m else m))  # fmt: skip
+        _per_row(ranks, "ranks", torch.int32, index, count), out.data_ptr(), _row_stride(out_stride, tokens, m)))  # fmt: skip
     return out
 
 
@@ -309,8 +315,7 @@ def process_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, 
             raise RuntimeError("tokens must have unit column stride")
         if lengths is None:
             raise RuntimeError("tokens need lengths")
-        if history_stride < most:
-            history_stride = most
+        history_stride = _row_stride(history_stride, rows, most)
         prompts = _per_row(prompt_lengths, "prompt_lengths", torch.int32, index, rows)
         counts = _per_row(lengths, "lengths", torch.int32, index, rows)
         rep = _per_row(repetition, "repetition", torch.float32, index, rows)
@@ -345,7 +350,7 @@ def process_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, 
         mask_stride, column = mask.stride()
         if words > 1 and column != 1:
             raise RuntimeError("mask must have unit column stride")
-        mask_ptr, mask_stride = mask.data_ptr(), mask_stride if mask_stride > words else words
+        mask_ptr, mask_stride = mask.data_ptr(), _row_stride(mask_stride, rows, words)
     if out is None:
         out = torch.empty_like(logits, dtype=torch.float32, memory_format=_CONTIGUOUS)
         out_stride = vocab
@@ -359,10 +364,9 @@ def process_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, 
         inputs = [t for t in (tokens, bias_ids, bias_values, mask) if t is not None]
         if (not same and _overlaps(out, logits)) or any(_overlaps(out, t) for t in inputs):
             raise RuntimeError("out must be the logits themselves or share no memory with the inputs")
-        if out_stride < vocab:
-            out_stride = vocab
+        out_stride = _row_stride(out_stride, rows, vocab)
     _call("pck_process_logits", index, _lib.LOGITS.pack(
-        logits.data_ptr(), code, rows, vocab, stride if stride > vocab else vocab, history, history_stride, most, prompts, counts,
+        logits.data_ptr(), code, rows, vocab, _row_stride(stride, rows, vocab), history, history_stride, most, prompts, counts,
         rep, freq, pres, starts, ids, amounts, biases, mask_ptr, mask_stride, out.data_ptr(), out_stride))  # fmt: skip
     return out
 
