@@ -19,11 +19,13 @@
 //     and for the values the weight p s of a token and group goes into the matrix product instead
 //     of p; sum of p z is added at the end.
 //   - Scores and sums are binary32. The weights p s are rounded to binary16 (11 bits, below the
-//     rounding of a bfloat16 output): they are first divided by a power of two that follows the
-//     size of the values' scales, so neither large nor small scales leave binary16's range.
-//   - The running maximum is raised only when a score passes it by 2^8 (weights then stay within
-//     2^8, which binary16 and the sums hold), so the accumulators are rarely rescaled and the
-//     common tile needs no exchange between lanes for it.
+//     rounding of a bfloat16 output), each row's and group's times a power of two that follows the
+//     largest p s met so far: that one lies in 2 to 2^15, so what the smallest lose is at most 2^-26
+//     of it. The size of a scale whose token has no weight is of no account.
+//   - The running maximum is a whole number (of log2) and is raised only when a score passes it by
+//     2^8 (weights then stay within 2^8), so the accumulators are rarely rescaled and the common
+//     tile needs no exchange between lanes for it. Raising it lowers all p s met so far, and with
+//     them the power of two, by the same factor: the products with the values stay as they are.
 //   - Work is cut by the lengths, on the device. With few (request, head, row block) items a CTA takes
 //     an equal piece of one of them; with many, the tiles of all items form one line that is cut into
 //     equal parts, a CTA each, so one long request among short ones takes no longer than the rest. A
@@ -50,6 +52,8 @@ constexpr int kItemCost = 8;
 constexpr int kMinPiece = 8;  // tiles of a piece of an item, at least: two for each warp
 constexpr int kMinPart = 16;  // length of a part, at least
 constexpr float kRaise = 8.0f;      // log2 by which a score may pass the running maximum
+constexpr int kUnitBias = 127;      // of a power of two's exponent field
+constexpr int kUnitMost = 245;      // field of a row's largest unit, 2^118: times a weight it stays finite
 constexpr int kJoinRows = 4;     // rows of a joining CTA, four warps each
 constexpr int kJoinThreads = kJoinRows * 4 * kWarp;
 
@@ -144,6 +148,17 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 }
 
 __device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+
+// 2^n, zero below binary32's normal range; n <= 127.
+__device__ __forceinline__ float power(int n) {
+  return n >= 1 - kUnitBias ? __uint_as_float(static_cast<uint32_t>(n + kUnitBias) << 23) : 0.0f;
+}
+
+// The exponent field of one of two positive bfloat16 numbers, and another for it (with a mantissa of 0).
+__device__ __forceinline__ int unit_field(uint32_t units, int e) { return static_cast<int>(units >> (16 * e + 7) & 255u); }
+__device__ __forceinline__ void set_unit_field(uint32_t& units, int e, int field) {
+  units = (units & 0xffff0000u >> 16 * e) | static_cast<uint32_t>(field) << (16 * e + 7);
+}
 
 // (w & mask) | bits in one instruction: both constants come in registers.
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
@@ -595,7 +610,12 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     // The running maximum (log2; 0 while there is none) and the score that raises it (-inf while there
     // is none).
     float top[kN][2], limit[kN][2];
-    uint32_t unit[kG];  // exponent field of the power of two that the values' weights are divided by
+    // The power of two by which a row's weights of the values are multiplied, as bfloat16 for two rows, and
+    // the largest of them.
+    uint32_t unit[kN][kG];
+    float unit_most[kG];
+#pragma unroll
+    for (int g = 0; g < kG; ++g) unit_most[g] = power(kUnitMost - kUnitBias);
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
@@ -606,18 +626,20 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
         zeros[n][g][0] = zeros[n][g][1] = 0.0f;
+        unit[n][g] = kUnitMost << 23 | kUnitMost << 7;
 #pragma unroll
         for (int m = 0; m < 4; ++m) acc[n][g][m][0] = acc[n][g][m][1] = acc[n][g][m][2] = acc[n][g][m][3] = 0.0f;
       }
     }
-#pragma unroll
-    for (int g = 0; g < kG; ++g) unit[g] = 127;
 
+    bool first = true;  // no stage yet
     // One stage. This lane's tokens are row8 + 8 j. kMasked: some row does not see some of them, or
     // a tile is missing.
     constexpr int kJ = 2 * kStage;
     auto stage_step = [&](const uint8_t* stage, int token0, uint32_t gone, auto masked_tag) {
       constexpr bool kMasked = decltype(masked_tag)::value;
+      const bool fresh = first;
+      first = false;
       float s[kN][kJ][2];  // element [j][e]: token row8 + 8 j, row 2 quarter + e
       bool off[kN][kJ][2];
 #pragma unroll
@@ -699,21 +721,28 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
             for (int j = 1; j < kJ; ++j) m = fmaxf(m, s[n][j][e]);
             const float old = limit[n][e] == -INFINITY ? -INFINITY : top[n][e];
-            m = fmaxf(old, m * factor[n][e]);
+            m = fmaxf(old, ceilf(m * factor[n][e]));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 4));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16));
-            const float keep = old == m ? 1.0f : exp2_fast(old - m);
             top[n][e] = m == -INFINITY ? 0.0f : m;
             limit[n][e] = (m + kRaise) / factor[n][e];
+            if (fresh) continue;  // the sums are zeros
+            // How far it rises (0 without a maximum; more than any product has bits is as good as all).
+            const int by = min(__float2int_rn(m - old), 512);
+            const float keep = power(-by);
             total_w[n][e] *= keep;
 #pragma unroll
             for (int g = 0; g < kG; ++g) {
               zeros[n][g][e] *= keep;
+              const int field = unit_field(unit[n][g], e), next = min(field + by, kUnitMost);
+              set_unit_field(unit[n][g], e, next);
+              unit_most[g] = fmaxf(unit_most[g], power(next - kUnitBias));
+              const float rest = power(next - field - by);  // 1 but where the unit can grow no further
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                acc[n][g][i][e] *= keep;
-                acc[n][g][i][e + 2] *= keep;
+                acc[n][g][i][e] *= rest;
+                acc[n][g][i][e + 2] *= rest;
               }
             }
           }
@@ -742,33 +771,53 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
           }
         }
       }
+      // Weights are up to 2^8: where a scale is up to 2^7 in the largest unit, no product leaves binary16.
+      bool outgrown = false;
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
-        // Keep the largest scale within 2^4 of the unit.
         uint32_t largest = 0;
 #pragma unroll
         for (int j = 0; j < kJ; ++j) largest = max(largest, pairs[j][g] << 16);
-        uint32_t field = __reduce_max_sync(kFullMask, largest) >> 23;
-        if (field == 255) {  // a token's NaN, which must not hide the others' size
-          largest = 0;
+        outgrown = outgrown || !(__uint_as_float(largest) * unit_most[g] <= 128.0f);  // (or a NaN)
+      }
+      if (__any_sync(kFullMask, outgrown)) {
+        // The units that the stage's products have really outgrown: one whose largest is 2^4 or more in it
+        // has it at 2 to 4 after that.
 #pragma unroll
-          for (int j = 0; j < kJ; ++j) {
-            if (pairs[j][g] << 16 < 0x7f800000u) largest = max(largest, pairs[j][g] << 16);
-          }
-          field = __reduce_max_sync(kFullMask, largest) >> 23;
-        }
-        if (field + 4 - unit[g] > 8 && field != 0) {
-          const uint32_t next = min(field, 253u);
-          const float ratio = __uint_as_float((254u - next) << 23) * __uint_as_float(unit[g] << 23);
-          unit[g] = next;
+        for (int g = 0; g < kG; ++g) {
+          int most = 0;
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
+            // Exponent fields of the two rows' largest products, times 2^-10, so that no weight of up to 2^8
+            // overflows them.
+            float largest[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
+            for (int j = 0; j < kJ; ++j) {
+              const float scale = bf16_lo(pairs[j][g]) * power(-10);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[n][g][m][e] *= ratio;
+              for (int e = 0; e < 2; ++e) {
+                if (!kMasked || !off[n][j][e]) largest[e] = fmaxf(largest[e], s[n][j][e] * scale);
+              }
+            }
+            uint32_t sizes = __byte_perm(__float_as_uint(largest[0]), __float_as_uint(largest[1]), 0x7632);
+            sizes = __vmaxu2(sizes, __shfl_xor_sync(kFullMask, sizes, 4));
+            sizes = __vmaxu2(sizes, __shfl_xor_sync(kFullMask, sizes, 8));
+            sizes = __vmaxu2(sizes, __shfl_xor_sync(kFullMask, sizes, 16));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int size = unit_field(sizes, e) - kUnitBias + 10, field = unit_field(unit[n][g], e);
+              const int next = size + field - kUnitBias >= 4 ? max(1 - size + kUnitBias, 1) : field;
+              set_unit_field(unit[n][g], e, next);
+              most = max(most, next);
+              const float ratio = power(next - field);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                acc[n][g][i][e] *= ratio;
+                acc[n][g][i][e + 2] *= ratio;
+              }
             }
           }
+          unit_most[g] = power(most - kUnitBias);
         }
       }
 #pragma unroll
@@ -789,14 +838,13 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
             for (int j = 0; j < 2; ++j) {
               const uint32_t pair = pairs[2 * u + j][g];
               const float scale = bf16_lo(pair), zero = fmaf(8.0f, scale, bf16_hi(pair));
-              const float unit_scale = scale * __uint_as_float((254u - unit[g]) << 23);
 #pragma unroll
               for (int n = 0; n < kN; ++n) {
                 float x[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   const float weight = s[n][2 * u + j][e];
-                  x[e] = weight * unit_scale;
+                  x[e] = weight * (e ? bf16_hi(unit[n][g]) : bf16_lo(unit[n][g])) * scale;
                   if constexpr (kMasked) {  // a NaN scale must not reach rows that do not see its token
                     if (off[n][2 * u + j][e]) {
                       x[e] = 0.0f;
@@ -860,7 +908,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
         for (int g = 0; g < kG; ++g) {
           float z = zeros[n][g][e];
           for (int o = 4; o < kWarp; o <<= 1) z += __shfl_xor_sync(kFullMask, z, o);
-          const float u = __uint_as_float(unit[g] << 23);
+          const float u = power(kUnitBias - unit_field(unit[n][g], e));
           float4* to = reinterpret_cast<float4*>(sums + (warp * kRows + r) * kDim + g * kKv4Group + 8 * row8);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
