@@ -555,8 +555,12 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       const uint32_t largest = __float_as_uint(unpack_pair<T>(max(packed & 0xffffu, packed >> 16)).x);
       uint32_t field = largest >> 23;
       field = field == 0 || field == 255 ? 131 : min(max(field, 8u), 250u);
-      const float scale = __uint_as_float((258u - field) << 23);
-      const float back = a.scale_log2 * __uint_as_float((field - 4u) << 23);
+      float scale = __uint_as_float((258u - field) << 23);
+      float back = a.scale_log2 * __uint_as_float((field - 4u) << 23);
+      if (back < 0x1p-126f) {  // below binary32's normal numbers: scores of 0 (a factor of 0 would make NaN of -inf)
+        scale = 0.0f;
+        back = 1.0f;
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         factor[n][e] = __shfl_sync(kFullMask, back, (2 * quarter + e) * 4);
