@@ -250,6 +250,9 @@ extern "C" int pck_kv4_append(const pck_kv4_append_desc* desc, void* stream) {
   if (pages < 0 || kv_heads < 1 || kv_heads > 0x3fff || page_tiles < 1 || page_tiles > 0x7fffffff || tokens < 0) {
     return report_error(PCK_ERR_ARGUMENT, "append: need pages >= 0, kv_heads in [1, 16383], page_tiles >= 1 and tokens >= 0");
   }
+  if (pages > (int64_t{1} << 62) / (kv_heads * kv4_tile_bytes(static_cast<int>(dim))) / page_tiles) {
+    return report_error(PCK_ERR_UNSUPPORTED, "append: a cache holds at most 2^62 bytes");
+  }
   if (dtype != PCK_LOGITS_F32 && dtype != PCK_LOGITS_BF16 && dtype != PCK_LOGITS_F16) {
     return report_error(PCK_ERR_ARGUMENT, "append: unknown dtype");
   }
