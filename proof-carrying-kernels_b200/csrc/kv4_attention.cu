@@ -38,6 +38,7 @@
 #include <algorithm>
 
 #include "kv4_layout.cuh"
+#include "kv4_ring.h"
 #include "serving_common.cuh"
 
 namespace pck {
@@ -456,7 +457,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
   const Masks masks{kept(0x000f000fu), kept(0x00f000f0u), kept(0x64006400u)};
   uint8_t* const ring = smem + warp * S::kSlots * S::kStageBytes;
   uint32_t phase = 0;  // parity bit of each slot
-  bool dead = false;   // a wait gave up
+  bool dead = false;   // a wait gave up: this warp takes no more tiles
   while (true) {
     __syncthreads();
     if (segment.count == 0) return;
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     const int rows = a.queries * a.group;
     // The warp's stages: kStage tiles each, every kAttnWarps-th.
     const int stages = max(0, hi - lo + kStage - 1) / kStage;
-    const int warp_stages = (max(0, stages - warp) + kAttnWarps - 1) / kAttnWarps;
+    const int warp_stages = dead ? 0 : (max(0, stages - warp) + kAttnWarps - 1) / kAttnWarps;
 
     // Where the tiles lie in the cache: those of 16 stages are looked up at once, a lane each, one
     // batch ahead of their use; -1 without a page or past the end.
@@ -876,12 +877,14 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
     };
 
-    int slot = 0;
-    for (int k = 0; k < warp_stages; ++k) {
-      if (!dead) dead = !__all_sync(kFullMask, mbar_wait(&full[warp][slot], phase >> slot & 1u));
+    auto wait = [&](int slot) {
+      const bool landed = __all_sync(kFullMask, mbar_wait(&full[warp][slot], phase >> slot & 1u));
       phase ^= 1u << slot;
+      return landed;
+    };
+    auto use = [&](int k, int slot) {
       const uint32_t gone = missing >> slot * kStage & kNone;
-      if (gone != kNone && !dead) {
+      if (gone != kNone) {
         const uint8_t* stage = ring + slot * S::kStageBytes;
         const int token0 = (lo + kStage * (warp + k * kAttnWarps)) * kKv4Tile;
         if (gone == 0 && token0 + kStage * kKv4Tile - 1 <= segment.pos0 &&
@@ -892,9 +895,8 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
         }
       }
       __syncwarp();
-      if (k + S::kSlots < warp_stages && !dead) issue(k + S::kSlots, slot);
-      slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-    }
+    };
+    dead |= !take_stages<S::kSlots>(warp_stages, wait, use, issue);
 
     // Join the warps: their sums in shared memory (over the rings, which are empty now), then a
     // thread for each element.
