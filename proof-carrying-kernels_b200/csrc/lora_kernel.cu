@@ -576,30 +576,32 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
         const int r = row8 + 8 * h;
         const bool on = active >> r & 1u;
         if (!on && !(copied >> r & 1u)) continue;
-        const float by = on && rank > 0 ? unit[16 * sub + r] : 0.0f;
+        const bool adds = on && rank > 0;  // the other rows are y, bit for bit
+        const float by = adds ? unit[16 * sub + r] : 0.0f;
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = on && rank > 0 ? acc[i / 2][2 * h + i % 2] * by : 0.0f;
+        for (int i = 0; i < 8; ++i) v[i] = acc[i / 2][2 * h + i % 2] * by;
+        auto sum = [&](float y, int i) { return adds ? y + v[i] : y; };
         float* out = a.out + row_of(r) * a.out_stride + c0;
         if (vector) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float4 from = yv[h][i];
             reinterpret_cast<float4*>(out)[i] =
-                make_float4(from.x + v[4 * i], from.y + v[4 * i + 1], from.z + v[4 * i + 2], from.w + v[4 * i + 3]);
+                make_float4(sum(from.x, 4 * i), sum(from.y, 4 * i + 1), sum(from.z, 4 * i + 2), sum(from.w, 4 * i + 3));
           }
         } else if constexpr (!kWhole) {
           const float y[8] = {yv[h][0].x, yv[h][0].y, yv[h][0].z, yv[h][0].w,
                               yv[h][1].x, yv[h][1].y, yv[h][1].z, yv[h][1].w};
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            if (c0 + 4 * i < a.m) out[4 * i] = y[i] + v[i];
+            if (c0 + 4 * i < a.m) out[4 * i] = sum(y[i], i);
           }
         } else {
           const float* y = a.y + row_of(r) * a.y_stride + c0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            if (c0 + i < a.m) out[i] = y[i] + v[i];
+            if (c0 + i < a.m) out[i] = sum(y[i], i);
           }
         }
       }
