@@ -10,9 +10,11 @@
 //      a warp reads them twice;
 //   2. the warps' and then the CTAs' partial sums are added in a fixed order, through shared and
 //      distributed shared memory: h stays in binary32;
-//   3. out = y + s B h: the CTAs and warps split the outputs m. h enters the products as three (bfloat16)
-//      or two (binary16, scaled by a power of two of its row) terms whose sum is h to binary32's
-//      precision, so nothing is lost against a binary32 product.
+//   3. out = y + s B h: the CTAs and warps split the outputs m. h enters the products as three bfloat16
+//      terms whose sum is h, or as two binary16 ones of h times a power of two of its row, the second
+//      times 2^12 beside it: 23 of its 24 bits for elements down to 2^-29 of the row's largest one, and of
+//      smaller ones what is above 2^-51 of that. (The sums go by 2^12 around the second term's products,
+//      which costs no bit.)
 // The floor is the adapters' bytes for decode batches and x, y and out for prompts. Few rows are bound by the
 // latency of the two dependent passes (one row of rank 16, 4096 x 4096: 7.1 us), which is why a row is spread
 // over a cluster. Prompts run their passes one after the other (4,099 rows, 14336 to 4096: 80 us against
@@ -199,6 +201,7 @@ template <typename T, int kSub, int kNT, bool kWhole>
 __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(const __grid_constant__ LoraArgs a) {
   using S = LoraShape<kSub, kNT>;
   constexpr int kTerms = std::is_same_v<T, __half> ? 2 : 3;
+  constexpr float kTermUnit = std::is_same_v<T, __half> ? 4096.0f : 1.0f;  // of the second term
   extern __shared__ __align__(16) uint8_t smem[];
   float* const part = reinterpret_cast<float*>(smem);              // [split][row][rank]
   uint16_t* const terms = reinterpret_cast<uint16_t*>(smem);       // [term][row][stride]
@@ -441,15 +444,15 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
         for (int i = 0; i < kPer; ++i) {
           const int c = i * kWarp + lane;
           h[i] = c < rank ? whole[r * S::kR + c] * scale : 0.0f;
-          largest = fmaxf(largest, fabsf(h[i]));
+          if (isfinite(h[i])) largest = fmaxf(largest, fabsf(h[i]));
         }
         float down = 1.0f;
-        if constexpr (std::is_same_v<T, __half>) {  // the row's largest between 1 and 2
+        if constexpr (std::is_same_v<T, __half>) {  // the row's largest finite one between 2^14 and 2^15
           for (int o = 16; o; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(kFullMask, largest, o));
           uint32_t field = __float_as_uint(largest) >> 23;
-          field = field == 0 || field == 255 ? 127 : min(field, 253u);
-          down = __uint_as_float((254u - field) << 23);
-          if (lane == 0) unit[r] = __uint_as_float(field << 23);
+          field = field == 0 ? 127 : max(field, 15u);
+          down = __uint_as_float((268u - field) << 23);
+          if (lane == 0) unit[r] = __uint_as_float((field - 14u) << 23);
         } else {
           if (lane == 0) unit[r] = 1.0f;
         }
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
           for (int t = 0; t < kTerms; ++t) {
             const T x = from_float<T>(v);
             terms[(t * S::kM + r) * S::kStride + c] = *reinterpret_cast<const uint16_t*>(&x);
-            v = isfinite(v) ? v - to_float(x) : 0.0f;
+            v = isfinite(v) ? (v - to_float(x)) * kTermUnit : 0.0f;
           }
         }
       }
@@ -559,16 +562,25 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
       for (int k0 = 0; k0 < rank && active; k0 += 16 * kK) {
         if (k0 > 0) load_b(b, k0, w);
         clear_b(k0, w);
+        auto times = [&](float by) {
 #pragma unroll
-        for (int k = 0; k < kK; ++k) {
+          for (int j = 0; j < 4; ++j) {
 #pragma unroll
-          for (int t = 0; t < kTerms; ++t) {
+            for (int i = 0; i < 4; ++i) acc[j][i] *= by;
+          }
+        };
+        if (kTermUnit != 1.0f && k0 > 0) times(kTermUnit);
+#pragma unroll
+        for (int t = kTerms - 1; t >= 0; --t) {
+#pragma unroll
+          for (int k = 0; k < kK; ++k) {
             const uint16_t* from = terms + (t * S::kM + 16 * sub + row8) * S::kStride + k0 + 4 * kK * quarter + 4 * k;
             const uint2 x0 = *reinterpret_cast<const uint2*>(from);
             const uint2 x1 = *reinterpret_cast<const uint2*>(from + 8 * S::kStride);
 #pragma unroll
             for (int j = 0; j < 4; ++j) lora_mma<T>(acc[j], x0.x, x1.x, x0.y, x1.y, w[j][2 * k], w[j][2 * k + 1]);
           }
+          if (kTermUnit != 1.0f && t == 1) times(1.0f / kTermUnit);
         }
       }
 #pragma unroll
