@@ -69,6 +69,17 @@ __device__ __forceinline__ void lora_mma(float (&d)[4], uint32_t a0, uint32_t a1
   }
 }
 
+// The first of the terms that an element becomes: cut off in bfloat16, whose rounding would make an
+// infinity of the largest binary32 numbers (the terms after it hold the rest all the same).
+template <typename T>
+__device__ __forceinline__ T first_term(float v) {
+  if constexpr (std::is_same_v<T, __half>) {
+    return __float2half_rn(v);
+  } else {
+    return __float2bfloat16_rz(v);
+  }
+}
+
 // Elements [at, at + kN) of a row of 16-bit elements, zeros from `end` on. A row holds `held` >= end
 // elements, a multiple of kN where `vector` is set; all loads are issued before any is waited for.
 template <int kN>
@@ -463,7 +474,7 @@ __global__ void __launch_bounds__(kLoraThreads, kNT <= 8 ? 2 : 1) lora_kernel(co
           float v = h[i] * down;
 #pragma unroll
           for (int t = 0; t < kTerms; ++t) {
-            const T x = from_float<T>(v);
+            const T x = t == 0 ? first_term<T>(v) : from_float<T>(v);
             terms[(t * S::kM + r) * S::kStride + c] = *reinterpret_cast<const uint16_t*>(&x);
             v = isfinite(v) ? (v - to_float(x)) * kTermUnit : 0.0f;
           }

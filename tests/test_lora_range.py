@@ -39,6 +39,23 @@ def test_ranks_of_different_sizes(tokens, rank, dtype) -> None:
 
 
 @pytest.mark.parametrize("tokens", [2, 300])
+def test_the_largest_finite_intermediate(tokens) -> None:
+    """A x times the scale rounds up past bfloat16's largest number, but not past binary32's."""
+    from pck.cuda import lora_add
+
+    top = torch.finfo(torch.bfloat16).max
+    x = torch.zeros(tokens, 8, dtype=torch.bfloat16)
+    x[:, 0] = 1.0
+    A = torch.zeros(1, 2, 8, dtype=torch.bfloat16)
+    A[0, 0, 0], A[0, 1, 0] = top, -top
+    B = torch.tensor([[1e-30, 0.0], [0.0, 1e-20], [1e-30, 1e-31]], dtype=torch.bfloat16)[None]
+    args = (x, torch.zeros(tokens, 3), A, B, torch.zeros(tokens, dtype=torch.int32), torch.tensor([1.0035]))
+    got = lora_add(*[t.cuda() for t in args]).cpu().double()
+    want, terms = ref.lora(*args)
+    assert bool(((got - want).abs() <= 2.0**-23 * 18 * terms).all())
+
+
+@pytest.mark.parametrize("tokens", [2, 300])
 def test_an_infinite_rank_beside_finite_ones(tokens) -> None:
     """One rank's product overflows with the scale; the others stay finite, so the sums are infinite, not NaN."""
     from pck.cuda import lora_add
