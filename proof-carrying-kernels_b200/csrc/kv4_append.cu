@@ -52,7 +52,7 @@ struct Raw16 {
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
     } else {
-      T e[16];
+      alignas(16) T e[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) e[i] = from[i];
 #pragma unroll
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 #pragma unroll
     for (int g = 0; g < kWidth; ++g) {
       T* to = values + (token * a.heads + head) * kDim + (plane * kWidth + g) * kKv4Group + 16 * quarter;
-      T e[16];
+      alignas(16) T e[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) e[i] = from_float<T>(v[g][i]);
 #pragma unroll

@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       const int t = r / a.group;
       const T* qr = static_cast<const T*>(a.q) + b * a.q_batch_stride + t * a.q_token_stride +
                     static_cast<int64_t>(kvh * a.group + r % a.group) * a.q_head_stride;
-      uint32_t x[kG][8];
+      alignas(16) uint32_t x[kG][8];
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
         if (r < rows) {
@@ -845,20 +845,20 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
               const float scale = bf16_lo(pair), zero = fmaf(8.0f, scale, bf16_hi(pair));
 #pragma unroll
               for (int n = 0; n < kN; ++n) {
-                float x[2];
+                float product[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   const float weight = s[n][2 * u + j][e];
-                  x[e] = weight * (e ? bf16_hi(unit[n][g]) : bf16_lo(unit[n][g])) * scale;
+                  product[e] = weight * (e ? bf16_hi(unit[n][g]) : bf16_lo(unit[n][g])) * scale;
                   if constexpr (kMasked) {  // a NaN scale must not reach rows that do not see its token
                     if (off[n][2 * u + j][e]) {
-                      x[e] = 0.0f;
+                      product[e] = 0.0f;
                       continue;
                     }
                   }
                   zeros[n][g][e] = fmaf(weight, zero, zeros[n][g][e]);
                 }
-                wf[n][j] = transpose8(half2_bits(__floats2half2_rn(x[0], x[1])));
+                wf[n][j] = transpose8(half2_bits(__floats2half2_rn(product[0], product[1])));
               }
             }
 #pragma unroll

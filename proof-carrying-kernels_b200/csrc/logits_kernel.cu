@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kPassThreads) pass_kernel(const __grid_constan
 // The logits of the tokens in a row's history or biases.
 template <typename T>
 __global__ void __launch_bounds__(kMarkThreads) mark_kernel(const __grid_constant__ LogitsArgs a) {
-  extern __shared__ uint32_t counts[];  // times put out, kInPrompt
+  extern __shared__ __align__(16) uint32_t counts[];  // times put out, kInPrompt
   uint16_t* const listed = reinterpret_cast<uint16_t*>(counts + kMarkSlice);  // tokens with a count
   __shared__ uint32_t met;
   const int tid = threadIdx.x;
