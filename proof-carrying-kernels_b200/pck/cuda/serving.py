@@ -206,8 +206,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
         out = torch.empty_like(q, memory_format=_CONTIGUOUS)
     elif out.shape != shape:
         raise RuntimeError(f"out must have shape {list(shape)}")
-    elif _overlaps(out, q) or _overlaps(out, cache):
-        raise RuntimeError("out must not share memory with q or the cache")
+    elif any(_overlaps(out, t) for t in (q, cache, page_table, lengths)):
+        raise RuntimeError("out must not share memory with the inputs")
     size = _scratch_bytes(index, batch, queries, heads, kv_heads, dim, table_pages * tiles * KV4_TILE)
     scratch = cache.new_empty((size,)) if size > 0 else None
     _call("pck_kv4_attention", index, _lib.KV4_ATTENTION.pack(
@@ -262,7 +262,8 @@ def lora_add(x: torch.Tensor, y: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
         if tokens > 1 and out_stride < m:
             raise RuntimeError("out must not overlap itself")
         same = out.data_ptr() == y.data_ptr() and out.stride() == y.stride()
-        if (not same and _overlaps(out, y)) or any(_overlaps(out, t) for t in (x, A, B, adapters)):
+        inputs = [t for t in (x, A, B, adapters, scales, ranks) if t is not None]
+        if (not same and _overlaps(out, y)) or any(_overlaps(out, t) for t in inputs):
             raise RuntimeError("out must be y itself or share no memory with the inputs")
     _call("pck_lora_add", index, _lib.LORA.pack(
         x.data_ptr(), code, tokens, n, _row_stride(x_stride, tokens, n), y.data_ptr(), m, _row_stride(y_stride, tokens, m),
@@ -361,7 +362,8 @@ def process_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, 
         if (vocab > 1 and column != 1) or (rows > 1 and out_stride < vocab):
             raise RuntimeError("out must have unit column stride and rows of their own")
         same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride() and out.dtype is logits.dtype
-        inputs = [t for t in (tokens, bias_ids, bias_values, mask) if t is not None]
+        inputs = [t for t in (tokens, prompt_lengths, lengths, repetition, frequency, presence, bias_starts, bias_ids, bias_values,
+                              mask) if t is not None]  # fmt: skip
         if (not same and _overlaps(out, logits)) or any(_overlaps(out, t) for t in inputs):
             raise RuntimeError("out must be the logits themselves or share no memory with the inputs")
         out_stride = _row_stride(out_stride, rows, vocab)
