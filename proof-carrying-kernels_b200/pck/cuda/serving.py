@@ -93,6 +93,11 @@ def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _same_rows(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices of one shape are the same memory, row for row."""
+    return a.data_ptr() == b.data_ptr() and a.dtype is b.dtype and (a.shape[0] <= 1 or a.stride() == b.stride())
+
+
 # -- 4-bit key/value cache -------------------------------------------------------------
 
 
@@ -261,7 +266,7 @@ def lora_add(x: torch.Tensor, y: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
         out_stride = out.stride(0)
         if tokens > 1 and out_stride < m:
             raise RuntimeError("out must not overlap itself")
-        same = out.data_ptr() == y.data_ptr() and out.stride() == y.stride()
+        same = _same_rows(out, y)
         inputs = [t for t in (x, A, B, adapters, scales, ranks) if t is not None]
         if (not same and _overlaps(out, y)) or any(_overlaps(out, t) for t in inputs):
             raise RuntimeError("out must be y itself or share no memory with the inputs")
@@ -361,7 +366,7 @@ def process_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, 
         out_stride, column = out.stride()
         if (vocab > 1 and column != 1) or (rows > 1 and out_stride < vocab):
             raise RuntimeError("out must have unit column stride and rows of their own")
-        same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride() and out.dtype is logits.dtype
+        same = _same_rows(out, logits)
         inputs = [t for t in (tokens, prompt_lengths, lengths, repetition, frequency, presence, bias_starts, bias_ids, bias_values,
                               mask) if t is not None]  # fmt: skip
         if (not same and _overlaps(out, logits)) or any(_overlaps(out, t) for t in inputs):

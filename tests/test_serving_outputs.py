@@ -44,3 +44,17 @@ def test_an_output_on_any_input_is_refused(recorded) -> None:  # noqa: F811
         with pytest.raises(RuntimeError, match="out must not share memory"):
             kv4_attention(*args, out=out)
     assert not recorded
+
+
+def test_one_row_in_place_whatever_its_stride(recorded) -> None:  # noqa: F811
+    """The same memory as a single row, written with another stride of rows, is still the input itself."""
+    from pck.cuda import _lib, lora_add, process_logits
+
+    logits = torch.randn(1000)
+    process_logits(logits.as_strided((1, 1000), (1200, 1)), out=logits.view(1, 1000))
+    got = _lib.LOGITS.unpack(recorded["pck_process_logits"])
+    assert got[0] == got[19] and got[4] == got[20] == 1000
+    x, y, *rest = lora_args(tokens=1)
+    lora_add(x, y.as_strided((1, 32), (40, 1)), *rest, out=y)
+    got = _lib.LORA.unpack(recorded["pck_lora_add"])
+    assert got[5] == got[15] and got[7] == got[16] == 32
