@@ -9,12 +9,12 @@
 //     row, and a lane then meets the scales of only two tokens. tcgen05 would want the unpacked codes
 //     written to shared memory first, which alone would exceed its bandwidth at two codes a byte.
 //   - Codes are unpacked to binary16 with a mask and an or, two codes an instruction: the four bits
-//     become mantissa bits of 1024 + n or 1024 + 16 n. Against the keys that excess, the same for
-//     every token, is the start of the product's sum (it costs the binary32 sum 7 of its 24 bits
-//     against the size of a code, far below what the 4 bits lost); the values' codes are brought
-//     to n - 8, exactly, since there it would add up over tokens whose values cancel. Queries become
-//     binary16 scaled by a power of two of their row. Scales never touch the codes: with
-//     k = code * s + z,
+//     become mantissa bits of 1024 + n or 1024 + 16 n, from which one more instruction makes n (keys)
+//     or n - 8 (values, whose sums then cancel less), exactly. Leaving the 1024 in the keys' products and
+//     taking it off their sums saved 3% with 8 rows (two requests of 262,143 tokens 137 and 141 us) but
+//     lost 3% with 16 (148 and 142) and 7 bits of the scores: 1e-5 of an ordinary score where a binary32
+//     dot product, and this one, err by 1e-7. Queries become binary16 scaled by a power of two of their
+//     row. Scales never touch the codes: with k = code * s + z,
 //       q.k = sum over groups of s (q.code) + z sum(q),
 //     and for the values the weight p s of a token and group goes into the matrix product instead
 //     of p; sum of p z is added at the end.
@@ -133,14 +133,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
 }
 
-// The same, from c.
-__device__ __forceinline__ void mma_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         const uint32_t (&b)[2], const float (&c)[4]) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
-}
-
 // Transposes an 8 x 8 matrix of 16-bit elements held two to a lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
@@ -189,10 +181,11 @@ __device__ __forceinline__ void unpack_raw(uint32_t w, const Masks& k, uint32_t 
   out[3] = and_or(w, k.high, k.bits);
 }
 
-// The same as n - 8, exactly.
+// The same as n - kLess, exactly.
+template <int kLess>
 __device__ __forceinline__ void unpack(uint32_t w, const Masks& k, uint32_t (&out)[4]) {
-  const __half2 low = __floats2half2_rn(1032.0f, 1032.0f);
-  const __half2 part = __floats2half2_rn(0.0625f, 0.0625f), high = __floats2half2_rn(-72.0f, -72.0f);
+  const __half2 low = __floats2half2_rn(1024.0f + kLess, 1024.0f + kLess);
+  const __half2 part = __floats2half2_rn(0.0625f, 0.0625f), high = __floats2half2_rn(-64.0f - kLess, -64.0f - kLess);
   unpack_raw(w, k, out);
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
@@ -517,7 +510,6 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
     uint32_t qf[kN][kG * 4][2];
     // What the products' columns belong to: rows 2 quarter and the next of each block.
     float qsum[kN][kG][2];
-    float excess[kN][kG][2];  // what the 1024 beside each code adds to a product, negated
     float factor[kN][2];  // of a score: the softmax's scale (log2) over the row's power of two
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
@@ -568,27 +560,19 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       }
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
-        float even = 0.0f, odd = 0.0f;
+        float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          // Channels that meet 16 n (the odd pairs: 1, 3, 5, 7 of each 8) are divided by 16.
           float2 v = unpack_pair<T>(x[g][i]);
-          const __half2 h = __floats2half2_rn(v.x * scale, v.y * (scale * 0.0625f));
+          const __half2 h = __floats2half2_rn(v.x * scale, v.y * scale);
           x[g][i] = half2_bits(h);
           v = __half22float2(h);
-          even += v.x;
-          odd += v.y;
+          sum += v.x + v.y;
         }
-        even += __shfl_xor_sync(kFullMask, even, 1);
-        even += __shfl_xor_sync(kFullMask, even, 2);
-        odd += __shfl_xor_sync(kFullMask, odd, 1);
-        odd += __shfl_xor_sync(kFullMask, odd, 2);
-        const float sum = fmaf(16.0f, odd, even), held = -1024.0f * (even + odd);
+        sum += __shfl_xor_sync(kFullMask, sum, 1);
+        sum += __shfl_xor_sync(kFullMask, sum, 2);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          qsum[n][g][e] = __shfl_sync(kFullMask, sum, (2 * quarter + e) * 4);
-          excess[n][g][e] = __shfl_sync(kFullMask, held, (2 * quarter + e) * 4);
-        }
+        for (int e = 0; e < 2; ++e) qsum[n][g][e] = __shfl_sync(kFullMask, sum, (2 * quarter + e) * 4);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const uint32_t* y = x[g] + 4 * w;
@@ -665,17 +649,12 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               uint32_t k0[4], k1[4];
-              unpack_raw(w[0][2 * i + c], masks, k0);
-              unpack_raw(w[1][2 * i + c], masks, k1);
+              unpack<0>(w[0][2 * i + c], masks, k0);
+              unpack<0>(w[1][2 * i + c], masks, k1);
 #pragma unroll
               for (int n = 0; n < kN; ++n) {
-                if (c == 0) {
-                  // (several blocks of rows leave no registers for the sums' starts: they are added below)
-                  const float x0 = kN == 1 ? excess[n][g][0] : 0.0f, x1 = kN == 1 ? excess[n][g][1] : 0.0f;
-                  mma_from(part[n], k0[0], k1[0], k0[1], k1[1], qf[n][g * 4], {x0, x1, x0, x1});
-                } else {
-                  mma(part[n], k0[0], k1[0], k0[1], k1[1], qf[n][g * 4 + 2]);
-                }
+                if (c == 0) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.0f;
+                mma(part[n], k0[0], k1[0], k0[1], k1[1], qf[n][g * 4 + 2 * c]);
                 mma(part[n], k0[2], k1[2], k0[3], k1[3], qf[n][g * 4 + 2 * c + 1]);
               }
             }
@@ -688,7 +667,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   float& to = s[n][2 * u + j][e];
-                  const float x = kN == 1 ? part[n][2 * j + e] : part[n][2 * j + e] + excess[n][g][e];
+                  const float x = part[n][2 * j + e];
                   to = g == 0 ? scale * x : fmaf(scale, x, to);
                   to = fmaf(zero, qsum[n][g][e], to);
                 }
@@ -864,8 +843,8 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
               uint32_t v0[4], v1[4];
-              unpack(w[0][2 * i + d], masks, v0);
-              unpack(w[1][2 * i + d], masks, v1);
+              unpack<8>(w[0][2 * i + d], masks, v0);
+              unpack<8>(w[1][2 * i + d], masks, v1);
 #pragma unroll
               for (int n = 0; n < kN; ++n) {
                 mma(acc[n][g][2 * d], v0[0], v0[1], v1[0], v1[1], wf[n]);
