@@ -13,8 +13,8 @@
 //     or n - 8 (values, whose sums then cancel less), exactly. Leaving the 1024 in the keys' products and
 //     taking it off their sums saved 3% with 8 rows (two requests of 262,143 tokens 137 and 141 us) but
 //     lost 3% with 16 (148 and 142) and 7 bits of the scores: 1e-5 of an ordinary score where a binary32
-//     dot product, and this one, err by 1e-7. Queries become binary16 scaled by a power of two of their
-//     row. Scales never touch the codes: with k = code * s + z,
+//     dot product, and this one, err by 1e-7. Queries become binary16 times a power of two of their
+//     row, which loses nothing. Scales never touch the codes: with k = code * s + z,
 //       q.k = sum over groups of s (q.code) + z sum(q),
 //     and for the values the weight p s of a token and group goes into the matrix product instead
 //     of p; sum of p z is added at the end.
@@ -535,8 +535,9 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
           for (int i = 0; i < 8; ++i) x[g][i] = 0;
         }
       }
-      // The row as binary16, its largest element between 16 and 32 by a power of two (rows of zeros,
-      // infinities or NaN as they are): what is lost of small elements is below 2^-25 of the largest.
+      // The row as binary16, its largest element between 2^15 and 2^16 by a power of two (rows of zeros,
+      // infinities or NaN as they are): binary16 queries lose nothing, bfloat16 ones nothing of elements
+      // down to 2^-32 of the largest. (Products with keys beyond 2^100 would overflow.)
       uint32_t packed = 0;
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
@@ -547,9 +548,9 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
       packed = __vmaxu2(packed, __shfl_xor_sync(kFullMask, packed, 2));
       const uint32_t largest = __float_as_uint(unpack_pair<T>(max(packed & 0xffffu, packed >> 16)).x);
       uint32_t field = largest >> 23;
-      field = field == 0 || field == 255 ? 131 : min(max(field, 8u), 250u);
-      float scale = __uint_as_float((258u - field) << 23);
-      float back = a.scale_log2 * __uint_as_float((field - 4u) << 23);
+      field = field == 0 || field == 255 ? 142 : max(field, 16u);
+      float scale = __uint_as_float((269u - field) << 23);
+      float back = a.scale_log2 * __uint_as_float((field - 15u) << 23);
       if (back < 0x1p-126f) {  // below binary32's normal numbers: scores of 0 (a factor of 0 would make NaN of -inf)
         scale = 0.0f;
         back = 1.0f;

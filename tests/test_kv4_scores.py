@@ -47,3 +47,34 @@ def test_the_difference_of_two_scores(dim, kind, heads) -> None:
     tol = dim * 2.0**-24 * size + 2.0**-10 * want.abs() + 2.0**-20
     err = (2 * torch.atanh(out) - want).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ratio", [2.0**10, 2.0**20, 2.0**24])
+def test_small_queries_that_meet_large_keys(ratio, dtype) -> None:
+    """One group's queries are 1 / ratio of the other's and its keys ratio times as large: both count alike."""
+    from pck.cuda import kv4_append, kv4_attention, kv4_cache
+
+    n, dim = 200, 128
+    gen = torch.Generator().manual_seed(9)
+    k = torch.randn(n, 2, 1, dim, generator=gen) * 2.0**-10
+    k[..., 64:] *= ratio
+    v = torch.ones(n, 2, 1, dim)
+    v[:, 1] = -1
+    cache = kv4_cache(n, 16, 1, dim)
+    slots = (16 * torch.arange(n)[:, None] + torch.arange(2)).reshape(-1)
+    kv4_append(cache, k.view(-1, 1, dim).cuda(), v.view(-1, 1, dim).cuda(), slots.cuda())
+    keys = ref.cache_values(cache.cpu())[0][:, :2, 0]
+    q = torch.randn(n, 1, dim, generator=gen) * 2.0**10
+    q[..., 64:] /= ratio
+    q = q.to(dtype)
+    table, lens = torch.arange(n, dtype=torch.int32)[:, None], torch.full((n,), 2, dtype=torch.int32)
+    out = kv4_attention(q.cuda(), cache, table.cuda(), lens.cuda(), scale=2.0**-7).cpu().double()[..., 0]
+    scores = torch.einsum("nhc,ntc->nht", q.double(), keys) * 2.0**-7
+    size = torch.einsum("nhc,ntc->nh", q.double().abs(), keys.abs()) * 2.0**-7
+    want = torch.tanh((scores[..., 0] - scores[..., 1]) / 2)
+    # the difference's tolerance, halved by tanh's slope, and the rounding of the output and of the two values
+    unit = 2.0**-8 if dtype is torch.bfloat16 else 2.0**-11
+    tol = dim * 2.0**-24 * size / 2 + unit * want.abs() + 2.0**-20
+    err = (out - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
