@@ -22,10 +22,10 @@
 //     rounding of a bfloat16 output), each row's and group's times a power of two that follows the
 //     largest p s met so far: that one lies in 2 to 2^15, so what the smallest lose is at most 2^-26
 //     of it. The size of a scale whose token has no weight is of no account.
-//   - The running maximum is a whole number (of log2) and is raised only when a score passes it by
-//     2^8 (weights then stay within 2^8), so the accumulators are rarely rescaled and the common
-//     tile needs no exchange between lanes for it. Raising it lowers all p s met so far, and with
-//     them the power of two, by the same factor: the products with the values stay as they are.
+//   - The running maximum is raised only when a score passes it by 2^8 (weights then stay within
+//     2^8, and that of a row's first maximum, which is mostly its last, is 1, so that its p s is exact),
+//     so the accumulators are rarely rescaled and the common tile needs no exchange between lanes for
+//     it. Raising it lowers all p s met so far: the power of two takes the whole powers of that.
 //   - Work is cut by the lengths, on the device. With few (request, head, row block) items a CTA takes
 //     an equal piece of one of them; with many, the tiles of all items form one line that is cut into
 //     equal parts, a CTA each, so one long request among short ones takes no longer than the rest. A
@@ -706,16 +706,17 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
 #pragma unroll
             for (int j = 1; j < kJ; ++j) m = fmaxf(m, s[n][j][e]);
             const float old = limit[n][e] == -INFINITY ? -INFINITY : top[n][e];
-            m = fmaxf(old, ceilf(m * factor[n][e]));
+            m = fmaxf(old, m * factor[n][e]);
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 4));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
             m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16));
             top[n][e] = m == -INFINITY ? 0.0f : m;
             limit[n][e] = (m + kRaise) / factor[n][e];
             if (fresh) continue;  // the sums are zeros
-            // How far it rises (0 without a maximum; more than any product has bits is as good as all).
-            const int by = min(__float2int_rn(m - old), 512);
-            const float keep = power(-by);
+            // How far it rises, and by how many whole powers (more than any product has bits is as good as all).
+            const float rise = old == m ? 0.0f : m - old;
+            const int by = min(__float2int_rd(rise), 512);
+            const float keep = exp2_fast(-rise);
             total_w[n][e] *= keep;
 #pragma unroll
             for (int g = 0; g < kG; ++g) {
@@ -723,7 +724,7 @@ __global__ void __launch_bounds__(kAttnThreads, Shape<T, kDim, kRows>::kCtas)
               const int field = unit_field(unit[n][g], e), next = min(field + by, kUnitMost);
               set_unit_field(unit[n][g], e, next);
               unit_most[g] = fmaxf(unit_most[g], power(next - kUnitBias));
-              const float rest = power(next - field - by);  // 1 but where the unit can grow no further
+              const float rest = exp2_fast(by - rise) * power(next - field - by);  // (1 to 1/2, if the unit can grow so far)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 acc[n][g][i][e] *= rest;
