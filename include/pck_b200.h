@@ -55,7 +55,7 @@ extern "C" {
 /* Message of the last failing call on this thread ("" if none). */
 const char* pck_last_error(void);
 
-/* ABI version of this library (increases when a declaration here changes, not when one is added): 6. */
+/* ABI version of this library (increases when a declaration here changes): 6. */
 int pck_abi_version(void);
 
 /*
@@ -69,7 +69,8 @@ const char* pck_source_digest(void);
 /*
  * Device status word shared by every kernel of the library: bit 0 = a bounded wait gave up
  * (the result of that launch is not valid); bit 1 = an index in device memory was out of range
- * (serving operators; the access was left out). Synchronizes the current device, stores the
+ * (serving operators only; the access was left out, and no other result is touched). A caller that
+ * asks for lost results looks at bit 0. Synchronizes the current device, stores the
  * word in *status and, if `clear`, resets it.
  */
 int pck_device_status(unsigned int* status, int clear);

@@ -32,9 +32,10 @@
 //     part of an item leaves its sums in scratch memory and a second kernel (a programmatic dependent)
 //     joins them. A CTA's four warps take pairs of tiles in turn, each through its own ring of bulk
 //     copies.
-// Measured with 32 query heads over 8 of dim 128, bfloat16: two requests of 262,143 tokens 140 us (604 MB at
-// 4.3 TB/s), 64 requests of 300 to 16,384 tokens 108 us, one of 1,027 tokens 11 us. A long request is bound
-// by instructions: 295 a tile, 129 cycles of an SM, and as long when every tile comes from L2.
+// Measured with 32 query heads over 8 of dim 128, bfloat16: two requests of 262,143 tokens 142 us (604 MB at
+// 4.3 TB/s), 64 requests of 300 to 16,384 tokens 116 us, one of 1,027 tokens 12 us. Long requests in pages of 64
+// tokens are bound by instructions: 335 a tile, 130 cycles of an SM, and as long when every tile comes from L2.
+// That explains 65 us of the 64 ragged requests'; segments that begin and end in a CTA are the likely rest.
 #include <algorithm>
 
 #include "kv4_layout.cuh"
@@ -120,6 +121,7 @@ __device__ __forceinline__ Cut cut_line(const AttentionArgs& a, int64_t total) {
   return {parts, length, total - length * parts};
 }
 
+// 2^x to 2^-22 of itself, 0 below 2^-126: a weight is rounded to 2^-11 of itself after it.
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -222,8 +224,8 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t*
 }
 
 // CTAs on an SM, by the registers that the rows' products take. Three of 8 rows at dim 128 have room for
-// what four spill (us with three and with four: a batch of 64 ragged requests 111 and 115, two requests of
-// 196,605 tokens 112 and 111, of 16,383 tokens 21 and 23; five: two requests of 196,605 tokens 148).
+// what four spill (us with two, three and four: a batch of 64 ragged requests 142, 116 and 122, two requests of
+// 196,605 tokens 125, 110 and 112, of 16,383 tokens 24, 22 and 25).
 constexpr int attention_ctas(int rows, int dim) {
   if (dim == 64) return rows <= 16 ? 4 : 2;
   if (dim == 128) return rows <= 16 ? 3 : 2;

@@ -2,10 +2,11 @@
 // written as the binary32 logits that the sampler and the membership check take.
 //
 // The floor is memory: the logits are read once and written once (64 rows of 128,256, binary32, histories to
-// 9,000 tokens: 22 us against 10.5; the marks' reads after the pass are the rest). Two kernels, since few
+// 9,000 tokens: 25 us against 10.5). Of the marks' CTAs 296 run at once, for their shared memory, so the second
+// turn of 512 counts after the pass. Two kernels, since few
 // tokens of a row are in its history or its biases and what they need is a chain of dependent reads:
 //   - the pass writes every logit, or -inf by the mask, at the memory's rate, and looks at nothing else;
-//   - the marks, a programmatic dependent that counts while the pass runs: a CTA takes 16,384 tokens of
+//   - the marks, a programmatic dependent that may count beside the pass's end: a CTA takes 16,384 tokens of
 //     a row's vocabulary, reads the row's history, and keeps a word of counts for each of its tokens in
 //     shared memory (integer atomics: their order does not matter) and a list of those that it met. Then
 //     it waits for the pass and computes the listed tokens' logits; biases are added after that, the last

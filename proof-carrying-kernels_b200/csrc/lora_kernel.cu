@@ -687,10 +687,12 @@ cudaError_t launch_rank(const LoraArgs& a, int tiles, int items, int ctas, cudaS
 // that (4096 x 4096, 48 adapters of rank 64, us with eight and with four: 1 row 10.7 and 14.6, 32 rows 15.8
 // and 15.5, 64 rows 18.2 and 19.4, 128 rows 29.5 and 21.8; of rank 16: 7.3 and 10.6, 8.7 and 10.5, 10.6
 // and 12.1, 17.7 and 13.5).
-// More are taken as prompts: two items of a tile at a time (it rarely meets more), and as many CTAs an item
-// as run at once; 64 ranks a launch, the later ones adding to out: the sums of 64 rows and more ranks leave
-// an SM one CTA and its registers no room for loads in flight (2,000 rows of rank 100: 145 us so, 125 us in
-// two launches).
+// (256 rows of one adapter of rank 16, 16 groups: 17 us.)
+// More are taken as prompts: two items of a tile at a time, and as many CTAs an item as run at once. That is
+// made for runs of one adapter; rows that mix adapters take a tile's items in turn (rows of 48 adapters of
+// rank 16: 256 in 21 us, 257 in 291; 257 of one adapter 17). 64 ranks a launch, the later ones adding to
+// out: the sums of 64 rows and more ranks leave an SM one CTA and its registers no room for loads in flight
+// (2,000 rows of rank 100: 145 us so, 125 us in two launches).
 template <typename T, bool kWhole>
 cudaError_t launch_tokens(LoraArgs a, cudaStream_t s) {
   if (a.tokens <= kLoraThreads) {

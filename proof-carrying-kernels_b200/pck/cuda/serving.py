@@ -6,9 +6,10 @@ path (the projections' checks and the membership check stay what they are).
 
 Every function makes one call of the C ABI on the current stream, without synchronizing, and can
 be captured in a CUDA graph. It calls the library directly, as the launch objects of
-`pck.cuda.plan` do, to keep the host cost of a decode step low; the same calls are registered as
-`torch.ops.pck.kv4_append`, `kv4_attention`, `lora_add` and `process_logits` for tracing. Shapes,
-types and strides are checked here, indices in device memory by the kernels (`device_status`, bit 1).
+`pck.cuda.plan` do, to keep the host cost of a decode step low. For tracing, `torch.ops.pck.kv4_append`,
+`kv4_attention`, `lora_add` and `process_logits` are the same operators without `out`, and the append
+without `values`. Shapes, types and strides are checked here, indices in device memory by the kernels
+(`device_status`, bit 1).
 """
 
 from __future__ import annotations
@@ -378,7 +379,7 @@ def process_logits(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, 
     return out
 
 
-# -- the same calls as PyTorch operators -----------------------------------------------
+# -- the operators as PyTorch custom operators (no `out`, no `values`) -------------------
 
 
 @torch.library.custom_op("pck::kv4_append", mutates_args=("cache",))
